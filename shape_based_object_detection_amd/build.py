@@ -4,7 +4,8 @@
 
 Compile flags that matter for parity: ``-ffp-contract=off`` (no FMA contraction: every
 IoU / threshold expression rounds like the reference's separate torch kernels) and the
-default IEEE fp32 division.
+default IEEE fp32 division.  ``-packed-fp32-ops``: no packed fp32 instructions (some of their
+forms have given wrong results on these GPUs now and then).
 
 Also builds ``lib/_sbodcall*.so``: a CPython extension (gcc, generated from ``_lib.SIGNATURES``)
 with one METH_FASTCALL wrapper per int-returning entry point of include/sbod.h.  It calls the
@@ -31,7 +32,8 @@ RESOURCES = os.path.join(PKG, 'lib', 'kernel_resources.json')
 ARCH = os.environ.get('SBOD_OFFLOAD_ARCH', 'gfx950')
 
 CXXFLAGS = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=' + ARCH, '-ffp-contract=off',
-            '-munsafe-fp-atomics', '-Wall', '-Wno-unused-function', '-I', INCLUDE, '-I', CSRC]
+            '-munsafe-fp-atomics', '-Wall', '-Wno-unused-function', '-I', INCLUDE, '-I', CSRC,
+            '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def hipcc():
