@@ -217,7 +217,7 @@ int sbod_codec_f32(int op, const float *in, const float *priors, int64_t n, int6
  * Workspace: sbod_loss_workspace_bytes(B, P). */
 enum { SBOD_REG_SMOOTHL1 = 0, SBOD_REG_L1 = 1, SBOD_REG_DIOU = 2 };
 enum { SBOD_CLS_FOCAL = 0, SBOD_CLS_CE = 1 };
-enum { SBOD_DT_F32 = 0, SBOD_DT_BF16 = 1 };
+enum { SBOD_DT_F32 = 0, SBOD_DT_BF16 = 1, SBOD_DT_F16 = 2 /* label-vocabulary operators only */ };
 enum { SBOD_LOSS_FOCAL_NORM = 4, SBOD_POOL_NONPOS = 0, SBOD_POOL_NEG = 8,
        SBOD_POOL_GLOBAL_NEG = 16, SBOD_POOL_NONPOS_NOT_EASY = 32 };
 size_t sbod_loss_workspace_bytes(int B, int P);
@@ -466,6 +466,66 @@ int sbod_map_f32(const float *det_boxes, const int64_t *det_labels, const float 
                  const uint8_t *true_difficulties, const int32_t *true_offsets, int B, int C,
                  int64_t n_det, int64_t n_true, double threshold, const float *recall_thresholds,
                  float *ap, float *mean_ap, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------- label vocabularies
+ * Operators over the class logits [N, V] and the label table [V, D] of a detector whose labels form a
+ * vocabulary (open-vocabulary classes, detectors that answer label by label); the reference has none.
+ * dtype: SBOD_DT_F32, SBOD_DT_BF16 or SBOD_DT_F16, computed in 32 bits and rounded once.  Rows start
+ * `ld` elements apart (ld >= V) at any alignment; ids are int32 or (ids64 != 0) int64, and an id
+ * outside [0, V) is an absent entry.  Nothing is accumulated with floating-point atomics: the same
+ * call gives the same bits.  A workspace belongs to one call at a time. */
+
+/* Distillation from a teacher's K kept logits per row (ids, top [N, K] contiguous, 1 <= K <= 1024),
+ * at temperature T:  p = softmax(top / T) over a row's entries, or with lse [N] (the teacher's
+ * log sum exp(logits / T) over its whole vocabulary) p = exp(top / T - lse) and one bucket for the
+ * mass outside the kept labels;  row = weights_row T^2 KL(p || softmax(logits / T)).  An entry listed
+ * twice adds its masses.  A row of weight 0, without an entry, or whose logits are all -inf gives
+ * loss 0 and a zero gradient, whatever else it holds.
+ *   rows [N] (reduction NONE): the row losses; loss, norm [1] (MEAN, SUM): the reduced loss and the factor
+ *   on each row's gradient (1 / sum of weights, 1 / N or 1; MEAN over weights that sum to 0 gives 0);
+ *   stats [sbod_distill_stat_floats(), per row]: kept for the gradient.
+ * fwd with grad != NULL (a reduction) also writes the gradient at upstream 1; bwd computes it for
+ * upstream [1] (a reduction) or [N] (NONE), and with skip_if_one != 0 leaves grad as it is where
+ * *upstream is 1 (grad then holds what fwd wrote). */
+enum { SBOD_REDUCE_NONE = 0, SBOD_REDUCE_MEAN = 1, SBOD_REDUCE_SUM = 2 };
+int sbod_distill_stat_floats(void);
+size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int dtype);
+int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids, int ids64,
+                     const void *top, int top_dtype, int k, const float *lse, const float *weights,
+                     float temperature, int reduction, float *rows, float *loss, float *norm, float *stats,
+                     void *grad, int64_t grad_ld, void *workspace, size_t workspace_bytes, void *stream);
+int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids, int ids64,
+                     const void *top, int top_dtype, int k, const float *lse, const float *weights,
+                     float temperature, int reduction, const float *norm, const float *stats,
+                     const float *upstream, int skip_if_one, void *grad, int64_t grad_ld, void *stream);
+
+/* Penalties, biases and masks on logits before a label is chosen.  history [N, history_cols] (row
+ * stride history_ld, 0: one row for all): a row's first history_len entries count (NULL: all), of
+ * them the first prompt_len were given, the others answered.  In this order:
+ *   x / r where x > 0, else x r, for a label in the history;  - frequency count - presence [count > 0],
+ *   count over the answered entries;  + bias (row stride bias_ld, 0: one row);  + the listed biases
+ *   (bias_ids, bias_values [N, bias_cols]; a label listed twice adds both, in order);
+ *   -inf where the mask is 0 (SBOD_MASK_BITS: int32 words, label v in bit v % 32 of word v / 32;
+ *   SBOD_MASK_BYTES: one byte per label; row stride mask_ld in words / bytes, 0: one row).
+ * repetition, presence, frequency: [N], or NULL for the value given for all.  out may be logits. */
+enum { SBOD_MASK_NONE = 0, SBOD_MASK_BITS = 1, SBOD_MASK_BYTES = 2 };
+int sbod_logits_process(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *history,
+                        int history64, int64_t history_cols, int64_t history_ld, const int32_t *history_len,
+                        const int32_t *prompt_len, const float *repetition, const float *presence,
+                        const float *frequency, float repetition_all, float presence_all, float frequency_all,
+                        const void *bias, int bias_dtype, int64_t bias_ld, const void *bias_ids, int bias_ids64,
+                        const float *bias_values, int bias_cols, int64_t bias_ids_ld, int64_t bias_values_ld,
+                        const void *mask, int mask_kind, int64_t mask_ld, void *out, int64_t out_ld, void *stream);
+
+/* out [N, D] = scale table[ids] (an absent id: zeros), and d table [V, D] = scale sum of grad's rows of
+ * each label, added in 32 bits in ascending position, zeros where none came; `padding` (-1: none) is a
+ * label that gets no gradient.  table, out, grad, grad_table are contiguous. */
+int sbod_embed_fwd(const void *table, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,
+                   float scale, void *out, void *stream);
+size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v);
+int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,
+                   int64_t padding, float scale, void *grad_table, void *workspace, size_t workspace_bytes,
+                   void *stream);
 
 #ifdef __cplusplus
 }

@@ -85,6 +85,16 @@ SIGNATURES = {
     'sbod_dcn_fwd_f32': (I32, [P, P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, P, P, SZ, P]),
     'sbod_dcn_bwd_f32': (I32, [P, P, P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, P, P, P, P,
                                P, SZ, P]),
+    'sbod_distill_stat_floats': (I32, []),
+    'sbod_distill_workspace_bytes': (SZ, [I64, I64, I32]),
+    'sbod_distill_fwd': (I32, [P, I32, I64, I64, I64, P, I32, P, I32, I32, P, P, F32, I32, P, P, P, P, P, I64, P,
+                               SZ, P]),
+    'sbod_distill_bwd': (I32, [P, I32, I64, I64, I64, P, I32, P, I32, I32, P, P, F32, I32, P, P, P, I32, P, I64, P]),
+    'sbod_logits_process': (I32, [P, I32, I64, I64, I64, P, I32, I64, I64, P, P, P, P, P, F32, F32, F32, P, I32, I64,
+                                  P, I32, P, I32, I64, I64, P, I32, I64, P, I64, P]),
+    'sbod_embed_fwd': (I32, [P, I32, I64, I64, P, I32, I64, F32, P, P]),
+    'sbod_embed_bwd_workspace_bytes': (SZ, [I64, I64]),
+    'sbod_embed_bwd': (I32, [P, I32, I64, I64, P, I32, I64, I64, F32, P, P, SZ, P]),
 }
 
 # Constants of include/sbod.h.
@@ -95,6 +105,9 @@ CODEC = dict(xy_to_cxcy=0, cxcy_to_xy=1, encode_tenfive=2, decode_tenfive=3, enc
 REG = dict(smoothl1=0, l1=1, diou=2)
 CLS = dict(focal=0, ce=1)
 DT_F32, DT_BF16 = 0, 1
+LABEL_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+REDUCE = dict(none=0, mean=1, sum=2)
+MASK_NONE, MASK_BITS, MASK_BYTES = 0, 1, 2
 LOSS_FOCAL_NORM = 4
 LOSS_DEFER_MINING = 64
 LOSS_WS_ZEROED = 128

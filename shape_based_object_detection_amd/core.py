@@ -3,6 +3,8 @@
 Everything here runs on ROCm device tensors; inputs on the CPU are rejected.  No call in this
 module synchronises with the host unless its docstring says so.
 """
+import contextlib
+
 import numpy as np
 import torch
 
@@ -1175,3 +1177,341 @@ def deform_conv2d(x, offset, mask_logits, weight, ks=3, padding=1, stride=1):
     c = lambda t: None if t is None else t.contiguous().float()
     return _DeformConv.apply(c(x), c(offset), c(mask_logits), c(weight), int(ks), int(padding),
                              int(stride))
+
+
+# ----------------------------------------------------------------------------- label vocabularies
+def _on_device(t):
+    """Context that makes ``t``'s device current for launches (nothing to do when it is)."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _one_device(what, tensors):
+    dev = tensors[0].device
+    for t in tensors[1:]:
+        if t.device != dev:
+            raise RuntimeError('%s: tensors on %s and %s' % (what, dev, t.device))
+
+
+def _constant(what, name, t):
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
+        raise ValueError('%s: %s requires a gradient, which is not computed: detach() it' % (what, name))
+
+
+def _integral(what, name, t):
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
+        raise TypeError('%s: %s must be int32 or int64, got %s' % (what, name, t.dtype))
+
+
+def _rows_of(t):
+    """A 2-d tensor whose rows are contiguous and do not overlap: itself, or a copy."""
+    if t.stride(1) == 1 or t.shape[1] <= 1:
+        if t.shape[0] <= 1 or t.stride(0) >= t.shape[1]:
+            return t
+    return t.contiguous()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _empty_rows(t):
+    """An uninitialised tensor like ``t`` [N, V] whose rows start at the same distance from a 16-byte boundary as
+    t's do, so that a kernel can write its granules as it read t's.  Contiguous where t is."""
+    n, v = t.shape
+    per = 16 // t.element_size()
+    shift = (t.data_ptr() % 16) // t.element_size()
+    ld = v + (_row_stride(t) - v) % per
+    if shift == 0 and ld == v:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return torch.empty(n * ld + shift, dtype=t.dtype, device=t.device).as_strided((n, v), (ld, 1), shift)
+
+
+def distill_arguments(logits, ids, top, lse, weights, temperature, reduction):
+    """The checks of ``topk_distill_loss``."""
+    what = 'topk_distill_loss'
+    if not logits.is_floating_point() or not top.is_floating_point():
+        raise TypeError('%s: logits of %s, teacher_logits of %s' % (what, logits.dtype, top.dtype))
+    _integral(what, 'teacher_ids', ids)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError('%s: logits %s have no labels' % (what, tuple(logits.shape)))
+    if ids.shape != top.shape or ids.dim() != logits.dim() or ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError('%s: logits %s, teacher_ids %s, teacher_logits %s'
+                         % (what, tuple(logits.shape), tuple(ids.shape), tuple(top.shape)))
+    if not 1 <= ids.shape[-1] <= 1024:
+        raise ValueError('%s: %d kept labels per row (1..1024)' % (what, ids.shape[-1]))
+    for name, t in (('teacher_lse', lse), ('weights', weights)):
+        if t is not None and t.shape != logits.shape[:-1]:
+            raise ValueError('%s: %s %s for logits %s' % (what, name, tuple(t.shape), tuple(logits.shape)))
+    if not 0.0 < float(temperature) < float('inf'):
+        raise ValueError('%s: temperature %s' % (what, temperature))
+    if reduction not in L.REDUCE:
+        raise ValueError('%s: reduction %r (mean, sum or none)' % (what, reduction))
+    _constant(what, 'teacher_logits', top)
+    _constant(what, 'teacher_lse', lse)
+    _constant(what, 'weights', weights)
+
+
+class _TopKDistill(torch.autograd.Function):
+    """Forward writes the loss and, at upstream 1, the gradient (the logits are read once); backward leaves it as it is
+    where the upstream gradient is 1 and computes it anew, rounded once, otherwise.  float16 gradients are
+    computed in backward only: at upstream 1 they would underflow before a loss scale reaches them."""
+
+    @staticmethod
+    def forward(ctx, x, ids, top, lse, w, temperature, reduction, want):
+        n, v = x.shape
+        dev = x.device
+        dt, red = L.LABEL_DT[x.dtype], L.REDUCE[reduction]
+        nst = L.lib().sbod_distill_stat_floats()
+        nb = L.lib().sbod_distill_workspace_bytes(n, v, dt)
+        kept = torch.empty(nst * n + 1, dtype=torch.float32, device=dev)   # statistics | the reduction's norm
+        loss = torch.empty((), dtype=torch.float32, device=dev) if red else None
+        rows = None if red else torch.empty(n, dtype=torch.float32, device=dev)
+        grad = _empty_rows(x) if want and red and x.dtype != torch.float16 else None
+        ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=dev)
+        args = (dt, n, v, _row_stride(x), L.ptr(ids), int(ids.dtype == torch.int64), L.ptr(top), L.LABEL_DT[top.dtype],
+                top.shape[1], L.ptr(lse), L.ptr(w), temperature, red)
+        with _on_device(x):
+            L.call('sbod_distill_fwd', L.ptr(x), *args, L.ptr(rows), L.ptr(loss), kept.data_ptr() + 4 * nst * n,
+                   L.ptr(kept), L.ptr(grad), 0 if grad is None else _row_stride(grad), L.ptr(ws), nb, L.stream_of(x))
+        if want:
+            ctx.save_for_backward(x, ids, top, lse, w, kept)
+            ctx.args, ctx.grad = args, grad
+            ctx.set_materialize_grads(False)
+        return loss if red else rows
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        none = (None,) * 7
+        if g is None:
+            return (None,) + none
+        x, ids, top, lse, w, kept = ctx.saved_tensors
+        grad, ctx.grad = ctx.grad, None   # (a second backward of a retained graph computes its own)
+        written = grad is not None
+        if written:
+            u = _UNIT.get(g.device)
+            if u is not None and g.data_ptr() == u.data_ptr():   # unit_grad(): nothing to apply
+                return (grad,) + none
+        else:
+            grad = _empty_rows(x)
+        g = g.detach().to(torch.float32).contiguous()
+        norm = kept.data_ptr() + 4 * (kept.numel() - 1)
+        with _on_device(x):
+            L.call('sbod_distill_bwd', L.ptr(x), *ctx.args, norm, L.ptr(kept), L.ptr(g), int(written),
+                   L.ptr(grad), _row_stride(grad), L.stream_of(x))
+        return (grad,) + none
+
+
+def topk_distill(logits, ids, top, lse, weights, temperature, reduction):
+    """``operators.Loss.topk_distill_loss`` on device tensors (checked by ``distill_arguments``)."""
+    _one_device('topk_distill_loss', [t for t in (logits, ids, top, lse, weights) if t is not None])
+    L.require_device(logits, what='topk_distill_loss')
+    if logits.dtype not in L.LABEL_DT:
+        raise TypeError('topk_distill_loss: logits must be float32, bfloat16 or float16, got %s' % logits.dtype)
+    lead, v, k = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
+    x = _rows_of(logits.reshape(-1, v))
+    ids, top = ids.reshape(-1, k).contiguous(), top.detach().reshape(-1, k).contiguous()
+    if top.dtype not in L.LABEL_DT:
+        top = top.float()
+    lse = None if lse is None else lse.detach().reshape(-1).to(torch.float32).contiguous()
+    w = None if weights is None else weights.detach().reshape(-1).to(torch.float32).contiguous()
+    want = torch.is_grad_enabled() and x.requires_grad
+    r = _TopKDistill.apply(x, ids, top, lse, w, temperature, reduction, want)
+    return r.reshape(lead) if reduction == 'none' else r
+
+
+def logits_arguments(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, bias_ids,
+                     bias_values, allowed, out):
+    """The checks of ``process_logits``; its arguments with every tensor per row or for all rows."""
+    what = 'process_logits'
+    if not logits.is_floating_point():
+        raise TypeError('%s: logits of %s' % (what, logits.dtype))
+    if logits.dim() not in (1, 2) or logits.shape[-1] < 1:
+        raise ValueError('%s: logits %s ([N, V] or [V])' % (what, tuple(logits.shape)))
+    n, v = (1, logits.shape[0]) if logits.dim() == 1 else logits.shape
+    _constant(what, 'logits', logits)
+
+    def rows(name, t, cols=None):
+        if t.dim() not in (1, 2) or (t.dim() == 2 and t.shape[0] != n) or (cols is not None and t.shape[-1] != cols):
+            raise ValueError('%s: %s %s for logits %s' % (what, name, tuple(t.shape), tuple(logits.shape)))
+
+    if history is not None:
+        _integral(what, 'history', history)
+        rows('history', history)
+    for name, t in (('history_len', history_len), ('prompt_len', prompt_len)):
+        if t is None:
+            continue
+        if history is None:
+            raise ValueError('%s: %s without a history' % (what, name))
+        _integral(what, name, t)
+        if t.shape != (n,):
+            raise ValueError('%s: %s %s for %d rows' % (what, name, tuple(t.shape), n))
+    for name, t in (('repetition', repetition), ('presence', presence), ('frequency', frequency)):
+        if torch.is_tensor(t):
+            if not t.is_floating_point() or t.shape != (n,):
+                raise ValueError('%s: %s is a number or a float tensor [%d]' % (what, name, n))
+            _constant(what, name, t)
+    if not torch.is_tensor(repetition) and not 0.0 < float(repetition) < float('inf'):
+        raise ValueError('%s: repetition %s' % (what, repetition))
+    if bias is not None:
+        if bias.dtype not in (torch.float32, logits.dtype):
+            raise TypeError('%s: bias of %s (float32 or %s)' % (what, bias.dtype, logits.dtype))
+        rows('bias', bias, v)
+        _constant(what, 'bias', bias)
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError('%s: bias_ids and bias_values go together' % what)
+    if bias_ids is not None:
+        _integral(what, 'bias_ids', bias_ids)
+        rows('bias_ids', bias_ids)
+        if bias_values.dtype != torch.float32:
+            raise TypeError('%s: bias_values of %s (float32)' % (what, bias_values.dtype))
+        rows('bias_values', bias_values, bias_ids.shape[-1])
+        _constant(what, 'bias_values', bias_values)
+    if allowed is not None:
+        if allowed.dtype == torch.bool:
+            rows('allowed', allowed, v)
+        elif allowed.dtype == torch.int32:
+            rows('allowed', allowed)
+            if allowed.shape[-1] < (v + 31) // 32:
+                raise ValueError('%s: allowed %s for %d labels: %d words are needed'
+                                 % (what, tuple(allowed.shape), v, (v + 31) // 32))
+        else:
+            raise TypeError('%s: allowed of %s (bool, or int32 words)' % (what, allowed.dtype))
+    if out is not None:
+        if out.shape != logits.shape or out.dtype != logits.dtype:
+            raise ValueError('%s: out %s of %s for logits %s of %s'
+                             % (what, tuple(out.shape), out.dtype, tuple(logits.shape), logits.dtype))
+        _constant(what, 'out', out)
+    return (logits, history, history_len, prompt_len, repetition, presence, frequency, bias, bias_ids, bias_values,
+            allowed, out)
+
+
+def _extent(t):
+    """[first, past the last) byte of a tensor's elements."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def process_logits(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, bias_ids, bias_values,
+                   allowed, out):
+    """``operators.Logits.process_logits`` on device tensors (checked by ``logits_arguments``)."""
+    what = 'process_logits'
+    tensors = [t for t in (logits, history, history_len, prompt_len, repetition, presence, frequency, bias, bias_ids,
+                           bias_values, allowed, out) if torch.is_tensor(t)]
+    _one_device(what, tensors)
+    L.require_device(logits, what=what)
+    if logits.dtype not in L.LABEL_DT:
+        raise TypeError('%s: logits must be float32, bfloat16 or float16, got %s' % (what, logits.dtype))
+    x = logits if logits.dim() == 2 else logits[None]
+    n, v = x.shape
+    x = _rows_of(x)
+    if out is None:
+        dst = _empty_rows(x)
+        result = dst if logits.dim() == 2 else dst[0]
+    else:
+        dst = result = out
+        if out.dim() == 1:
+            dst = out[None]
+        if (v > 1 and dst.stride(1) != 1) or (n > 1 and dst.stride(0) < v):
+            raise ValueError('%s: the rows of out must be contiguous and apart, strides %s' % (what, tuple(out.stride())))
+        same = dst.data_ptr() == x.data_ptr() and _row_stride(dst) == _row_stride(x)
+        for t in tensors:
+            if t is out or (same and t is logits):
+                continue
+            a, b = _extent(t), _extent(out)
+            if a[0] < b[1] and b[0] < a[1]:
+                raise ValueError('%s: out overlaps another argument in memory (it may be the logits themselves)' % what)
+
+    def per_row(t):   # (tensor, row stride): 0 where one row serves all
+        if t is None:
+            return None, 0
+        if t.dim() == 1:
+            t = t.contiguous()
+            return t, 0
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            t = t.contiguous()
+        return t, t.stride(0)
+
+    def scalar(t):
+        return (t.to(torch.float32).contiguous(), 0.0) if torch.is_tensor(t) else (None, float(t))
+
+    def lens(t):
+        return None if t is None else t.to(torch.int32).contiguous()
+
+    history, ldh = per_row(history)
+    bias, ldb = per_row(bias)
+    bias_ids, ldi = per_row(bias_ids)
+    bias_values, ldv = per_row(bias_values)
+    allowed, ldm = per_row(allowed)
+    history_len, prompt_len = lens(history_len), lens(prompt_len)
+    (rep, rep1), (pres, pres1), (freq, freq1) = scalar(repetition), scalar(presence), scalar(frequency)
+    kind = L.MASK_NONE if allowed is None else L.MASK_BYTES if allowed.dtype == torch.bool else L.MASK_BITS
+    with _on_device(x):
+        L.call('sbod_logits_process', L.ptr(x), L.LABEL_DT[x.dtype], n, v, _row_stride(x), L.ptr(history),
+               int(history is not None and history.dtype == torch.int64), 0 if history is None else history.shape[-1], ldh,
+               L.ptr(history_len), L.ptr(prompt_len), L.ptr(rep), L.ptr(pres), L.ptr(freq), 1.0 if rep is not None else rep1,
+               pres1, freq1, L.ptr(bias), 0 if bias is None else L.LABEL_DT[bias.dtype], ldb, L.ptr(bias_ids),
+               int(bias_ids is not None and bias_ids.dtype == torch.int64), L.ptr(bias_values),
+               0 if bias_ids is None else bias_ids.shape[-1], ldi, ldv, L.ptr(allowed), kind, ldm, L.ptr(dst),
+               _row_stride(dst), L.stream_of(x))
+    return result
+
+
+def embedding_arguments(ids, weight, scale, padding_idx):
+    """The checks of ``scaled_embedding``; the padding id counted from the front (-1: none)."""
+    what = 'scaled_embedding'
+    _integral(what, 'ids', ids)
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError('%s: weight %s of %s ([V, D] of a floating type)' % (what, tuple(weight.shape), weight.dtype))
+    v = weight.shape[0]
+    if ids.numel() and v == 0:
+        raise ValueError('%s: ids for an empty table' % what)
+    if not abs(float(scale)) < float('inf'):
+        raise ValueError('%s: scale %s' % (what, scale))
+    if padding_idx is None:
+        return -1
+    if not -v <= padding_idx < v:
+        raise ValueError('%s: padding_idx %d for %d rows' % (what, padding_idx, v))
+    return padding_idx % v
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, pad):
+        v, d = weight.shape
+        out = torch.empty(ids.shape + (d,), dtype=weight.dtype, device=weight.device)
+        wide = int(ids.dtype == torch.int64)
+        with _on_device(weight):
+            L.call('sbod_embed_fwd', L.ptr(weight), L.LABEL_DT[weight.dtype], v, d, L.ptr(ids), wide, ids.numel(), scale,
+                   L.ptr(out), L.stream_of(weight))
+        ctx.save_for_backward(ids)
+        ctx.args = (v, d, wide, scale, pad)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        v, d, wide, scale, pad = ctx.args
+        g = g.contiguous()
+        n = ids.numel()
+        grad = torch.empty(v, d, dtype=g.dtype, device=g.device)
+        nb = L.lib().sbod_embed_bwd_workspace_bytes(n, v)
+        ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=g.device)
+        with _on_device(g):
+            L.call('sbod_embed_bwd', L.ptr(g), L.LABEL_DT[g.dtype], v, d, L.ptr(ids), wide, n, pad, scale, L.ptr(grad),
+                   L.ptr(ws), nb, L.stream_of(g))
+        return grad, None, None, None
+
+
+def scaled_embedding(ids, weight, scale, pad):
+    """``operators.Embedding.scaled_embedding`` on device tensors (checked by ``embedding_arguments``)."""
+    _one_device('scaled_embedding', [weight, ids])
+    L.require_device(weight, what='scaled_embedding')
+    if weight.dtype not in L.LABEL_DT:
+        raise TypeError('scaled_embedding: weight must be float32, bfloat16 or float16, got %s' % weight.dtype)
+    return _ScaledEmbedding.apply(weight.contiguous(), ids.contiguous(), float(scale), pad)

@@ -1,0 +1,445 @@
+// Distillation from a teacher's top logits (a class vocabulary's knowledge-distillation loss), with
+// its gradient.
+//
+// For a row of student logits x [V] and the teacher's K kept (label, logit) pairs, at temperature T:
+//   q = softmax(x / T);
+//   without lse: p = softmax(t / T) over the kept labels, KL = sum_k p_k (log p_k - log q_k);
+//   with the teacher's lse (log sum exp of its whole row / T): p_k = exp(t_k / T - lse), and the mass
+//   it did not keep, rest = 1 - sum p, is one bucket against the student's mass outside the kept
+//   labels, q_o: KL += rest (log rest - log q_o).
+//   row loss = w T^2 KL;  d/dx_v = w T (q_v - p_v) for a kept label (p summed over its repetitions),
+//   w T q_v for another one, or with a bucket w T (q_o - rest) q_v / q_o.
+//
+// The other labels' sum has a maximum of its own: q_o would underflow, and 1 - sum of the kept q
+// cancel, where the student is sure of a kept label.  The kept labels are gathered by themselves.
+#include "label_dev.h"
+
+namespace sbod {
+namespace label {
+
+constexpr int kMaxTop = 1024;       // kept labels per row
+constexpr int kDistThreads = 256;   // k_distill_part / k_distill_grad
+constexpr int kDistGran = 1024;     // 16-byte granules of a row per item: 4 per thread, 16 KB
+constexpr float kNegInf = -__builtin_inff();
+
+struct DistillArgs {
+  const void *x;          // [n, v], row stride ldx
+  const void *ids;        // [n, k] int32 / int64
+  const void *top;        // [n, k] of top_dt
+  const float *lse;       // [n] or null
+  const float *w;         // [n] or null
+  float *rows;            // [n] row losses (weighted), or for a reduction
+  double *rows64;         // in 64 bits: a mean holds where single rows are beyond float
+  float *stats;           // [n, kStats]
+  float *loss, *norm;     // the reduced loss, and the factor on each row's gradient; null: no reduction
+  float2 *part;           // [n, nchunk] {max, sum} of each chunk
+  void *dx;               // [n, v], row stride lddx
+  const float *up;        // upstream gradient, null for 1
+  int64_t n, v, ldx, lddx, up_stride;
+  int k, ids64, top_dt, nchunk, reduction, skip_one;
+  float t, inv_t, s;      // temperature, 1 / T, log2(e) / T
+  double inv_td;
+};
+
+// What a row leaves for its gradient: q_v = 2^((x - m) s - l2s); another label than the kept ones
+// gets coef 2^((x - mo) s - l2so); p_k = exp((t_k - tb) / T - tl).
+enum { kStM, kStL2s, kStMo, kStL2so, kStCoef, kStTb, kStTl, kStLive, kStats };
+
+__device__ __forceinline__ bool row_has_weight(const DistillArgs &a, int64_t r) { return !a.w || a.w[r] != 0.f; }
+
+__device__ __forceinline__ void put_row(const DistillArgs &a, int64_t r, double loss) {
+  if (a.rows64) a.rows64[r] = loss;
+  else a.rows[r] = static_cast<float>(loss);
+}
+
+// Bits of the kept labels among the elements [e0, e0 + 32 nwords): all threads of the block.
+__device__ __forceinline__ void mark_kept(const DistillArgs &a, int64_t r, int64_t e0, uint32_t *bits, int nwords) {
+  for (int i = threadIdx.x; i < nwords; i += blockDim.x) bits[i] = 0;
+  __syncthreads();
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+    const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
+    const int64_t at = id - e0;
+    if (id >= 0 && at >= 0 && at < 32 * static_cast<int64_t>(nwords)) atomicOr(&bits[at >> 5], 1u << (at & 31));
+  }
+  __syncthreads();
+}
+
+// {max, sum of 2^((x - max) s)} of each chunk of a row; with a bucket, of its labels not kept.
+template <int DT, bool kBucket>
+__global__ __launch_bounds__(kDistThreads) void k_distill_part(DistillArgs a) {
+  using T = typename Elt<DT>::T;
+  constexpr int P = Elt<DT>::P, kPer = kDistGran / kDistThreads;
+  __shared__ uint32_t bits[kBucket ? kDistGran * P / 32 : 1];
+  __shared__ float red[2][kDistThreads / kWave];
+  const int64_t items = a.n * a.nchunk;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t r = it / a.nchunk;
+    if (!row_has_weight(a, r)) continue;
+    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+    const int64_t e0 = (it - r * a.nchunk) * kDistGran * P - row_phase(row);
+    if (kBucket) mark_kept(a, r, e0, bits, kDistGran * P / 32);
+    float f[kPer][P], m = kNegInf;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      ld_granule<DT>(row, e0 + static_cast<int64_t>(i * kDistThreads + threadIdx.x) * P, a.v, kNegInf, f[i]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (kBucket) {
+        const int g = i * kDistThreads + threadIdx.x;
+        const uint32_t b = bits[g * P >> 5] >> (g * P & 31);
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (b >> j & 1) f[i][j] = kNegInf;
+      }
+#pragma unroll
+      for (int j = 0; j < P; ++j) m = fmaxf(m, f[i][j]);
+    }
+    m = wave_max_f32(m);
+    const int wv = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[0][wv] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kDistThreads / kWave; ++i) m = fmaxf(m, red[0][i]);
+    // (a chunk of -inf alone: its terms are 2^-inf = 0; NaN stays NaN)
+    const float base = m == kNegInf ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) sum += exp2_hw((f[i][j] - base) * a.s);
+    sum = wave_sum_f32(sum);
+    if ((threadIdx.x & 63) == 0) red[1][wv] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < kDistThreads / kWave; ++i) sum += red[1][i];
+      a.part[it] = make_float2(m, sum);
+    }
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
+  return v;
+}
+
+// One wave: the teacher's normaliser of a row, p_k = exp((t_k - tb) / T - tl); false without a kept
+// label that has mass.
+__device__ __forceinline__ bool teacher_norm(const DistillArgs &a, int64_t r, int lane, float *tb, float *tl) {
+  if (a.lse) {
+    *tb = 0.f;
+    *tl = a.lse[r];
+    return true;
+  }
+  float tm = kNegInf;
+  for (int k = lane; k < a.k; k += kWave)
+    if (ld_id(a.ids, r * a.k + k, a.ids64, a.v) >= 0) tm = fmaxf(tm, ld_any(a.top, r * a.k + k, a.top_dt));
+  tm = wave_max_f32(tm);
+  const float base = tm == kNegInf ? 0.f : tm;
+  float sum = 0.f;
+  for (int k = lane; k < a.k; k += kWave)
+    if (ld_id(a.ids, r * a.k + k, a.ids64, a.v) >= 0)
+      sum += expf((ld_any(a.top, r * a.k + k, a.top_dt) - base) * a.inv_t);
+  sum = wave_sum_f32(sum);
+  *tb = base;
+  *tl = logf(sum);
+  return !(sum == 0.f);
+}
+
+// (the difference in 64 bits: with lse, t / T and lse are large against it)
+__device__ __forceinline__ float teacher_logp(const DistillArgs &a, int64_t i, float tb, float tl) {
+  return static_cast<float>((static_cast<double>(ld_any(a.top, i, a.top_dt)) - tb) * a.inv_td - tl);
+}
+
+// One wave per row: the chunks joined, the teacher's side, the row's loss and statistics.
+template <int DT, bool kBucket>
+__global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
+  using T = typename Elt<DT>::T;
+  __shared__ int ids_s[kBucket ? 4 : 1][kBucket ? kMaxTop : 1];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  for (int64_t r = blockIdx.x * 4ll + wv; r < a.n; r += gridDim.x * 4ll) {
+    float *st = a.stats + r * kStats;
+    float tb = 0.f, tl = 0.f;
+    bool live = row_has_weight(a, r) && teacher_norm(a, r, lane, &tb, &tl);
+    float mo = kNegInf, so = 0.f;
+    if (live) {
+      for (int c = lane; c < a.nchunk; c += kWave) mo = fmaxf(mo, a.part[r * a.nchunk + c].x);
+      mo = wave_max_f32(mo);
+      for (int c = lane; c < a.nchunk; c += kWave) {
+        const float2 p = a.part[r * a.nchunk + c];
+        so += p.x == kNegInf ? p.y : p.y * exp2_hw((p.x - mo) * a.s);
+      }
+      so = wave_sum_f32(so);
+    }
+    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+    float m = mo, sum = so;
+    int kept = 0;   // different labels kept
+    if (live && kBucket) {
+      for (int k = lane; k < a.k; k += kWave) {
+        const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
+        ids_s[wv][k] = id;
+        if (id >= 0) m = fmaxf(m, static_cast<float>(row[id]));
+      }
+      m = wave_max_f32(m);
+      const float base = m == kNegInf ? 0.f : m;
+      wave_lds_fence();
+      float sk = 0.f;
+      for (int k = lane; k < a.k; k += kWave) {
+        const int id = ids_s[wv][k];
+        bool first = id >= 0;
+        for (int j = 0; j < k && first; ++j) first = ids_s[wv][j] != id;
+        if (first) {
+          sk += exp2_hw((static_cast<float>(row[id]) - base) * a.s);
+          ++kept;
+        }
+      }
+      kept = wave_sum_i32(kept);
+      sum = wave_sum_f32(sk) + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
+      wave_lds_fence();
+    }
+    // a row of -inf alone has no distribution: it is left out, as one of weight 0
+    if (m == kNegInf && sum == 0.f) live = false;
+    if (!live) {
+      if (lane < kStats) st[lane] = 0.f;
+      if (lane == 0) put_row(a, r, 0.0);
+      continue;
+    }
+    const float logs = logf(sum);
+    // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
+    double kl = 0;
+    float mass = 0.f;
+    for (int k = lane; k < a.k; k += kWave) {
+      const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
+      if (id < 0) continue;
+      const float logp = teacher_logp(a, r * a.k + k, tb, tl), p = expf(logp);
+      const double logq = (static_cast<double>(row[id]) - m) * a.inv_td - logs;
+      if (p != 0.f) kl += p * (logp - logq);   // 0 log 0 = 0
+      mass += p;
+    }
+    kl = wave_sum_f64(kl);
+    float coef = 1.f;
+    if (kBucket) {
+      mass = wave_sum_f32(mass);
+      float rest = 1.f - mass;
+      // (no label outside the kept ones: what is left of the teacher's mass is rounding)
+      if (rest < 0.f || kept == a.v) rest = 0.f;
+      const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - m) * a.inv_td + logf(so) - logs;
+      kl += rest > 0.f ? rest * (logf(rest) - logo) : rest;
+      coef = expf(static_cast<float>(logo)) - rest;
+    }
+    if (lane == 0) {
+      st[kStM] = m;
+      st[kStL2s] = log2f(sum);
+      // (no other label with mass: 2^((x - 0) s - 0) is 0 for each of them)
+      st[kStMo] = so == 0.f ? 0.f : mo;
+      st[kStL2so] = so == 0.f ? 0.f : log2f(so);
+      st[kStCoef] = coef;
+      st[kStTb] = tb;
+      st[kStTl] = tl;
+      st[kStLive] = 1.f;
+      put_row(a, r, kl * a.t * a.t * (a.w ? a.w[r] : 1.f));
+    }
+  }
+}
+
+// One block: {loss, norm} of the rows.  Sums in 64 bits, in a fixed order.
+__global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
+  __shared__ double red[16];
+  double sum = 0, w = 0;
+  for (int64_t i = threadIdx.x; i < a.n; i += blockDim.x) {
+    sum += a.rows64[i];
+    if (a.w) w += a.w[i];
+  }
+  sum = block_sum(sum, red);
+  w = a.w ? block_sum(w, red) : static_cast<double>(a.n);
+  if (threadIdx.x == 0) {
+    const double norm = a.reduction == SBOD_REDUCE_MEAN ? (w == 0 ? 0.0 : 1.0 / w) : 1.0;
+    *a.loss = static_cast<float>(norm == 0 ? 0.0 : sum * norm);
+    *a.norm = static_cast<float>(norm);
+  }
+}
+
+// dx of one chunk of a row from the row's statistics.  The kept labels are written a second time,
+// behind a barrier, by a thread each.
+template <int DT>
+__global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
+  using T = typename Elt<DT>::T;
+  constexpr int P = Elt<DT>::P, kPer = kDistGran / kDistThreads;
+  __shared__ int ids_s[kMaxTop];
+  __shared__ float p_s[kMaxTop];
+  if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
+  const int64_t items = a.n * a.nchunk;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t r = it / a.nchunk;
+    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+    T *drow = static_cast<T *>(a.dx) + r * a.lddx;
+    const int phase = row_phase(row);
+    const bool aligned = row_phase(drow) == phase;
+    const int64_t e0 = (it - r * a.nchunk) * kDistGran * P - phase, e1 = e0 + kDistGran * P;
+    const float *st = a.stats + r * kStats;
+    float f[P];
+    if (st[kStLive] == 0.f) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) f[j] = 0.f;
+      for (int i = 0; i < kPer; ++i)
+        st_granule<DT>(drow, e0 + static_cast<int64_t>(i * kDistThreads + threadIdx.x) * P, a.v, aligned, f);
+      continue;
+    }
+    float g = a.t * (a.w ? a.w[r] : 1.f);
+    if (a.norm) g *= *a.norm;
+    if (a.up) g *= a.up[r * a.up_stride];
+    const float mo = st[kStMo], l2so = st[kStL2so], gc = g * st[kStCoef];
+    const float tb = st[kStTb], tl = st[kStTl];
+    for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
+      const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
+      ids_s[k] = id;
+      p_s[k] = id >= 0 ? expf(teacher_logp(a, r * a.k + k, tb, tl)) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t e = e0 + static_cast<int64_t>(i * kDistThreads + threadIdx.x) * P;
+      ld_granule<DT>(row, e, a.v, kNegInf, f);
+#pragma unroll
+      for (int j = 0; j < P; ++j) f[j] = gc * exp2_hw((f[j] - mo) * a.s - l2so);
+      st_granule<DT>(drow, e, a.v, aligned, f);
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
+      const int id = ids_s[k];
+      if (id < 0 || id < e0 || id >= e1) continue;
+      float p = 0.f;
+      for (int j = 0; j < a.k; ++j) p += ids_s[j] == id ? p_s[j] : 0.f;
+      const float q = exp2_hw((static_cast<float>(row[id]) - st[kStM]) * a.s - st[kStL2s]);
+      drow[id] = static_cast<T>(g * (q - p));
+    }
+    __syncthreads();
+  }
+}
+
+int distill_chunks(int64_t v, int dt) {
+  const int64_t per = static_cast<int64_t>(kDistGran) * 16 / elt_bytes(dt);
+  return static_cast<int>((v + 16 / elt_bytes(dt) - 1 + per - 1) / per);   // (a phase of P - 1 at most)
+}
+
+// A grid that walks `items`: enough workgroups for every CU many times over, far below the launch limit.
+unsigned grid_for(int64_t items) { return static_cast<unsigned>(items < 65536 ? items : 65536); }
+
+int launch_grad(const DistillArgs &a, int dt, hipStream_t s) {
+  const dim3 grid(grid_for(a.n * a.nchunk)), block(kDistThreads);
+  if (dt == SBOD_DT_F32)
+    hipLaunchKernelGGL(k_distill_grad<SBOD_DT_F32>, grid, block, 0, s, a);
+  else if (dt == SBOD_DT_BF16)
+    hipLaunchKernelGGL(k_distill_grad<SBOD_DT_BF16>, grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL(k_distill_grad<SBOD_DT_F16>, grid, block, 0, s, a);
+  SBOD_LAUNCHED("k_distill_grad");
+  return SBOD_OK;
+}
+
+template <int DT, bool kBucket>
+int launch_rows(const DistillArgs &a, hipStream_t s) {
+  hipLaunchKernelGGL((k_distill_part<DT, kBucket>), dim3(grid_for(a.n * a.nchunk)), dim3(kDistThreads), 0, s, a);
+  SBOD_LAUNCHED("k_distill_part");
+  hipLaunchKernelGGL((k_distill_join<DT, kBucket>), dim3(grid_for((a.n + 3) / 4)), dim3(256), 0, s, a);
+  SBOD_LAUNCHED("k_distill_join");
+  return SBOD_OK;
+}
+
+int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, int64_t ldx, const void *ids,
+                 const void *top, int top_dt, int k, float temperature, int reduction) {
+  SBOD_REQUIRE(known_dt(dt) && known_dt(top_dt), "%s: dtype %d / %d", what, dt, top_dt);
+  SBOD_REQUIRE(n >= 0 && v >= 1 && v < (1ll << 31) - 65536 && ldx >= v, "%s: logits [%lld, %lld] with row stride %lld",
+               what, static_cast<long long>(n), static_cast<long long>(v), static_cast<long long>(ldx));
+  SBOD_REQUIRE(k >= 1 && k <= kMaxTop, "%s: %d kept labels per row (1..%d)", what, k, kMaxTop);
+  SBOD_REQUIRE(n < (1ll << 40) / v, "%s: %lld rows of %lld labels", what, static_cast<long long>(n), static_cast<long long>(v));
+  SBOD_REQUIRE(temperature > 0.f && temperature < __builtin_inff(), "%s: temperature %g", what, temperature);
+  SBOD_REQUIRE(reduction >= SBOD_REDUCE_NONE && reduction <= SBOD_REDUCE_SUM, "%s: reduction %d", what, reduction);
+  SBOD_REQUIRE(n == 0 || (x && ids && top), "%s: null tensor", what);
+  return SBOD_OK;
+}
+
+void set_temperature(DistillArgs &a, float t) {
+  a.t = t;
+  a.inv_td = 1.0 / t;
+  a.inv_t = static_cast<float>(a.inv_td);
+  a.s = static_cast<float>(a.inv_td * 1.44269504088896340736);
+}
+
+}  // namespace label
+}  // namespace sbod
+
+using namespace sbod;
+using namespace sbod::label;
+
+extern "C" int sbod_distill_stat_floats(void) { return kStats; }
+
+extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int dtype) {
+  if (n <= 0 || v <= 0 || !known_dt(dtype)) return 0;
+  return align_up(static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2)) + static_cast<size_t>(n) * sizeof(double);
+}
+
+extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
+                                int ids64, const void *top, int top_dtype, int k, const float *lse,
+                                const float *weights, float temperature, int reduction, float *rows, float *loss,
+                                float *norm, float *stats, void *grad, int64_t grad_ld, void *workspace, size_t workspace_bytes,
+                                void *stream) {
+  const int bad = check_common("sbod_distill_fwd", logits, dtype, n, v, ld, ids, top, top_dtype, k, temperature, reduction);
+  if (bad != SBOD_OK) return bad;
+  SBOD_REQUIRE(n == 0 || ((rows || reduction != SBOD_REDUCE_NONE) && stats), "sbod_distill_fwd: null output");
+  SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || (loss && norm), "sbod_distill_fwd: a reduction needs loss and norm");
+  SBOD_REQUIRE(!grad || (grad_ld >= v && reduction != SBOD_REDUCE_NONE), "sbod_distill_fwd: gradient with row stride %lld, reduction %d",
+               static_cast<long long>(grad_ld), reduction);
+  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, dtype) || (n > 0 && !workspace)) {
+    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, dtype));
+    return SBOD_E_WORKSPACE;
+  }
+  hipStream_t s = as_stream(stream);
+  DistillArgs a = {};
+  a.x = logits, a.n = n, a.v = v, a.ldx = ld, a.ids = ids, a.ids64 = ids64, a.top = top, a.top_dt = top_dtype;
+  a.k = k, a.lse = lse, a.w = weights, a.rows = rows, a.stats = stats, a.reduction = reduction;
+  a.part = static_cast<float2 *>(workspace), a.nchunk = distill_chunks(v, dtype);
+  if (reduction != SBOD_REDUCE_NONE) {
+    a.loss = loss, a.norm = norm;
+    a.rows64 = ws_at<double>(workspace, align_up(static_cast<size_t>(n) * a.nchunk * sizeof(float2)));
+  }
+  a.dx = grad, a.lddx = grad_ld;
+  set_temperature(a, temperature);
+  if (n > 0) {
+    int st;
+    if (dtype == SBOD_DT_F32)
+      st = lse ? launch_rows<SBOD_DT_F32, true>(a, s) : launch_rows<SBOD_DT_F32, false>(a, s);
+    else if (dtype == SBOD_DT_BF16)
+      st = lse ? launch_rows<SBOD_DT_BF16, true>(a, s) : launch_rows<SBOD_DT_BF16, false>(a, s);
+    else
+      st = lse ? launch_rows<SBOD_DT_F16, true>(a, s) : launch_rows<SBOD_DT_F16, false>(a, s);
+    if (st != SBOD_OK) return st;
+  }
+  if (a.loss) {
+    hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, s, a);
+    SBOD_LAUNCHED("k_distill_sum");
+  }
+  return grad && n > 0 ? launch_grad(a, dtype, s) : SBOD_OK;
+}
+
+extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
+                                int ids64, const void *top, int top_dtype, int k, const float *lse,
+                                const float *weights, float temperature, int reduction, const float *norm,
+                                const float *stats,
+                                const float *upstream, int skip_if_one, void *grad, int64_t grad_ld, void *stream) {
+  const int bad = check_common("sbod_distill_bwd", logits, dtype, n, v, ld, ids, top, top_dtype, k, temperature, reduction);
+  if (bad != SBOD_OK) return bad;
+  if (n == 0) return SBOD_OK;
+  SBOD_REQUIRE(stats && grad && upstream && grad_ld >= v, "sbod_distill_bwd: null tensor or row stride %lld",
+               static_cast<long long>(grad_ld));
+  SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || norm, "sbod_distill_bwd: a reduction needs the forward's norm");
+  SBOD_REQUIRE(!skip_if_one || reduction != SBOD_REDUCE_NONE, "sbod_distill_bwd: skip_if_one needs a reduction");
+  DistillArgs a = {};
+  a.x = logits, a.n = n, a.v = v, a.ldx = ld, a.ids = ids, a.ids64 = ids64, a.top = top, a.top_dt = top_dtype;
+  a.k = k, a.lse = lse, a.w = weights, a.reduction = reduction, a.skip_one = skip_if_one;
+  a.norm = reduction == SBOD_REDUCE_NONE ? nullptr : const_cast<float *>(norm);
+  a.stats = const_cast<float *>(stats), a.up = upstream, a.up_stride = reduction == SBOD_REDUCE_NONE ? 1 : 0;
+  a.nchunk = distill_chunks(v, dtype), a.dx = grad, a.lddx = grad_ld;
+  set_temperature(a, temperature);
+  return launch_grad(a, dtype, as_stream(stream));
+}

@@ -1,0 +1,107 @@
+// Device helpers of the label-vocabulary operators (distill.hip, logits.hip, embed.hip): element
+// types, and rows that start anywhere read and written in aligned 16-byte granules.
+#pragma once
+
+#include "sbod_common.h"
+
+namespace sbod {
+namespace label {
+
+// One element type of the ABI (SBOD_DT_*): P elements fill a 16-byte granule.  All arithmetic is
+// in 32 bits; a store rounds once to nearest even (gfx950's own conversions).
+template <int DT>
+struct Elt;
+template <>
+struct Elt<SBOD_DT_F32> {
+  using T = float;
+  static constexpr int P = 4;
+};
+template <>
+struct Elt<SBOD_DT_BF16> {
+  using T = __bf16;
+  static constexpr int P = 8;
+};
+template <>
+struct Elt<SBOD_DT_F16> {
+  using T = _Float16;
+  static constexpr int P = 8;
+};
+
+inline size_t elt_bytes(int dt) { return dt == SBOD_DT_F32 ? 4 : 2; }
+inline bool known_dt(int dt) { return dt == SBOD_DT_F32 || dt == SBOD_DT_BF16 || dt == SBOD_DT_F16; }
+
+template <typename T, int N>
+using vec_t = T __attribute__((ext_vector_type(N)));
+
+__device__ __forceinline__ float ld_any(const void *p, int64_t i, int dt) {
+  if (dt == SBOD_DT_F32) return static_cast<const float *>(p)[i];
+  if (dt == SBOD_DT_BF16) return static_cast<float>(static_cast<const __bf16 *>(p)[i]);
+  return static_cast<float>(static_cast<const _Float16 *>(p)[i]);
+}
+
+// A label id as the caller holds it (int32 or int64); -1 for anything outside [0, v).
+__device__ __forceinline__ int ld_id(const void *ids, int64_t i, bool wide, int64_t v) {
+  const int64_t id = wide ? static_cast<const int64_t *>(ids)[i] : static_cast<const int32_t *>(ids)[i];
+  return id >= 0 && id < v ? static_cast<int>(id) : -1;
+}
+
+// Elements between the 16-byte boundary at or below p and p itself: granule g of a row at p holds
+// the elements [g P - phase, (g + 1) P - phase) of it.
+template <typename T>
+__device__ __forceinline__ int row_phase(const T *p) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+}
+
+// The elements [e, e + P) of a row of v at p; those outside the row read as `fill`.  p + e is
+// 16-byte aligned (row_phase), so a granule inside the row is one load, and nothing outside the row
+// is touched.
+template <int DT>
+__device__ __forceinline__ void ld_granule(const typename Elt<DT>::T *p, int64_t e, int64_t v, float fill,
+                                           float (&f)[Elt<DT>::P]) {
+  using T = typename Elt<DT>::T;
+  constexpr int P = Elt<DT>::P;
+  if (e >= 0 && e + P <= v) {
+    const vec_t<T, P> r = *reinterpret_cast<const vec_t<T, P> *>(p + e);
+#pragma unroll
+    for (int j = 0; j < P; ++j) f[j] = static_cast<float>(r[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) f[j] = e + j >= 0 && e + j < v ? static_cast<float>(p[e + j]) : fill;
+  }
+}
+
+// The same elements written.  `aligned`: p + e is 16-byte aligned; else element by element.
+template <int DT>
+__device__ __forceinline__ void st_granule(typename Elt<DT>::T *p, int64_t e, int64_t v, bool aligned,
+                                           const float (&f)[Elt<DT>::P]) {
+  using T = typename Elt<DT>::T;
+  constexpr int P = Elt<DT>::P;
+  if (aligned && e >= 0 && e + P <= v) {
+    vec_t<T, P> r;
+#pragma unroll
+    for (int j = 0; j < P; ++j) r[j] = static_cast<T>(f[j]);
+    *reinterpret_cast<vec_t<T, P> *>(p + e) = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+      if (e + j >= 0 && e + j < v) p[e + j] = static_cast<T>(f[j]);
+  }
+}
+
+// LDS written by lanes of a wave before this is seen by its other lanes after it.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ float wave_max_f32(float v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, kWave));
+  return v;
+}
+
+// 2^x by the hardware instruction (1 ulp; results below 2^-126 are 0).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+}  // namespace label
+}  // namespace sbod

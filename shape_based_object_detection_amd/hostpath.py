@@ -453,3 +453,132 @@ def calculate_mAP(det_boxes, det_labels, det_scores, true_boxes, true_labels, tr
             pr[i] = prec[above].max() if above.any() else 0.
         aps[c - 1] = pr.mean()
     return aps.tolist(), aps.mean().item()
+
+
+# ----------------------------------------------------------------------------- label vocabularies
+class _TopKDistill(torch.autograd.Function):
+    """The row losses of ``operators.Loss.topk_distill_loss`` and their gradient, in 64 bits."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, top, lse, temperature):
+        n, v = logits.shape
+        x, t = logits.double() / temperature, top.double() / temperature
+        there = (ids >= 0) & (ids < v)
+        ids = ids.long().masked_fill(~there, 0)
+        p = torch.softmax(t.masked_fill(~there, -math.inf), 1) if lse is None else torch.exp(t - lse.double()[:, None])
+        p = p.masked_fill(~there, 0.0)
+        live = ~(logits == -math.inf).all(1)
+        if lse is None:   # without an entry that has mass there is nothing to learn
+            live &= ~(~there | (top == -math.inf)).all(1)
+        x, p = x.masked_fill(~live[:, None], 0.0), p.masked_fill(~live[:, None], 0.0)
+        logq = torch.log_softmax(x, 1)
+        logp = torch.log(p)
+        kl = torch.where(p == 0, torch.zeros_like(p), p * (logp - logq.gather(1, ids))).sum(1)
+        mass = torch.zeros_like(x).scatter_add_(1, ids, p)
+        grad = logq.exp() - mass
+        if lse is not None:
+            listed = torch.zeros(n, v).scatter_add_(1, ids, there.to(torch.float32)) > 0
+            others = logq.masked_fill(listed, -math.inf)
+            logo = torch.logsumexp(others, 1)
+            rest = (1.0 - p.sum(1)).clamp(min=0.0)
+            rest = rest.masked_fill(listed.all(1), 0.0)
+            kl = kl + torch.where(rest > 0, rest * (torch.log(rest) - logo), rest)
+            share = torch.softmax(others, 1).masked_fill((logo == -math.inf)[:, None], 0.0)
+            grad = torch.where(listed, grad, share * (logo.exp() - rest)[:, None])
+        elif not live.all():
+            grad = grad.masked_fill(~live[:, None], 0.0)
+        ctx.live = live
+        ctx.save_for_backward(grad.masked_fill_(~live[:, None], 0.0) * temperature)
+        ctx.dtype = logits.dtype
+        return (temperature * temperature * kl).masked_fill(~live, 0.0)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        (grad,) = ctx.saved_tensors
+        g = g.masked_fill(~ctx.live, 0.0)
+        return (g[:, None] * grad).to(ctx.dtype), None, None, None, None
+
+
+def topk_distill(logits, ids, top, lse, weights, temperature, reduction):
+    """``operators.Loss.topk_distill_loss`` on CPU tensors."""
+    lead, v, k = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
+    w = torch.ones(lead).reshape(-1) if weights is None else weights.detach().reshape(-1).float()
+    live = w != 0   # (a row of weight 0 is left out, whatever it holds)
+    x = logits.reshape(-1, v).masked_fill(~live[:, None], 0.0)
+    rows = _TopKDistill.apply(x, ids.reshape(-1, k), top.detach().reshape(-1, k).masked_fill(~live[:, None], 0.0),
+                              None if lse is None else lse.detach().reshape(-1).masked_fill(~live, 0.0), temperature)
+    rows = torch.where(live, rows * w, torch.zeros_like(rows))
+    if reduction == 'none':
+        return rows.float().reshape(lead)
+    norm = w.double().sum() if reduction == 'mean' else torch.ones((), dtype=torch.float64)
+    return (rows.sum() / norm if norm != 0 else rows.sum() * 0.0).float()
+
+
+def process_logits(logits, history, history_len, prompt_len, repetition, presence, frequency, bias, bias_ids, bias_values,
+                   allowed, out):
+    """``operators.Logits.process_logits`` on CPU tensors."""
+    x = (logits if logits.dim() == 2 else logits[None]).detach()
+    x = x.float() if x.dtype != torch.float64 else x.clone()
+    n, v = x.shape
+
+    def column(t):
+        return t.to(x.dtype)[:, None] if torch.is_tensor(t) else t
+
+    def counts(ids, live):   # [n, v]: how often each label is among a row's live entries
+        live = live & (ids >= 0) & (ids < v)
+        c = torch.zeros(n, v, dtype=torch.int64)
+        return c.scatter_add_(1, ids.long().masked_fill(~live, 0), live.long())
+
+    if history is not None:
+        history = history.expand(n, -1)
+        place = torch.arange(history.shape[1]).expand(n, -1)
+        live = place < history_len.long()[:, None] if history_len is not None else place >= 0
+        answered = place >= prompt_len.long()[:, None] if prompt_len is not None else place >= 0
+        rep = column(repetition)
+        x = torch.where(counts(history, live) > 0, torch.where(x > 0, x / rep, x * rep), x)
+        count = counts(history, live & answered)
+        x = torch.where(count > 0, x - column(frequency) * count.to(x.dtype) - column(presence), x)
+    if bias is not None:
+        x = x + bias
+    if bias_ids is not None:
+        ids, val = bias_ids.expand(n, -1), bias_values.expand(n, -1)
+        there = (ids >= 0) & (ids < v)
+        listed = torch.zeros_like(x).scatter_add_(1, ids.long().masked_fill(~there, 0), val.masked_fill(~there, 0.0).to(x.dtype))
+        x = x + listed
+    if allowed is not None:
+        if allowed.dtype != torch.bool:
+            label = torch.arange(v)
+            allowed = (allowed.expand(n, -1)[:, label // 32] >> (label % 32)) & 1 > 0
+        x = x.masked_fill(~allowed, -math.inf)
+    x = x.to(logits.dtype).reshape(logits.shape)
+    return x if out is None else out.copy_(x)
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, pad):
+        v = weight.shape[0]
+        wide = torch.float64 if weight.dtype == torch.float64 else torch.float32
+        there = (ids >= 0) & (ids < v)
+        flat = ids.long().masked_fill(~there, 0)
+        out = torch.zeros(ids.shape + weight.shape[1:], dtype=weight.dtype)
+        if ids.numel():
+            out = (weight[flat].to(wide) * scale).to(weight.dtype).masked_fill(~there[..., None], 0.0)
+        ctx.save_for_backward(flat, there & (ids != pad))
+        ctx.args = (weight.shape, scale, wide)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        flat, live = ctx.saved_tensors
+        shape, scale, wide = ctx.args
+        g2 = g.reshape(-1, shape[1]).to(wide)[live.reshape(-1)]
+        grad = torch.zeros(shape, dtype=wide).index_add_(0, flat.reshape(-1)[live.reshape(-1)], g2)
+        return (grad * scale).to(g.dtype), None, None, None
+
+
+def scaled_embedding(ids, weight, scale, pad):
+    """``operators.Embedding.scaled_embedding`` on CPU tensors."""
+    return _ScaledEmbedding.apply(weight, ids, float(scale), pad)

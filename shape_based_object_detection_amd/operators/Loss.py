@@ -109,3 +109,36 @@ class SmoothL1Loss(nn.Module):
         if self.reduction == 'mean':
             return l1_loss.sum() / num
         return l1_loss.sum()
+
+
+def topk_distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=None, temperature=1.0,
+                      reduction='mean'):
+    """Distillation from the few top logits kept of a teacher (the reference has none):
+    ``T^2 KL(teacher || softmax(logits / T))`` of each row of class logits [..., V].
+
+    ``teacher_ids`` [..., K] (int32 / int64; an id outside [0, V) is an absent entry, one listed twice adds its
+    masses) and ``teacher_logits`` [..., K], 1 <= K <= 1024: the teacher is their softmax at T.  With
+    ``teacher_lse`` [...], its log-sum-exp of logits / T over the whole vocabulary, the kept entries keep their own
+    probabilities and what is left is one bucket against the student's mass on all other labels.
+
+    ``weights`` [...]: each row's share.  'mean' divides by their sum (without weights: by the rows; 0 where that
+    is 0), 'sum' adds, 'none' returns the weighted row losses [...].  Loss in float32, gradient in the logits'
+    type.  A row of weight 0, without an entry that has mass, or whose logits are all -inf gives loss 0 and a zero
+    gradient.  The teacher's tensors and the weights are constants: one that requires a gradient is refused."""
+    core.distill_arguments(logits, teacher_ids, teacher_logits, teacher_lse, weights, temperature, reduction)
+    on = on_host(*[t for t in (logits, teacher_ids, teacher_logits, teacher_lse, weights) if t is not None])
+    run = hostpath.topk_distill if on else core.topk_distill
+    return run(logits, teacher_ids, teacher_logits, teacher_lse, weights, float(temperature), reduction)
+
+
+class TopKDistillLoss(nn.Module):
+    """``topk_distill_loss`` with its temperature and reduction."""
+
+    def __init__(self, temperature=1.0, reduction='mean'):
+        super().__init__()
+        self.temperature = temperature
+        self.reduction = reduction
+
+    def forward(self, logits, teacher_ids, teacher_logits, teacher_lse=None, weights=None):
+        return topk_distill_loss(logits, teacher_ids, teacher_logits, teacher_lse, weights, self.temperature,
+                                 self.reduction)

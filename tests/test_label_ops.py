@@ -1,0 +1,188 @@
+"""Label-vocabulary operators on CPU tensors, and their refusals (no device call is made)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import label_cases as C
+from oracle import label_ref as R
+from shape_based_object_detection_amd import _lib as L
+from shape_based_object_detection_amd.operators.Embedding import ScaledEmbedding, scaled_embedding
+from shape_based_object_detection_amd.operators.Logits import process_logits
+from shape_based_object_detection_amd.operators.Loss import TopKDistillLoss, topk_distill_loss
+
+
+@pytest.mark.parametrize('tail', [False, True])
+@pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
+def test_distill_host(tail, reduction):
+    x, ids, top, lse = C.distill_inputs(9, 21, 5, torch.float32, 1, tail)
+    ids[2] = -1
+    ids[3, 1] = ids[3, 0]
+    x[4] = -math.inf
+    x[5, ids[5, 0]] = -1e9
+    w = torch.rand(9)
+    w[6] = 0
+    x[6, 3] = math.nan
+    x.requires_grad_(True)
+    up = torch.rand(9) if reduction == 'none' else torch.tensor(0.5)
+    loss = topk_distill_loss(x, ids, top, lse, w, 2.0, reduction)
+    grad, = torch.autograd.grad(loss, x, up)
+    C.check_distill(loss, grad, x, ids, top, lse, w, 2.0, reduction, up)
+
+
+def test_distill_oracle_gradient_by_differences():
+    """d loss / dx of the oracle against central differences of its own loss (step 1e-5: error 1e-9 or so)."""
+    for tail in (False, True):
+        x, ids, top, lse = C.distill_inputs(1, 11, 4, torch.float64, 3, tail)
+        ids[0, 3] = ids[0, 0]
+        xn, ln = x.numpy()[0], None if lse is None else lse.numpy()[0]
+        _, g = R.distill_row(xn, ids[0].numpy(), top.numpy()[0], ln, 1.5)
+        for v in range(11):
+            d = np.zeros(11)
+            d[v] = 1e-5
+            hi, lo = (R.distill_row(xn + s * d, ids[0].numpy(), top.numpy()[0], ln, 1.5)[0] for s in (1, -1))
+            assert abs((hi - lo) / 2e-5 - g[v]) < 1e-7
+
+
+def test_logits_host():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(4, 37, generator=g)
+    x[0, 5] = math.nan
+    hist = torch.randint(-1, 40, (4, 12), generator=g)
+    lens, prompt = torch.tensor([12, 0, 5, 99]), torch.tensor([3, 0, 9, 0])
+    rep, bias = torch.tensor([1.5, 1.0, 2.0, 0.5]), torch.randn(37, generator=g)
+    bi = torch.tensor([[3, 3, -1, 36]] * 4)
+    bv = torch.randn(4, 4, generator=g)
+    ok = torch.rand(4, 37, generator=g) < 0.5
+    ok[0, 5] = False
+    ok[3] = False
+    want, mag = R.process_logits(x.numpy(), hist.numpy(), lens.numpy(), prompt.numpy(), rep.numpy(), 0.3, 0.2,
+                                 bias.numpy(), bi.numpy(), bv.numpy(), ok.numpy())
+    words = torch.zeros(4, 2, dtype=torch.int32)
+    for v in range(37):
+        words[:, v // 32] |= ok[:, v].int() << (v % 32)
+    for allowed in (ok, words):
+        got = process_logits(x, hist, lens, prompt, rep, 0.3, 0.2, bias, bi, bv, allowed)
+        C.check_logits(got, want, mag, torch.float32, 8)
+    y = x.clone()
+    assert process_logits(y, hist, lens, prompt, rep, 0.3, 0.2, bias, bi, bv, ok, out=y) is y
+    assert torch.equal(y, got)
+    one = process_logits(x[1], hist[1], repetition=2.0, allowed=ok[1])
+    assert torch.equal(one, process_logits(x[1:2], hist[1:2], repetition=2.0, allowed=ok[1:2])[0])
+
+
+def test_embedding_host():
+    m = ScaledEmbedding(13, 6, padding_idx=-1)
+    assert m.scale == math.sqrt(6) and torch.all(m.weight[12] == 0)
+    ids = torch.tensor([[1, 12, 1], [0, -1, 13]])
+    g = torch.randn(2, 3, 6)
+    out = m(ids)
+    assert torch.all(out[1, 1:] == 0) and torch.allclose(out[0, 0], m.weight[1] * m.scale)
+    grad, = torch.autograd.grad(out, m.weight, g)
+    C.check_embedding_grad(grad, ids, g, 13, m.scale, 12)
+
+
+X, IDS, TOP = torch.zeros(2, 5), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+
+
+@pytest.mark.parametrize('args,error', [
+    ((X.long(), IDS, TOP), TypeError),
+    ((X, IDS.float(), TOP), TypeError),
+    ((X, IDS, TOP.long()), TypeError),
+    ((X, IDS[:1], TOP[:1]), ValueError),
+    ((X, IDS, TOP[:, :2]), ValueError),
+    ((X, IDS[:, :0], TOP[:, :0]), ValueError),
+    ((X[:, :0], IDS, TOP), ValueError),
+    ((X, IDS.repeat(1, 400), TOP.repeat(1, 400)), ValueError),
+    ((X, IDS, TOP, torch.zeros(3)), ValueError),
+    ((X, IDS, TOP, None, torch.zeros(2, 1)), ValueError),
+    ((X, IDS, TOP, None, None, 0.0), ValueError),
+    ((X, IDS, TOP, None, None, math.inf), ValueError),
+    ((X, IDS, TOP, None, None, 1.0, 'batchmean'), ValueError),
+    ((X, IDS, TOP.clone().requires_grad_(True)), ValueError),
+    ((X, IDS, TOP, None, torch.ones(2, requires_grad=True)), ValueError),
+])
+def test_distill_refusals(args, error):
+    with pytest.raises(error, match='topk_distill_loss'):
+        topk_distill_loss(*args)
+
+
+H = torch.zeros(2, 4, dtype=torch.int64)
+
+
+@pytest.mark.parametrize('kw,error', [
+    (dict(logits=X.int()), TypeError),
+    (dict(logits=X[None]), ValueError),
+    (dict(logits=X[:, :0]), ValueError),
+    (dict(logits=X.clone().requires_grad_(True)), ValueError),
+    (dict(history=H.float()), TypeError),
+    (dict(history=H[:1]), ValueError),
+    (dict(history_len=torch.tensor([1, 2])), ValueError),
+    (dict(history=H, history_len=torch.tensor([1])), ValueError),
+    (dict(history=H, prompt_len=torch.tensor([1.0, 2.0])), TypeError),
+    (dict(history=H, repetition=0.0), ValueError),
+    (dict(history=H, repetition=-1.0), ValueError),
+    (dict(history=H, presence=torch.tensor([1, 2])), ValueError),
+    (dict(history=H, frequency=torch.ones(3)), ValueError),
+    (dict(bias=torch.zeros(5, dtype=torch.float64)), TypeError),
+    (dict(bias=torch.zeros(4)), ValueError),
+    (dict(bias_ids=H), ValueError),
+    (dict(bias_ids=H, bias_values=torch.zeros(2, 3)), ValueError),
+    (dict(bias_ids=H, bias_values=torch.zeros(2, 4, dtype=torch.float16)), TypeError),
+    (dict(allowed=torch.ones(2, 4, dtype=torch.bool)), ValueError),
+    (dict(allowed=torch.ones(2, 0, dtype=torch.int32)), ValueError),
+    (dict(allowed=torch.ones(2, 5)), TypeError),
+    (dict(out=torch.zeros(2, 5, dtype=torch.float16)), ValueError),
+    (dict(out=torch.zeros(2, 6)), ValueError),
+])
+def test_logits_refusals(kw, error):
+    with pytest.raises(error, match='process_logits'):
+        process_logits(**dict(dict(logits=X), **kw))
+
+
+@pytest.mark.parametrize('args,error', [
+    ((torch.zeros(3), X), TypeError),
+    ((IDS, X[0]), ValueError),
+    ((IDS, X.int()), ValueError),
+    ((IDS, X[:0]), ValueError),
+    ((IDS, X, math.nan), ValueError),
+    ((IDS, X, 1.0, 2), ValueError),
+    ((IDS, X, 1.0, -3), ValueError),
+])
+def test_embedding_refusals(args, error):
+    with pytest.raises(error, match='scaled_embedding'):
+        scaled_embedding(*args)
+
+
+def test_entry_points_refuse_before_any_launch():
+    """Bad sizes at the C ABI come back as a status, with a message and without a launch."""
+    def distill(dt=0, n=2, v=5, ld=5, k=3, T=1.0, red=1, ws=1 << 20):
+        return L.call('sbod_distill_fwd', 8, dt, n, v, ld, 8, 1, 8, 0, k, None, None, T, red, 8, 8, 8, 8, None, 0, 8, ws, None)
+
+    for kw in (dict(dt=3), dict(n=-1), dict(v=0), dict(ld=4), dict(k=0), dict(k=1025), dict(T=0.0), dict(T=math.inf),
+               dict(red=3), dict(ws=0), dict(v=1 << 31, ld=1 << 31)):
+        with pytest.raises(L.SbodError, match='sbod_distill_fwd'):
+            distill(**kw)
+
+    def logits(dt=0, n=2, v=5, ld=5, cols=4, hist=8, rep=1.0, kind=0, mask=None, out_ld=5):
+        return L.call('sbod_logits_process', 8, dt, n, v, ld, hist, 1, cols, 4, None, None, None, None, None, rep, 0.0, 0.0,
+                      None, 0, 0, None, 0, None, 0, 0, 0, mask, kind, 0, 8, out_ld, None)
+
+    for kw in (dict(dt=5), dict(n=-1), dict(v=0), dict(ld=4), dict(out_ld=4), dict(hist=None), dict(rep=0.0), dict(kind=1),
+               dict(kind=7, mask=8), dict(cols=-1)):
+        with pytest.raises(L.SbodError, match='sbod_logits_process'):
+            logits(**kw)
+    for name, args in (('sbod_embed_fwd', (8, 3, 5, 4, 8, 1, 2, 1.0, 8, None)), ('sbod_embed_fwd', (8, 0, 0, 4, 8, 1, 2, 1.0, 8, None)),
+                       ('sbod_embed_fwd', (8, 0, 5, 4, 8, 1, -2, 1.0, 8, None)),
+                       ('sbod_embed_bwd', (8, 0, 5, 4, 8, 1, 2, -1, 1.0, 8, 8, 1, None)),
+                       ('sbod_embed_bwd', (8, 0, 5, 4, 8, 1, 2, -1, 1.0, None, 8, 1 << 20, None))):
+        with pytest.raises(L.SbodError, match=name):
+            L.call(name, *args)
+
+
+def test_module_holds_its_settings():
+    x, ids, top, _ = C.distill_inputs(3, 7, 2, torch.float32, 0)
+    m = TopKDistillLoss(temperature=2.0, reduction='sum')
+    assert torch.equal(m(x, ids, top), topk_distill_loss(x, ids, top, temperature=2.0, reduction='sum'))
+    assert topk_distill_loss(x[:0], ids[:0], top[:0]) == 0
