@@ -522,7 +522,7 @@ int sbod_logits_process(const void *logits, int dtype, int64_t n, int64_t v, int
  * label that gets no gradient.  table, out, grad, grad_table are contiguous. */
 int sbod_embed_fwd(const void *table, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,
                    float scale, void *out, void *stream);
-size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v);
+size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v, int64_t d);
 int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,
                    int64_t padding, float scale, void *grad_table, void *workspace, size_t workspace_bytes,
                    void *stream);

@@ -93,7 +93,7 @@ SIGNATURES = {
     'sbod_logits_process': (I32, [P, I32, I64, I64, I64, P, I32, I64, I64, P, P, P, P, P, F32, F32, F32, P, I32, I64,
                                   P, I32, P, I32, I64, I64, P, I32, I64, P, I64, P]),
     'sbod_embed_fwd': (I32, [P, I32, I64, I64, P, I32, I64, F32, P, P]),
-    'sbod_embed_bwd_workspace_bytes': (SZ, [I64, I64]),
+    'sbod_embed_bwd_workspace_bytes': (SZ, [I64, I64, I64]),
     'sbod_embed_bwd': (I32, [P, I32, I64, I64, P, I32, I64, I64, F32, P, P, SZ, P]),
 }
 

@@ -1500,7 +1500,7 @@ class _ScaledEmbedding(torch.autograd.Function):
         g = g.contiguous()
         n = ids.numel()
         grad = torch.empty(v, d, dtype=g.dtype, device=g.device)
-        nb = L.lib().sbod_embed_bwd_workspace_bytes(n, v)
+        nb = L.lib().sbod_embed_bwd_workspace_bytes(n, v, d)
         ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=g.device)
         with _on_device(g):
             L.call('sbod_embed_bwd', L.ptr(g), L.LABEL_DT[g.dtype], v, d, L.ptr(ids), wide, n, pad, scale, L.ptr(grad),

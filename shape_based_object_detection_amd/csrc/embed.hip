@@ -6,6 +6,7 @@
 // The gradient's order is fixed: the positions of each label are sorted first, one launch of workgroups
 // that own a range of labels each, then each row of the table is summed by the threads that own its
 // columns, in 32 bits, and written once (zeros where no label came): no atomics on sums, no clearing pass.
+// A label that came often is summed in pieces first (k_embed_pieces), so that no thread walks a long run.
 #include "label_dev.h"
 
 namespace sbod {
@@ -139,11 +140,76 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const void *table, c
   }
 }
 
+// Rows of a run per piece: about half the square root of the positions, so that a run's pieces are no
+// more than the rows of one.
+__host__ __device__ inline int piece_rows(int64_t n) {
+  int s = 16;
+  while (s < 1024 && 4ll * s * s < n) s *= 2;
+  return s;
+}
+
+// acc += the rows sorted[b .. e) of grad, in that order; kU of them in flight.
+template <typename T, int kV>
+__device__ __forceinline__ void add_rows(float (&acc)[kV], const T *grad, const int32_t *sorted, int b, int e, int64_t d,
+                                         int64_t g) {
+  using V = vec_t<T, kV>;
+  constexpr int kU = 8;
+  for (int i = b; i < e; i += kU) {
+    int at[kU];
+    V s[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) at[u] = sorted[min(i + u, e - 1)];
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (i + u < e) s[u] = reinterpret_cast<const V *>(grad + at[u] * d)[g];
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+      if (i + u < e) {
+#pragma unroll
+        for (int j = 0; j < kV; ++j) acc[j] += static_cast<float>(s[u][j]);
+      }
+  }
+}
+
+// Sums of the positions [c rows, (c + 1) rows) for the labels that came more than `rows` times: such a
+// run covers the chunk's first position (pieces[c][0]) or, begun inside, its last one (pieces[c][1]).
+template <int DT, int kV>
+__global__ __launch_bounds__(kEmbThreads) void k_embed_pieces(const void *grad, const void *ids, int ids64,
+                                                              const int32_t *begin, const int32_t *sorted, int64_t v,
+                                                              int64_t chunks, int rows, int64_t groups, float *pieces) {
+  using T = typename Elt<DT>::T;
+  const int64_t d = groups * kV;
+  const int total = begin[v];
+  for (int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y; c < chunks;
+       c += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+    const int c0 = static_cast<int>(c * rows), c1 = min(c0 + rows, total);
+    if (c0 >= total) break;
+    const int first = ld_id(ids, sorted[c0], ids64, v), last = ld_id(ids, sorted[c1 - 1], ids64, v);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const int label = side ? last : first;
+      if (side && last == first) break;
+      const int b = begin[label], e = begin[label + 1];
+      if (e - b <= rows) continue;
+      for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
+        float acc[kV];
+#pragma unroll
+        for (int j = 0; j < kV; ++j) acc[j] = 0.f;
+        add_rows<T, kV>(acc, static_cast<const T *>(grad), sorted, max(b, c0), min(e, c1), d, g);
+        vec_t<float, kV> o;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) o[j] = acc[j];
+        reinterpret_cast<vec_t<float, kV> *>(pieces + (2 * c + side) * d)[g] = o;
+      }
+    }
+  }
+}
+
 // d table[v] from the sorted positions.  The same blocks over the table's rows.
 template <int DT, int kV>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, const int32_t *begin,
-                                                            const int32_t *sorted, int64_t v, int64_t groups,
-                                                            float scale, void *dtable) {
+                                                            const int32_t *sorted, int64_t v, int rows, int64_t groups,
+                                                            const float *pieces, float scale, void *dtable) {
   using T = typename Elt<DT>::T;
   using V = vec_t<T, kV>;
   const int64_t d = groups * kV;
@@ -155,10 +221,25 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, co
       float acc[kV];
 #pragma unroll
       for (int j = 0; j < kV; ++j) acc[j] = 0.f;
-      for (int i = b; i < e; ++i) {
-        const V s = reinterpret_cast<const V *>(static_cast<const T *>(grad) + sorted[i] * d)[g];
+      if (e - b <= rows) {
+        add_rows<T, kV>(acc, static_cast<const T *>(grad), sorted, b, e, d, g);
+      } else {
+        constexpr int kU = 4;
+        const int last = (e - 1) / rows;
+        for (int c = b / rows; c <= last; c += kU) {
+          vec_t<float, kV> s[kU];
 #pragma unroll
-        for (int j = 0; j < kV; ++j) acc[j] += static_cast<float>(s[j]);
+          for (int u = 0; u < kU; ++u) {
+            const int64_t at = min(c + u, last);
+            s[u] = reinterpret_cast<const vec_t<float, kV> *>(pieces + (2 * at + (at * rows < b)) * d)[g];
+          }
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+            if (c + u <= last) {
+#pragma unroll
+              for (int j = 0; j < kV; ++j) acc[j] += s[u][j];
+            }
+        }
       }
       V o;
 #pragma unroll
@@ -235,9 +316,11 @@ extern "C" int sbod_embed_fwd(const void *table, int dtype, int64_t v, int64_t d
   return SBOD_OK;
 }
 
-extern "C" size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v) {
-  if (n < 0 || v <= 0) return 0;
-  return align_up((v + 1) * sizeof(int32_t)) + align_up((n > 0 ? n : 1) * sizeof(int32_t));
+extern "C" size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v, int64_t d) {
+  if (n < 0 || v <= 0 || d < 0) return 0;
+  const int64_t rows = piece_rows(n), chunks = n > rows ? (n + rows - 1) / rows : 0;
+  return align_up((v + 1) * sizeof(int32_t)) + align_up((n > 0 ? n : 1) * sizeof(int32_t)) +
+         static_cast<size_t>(chunks) * 2 * d * sizeof(float);
 }
 
 extern "C" int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,
@@ -247,8 +330,8 @@ extern "C" int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d,
   if (bad != SBOD_OK) return bad;
   if (v == 0 || d == 0) return SBOD_OK;
   SBOD_REQUIRE(grad_table && (n == 0 || (grad && ids)), "sbod_embed_bwd: null tensor");
-  if (!workspace || workspace_bytes < sbod_embed_bwd_workspace_bytes(n, v)) {
-    set_error("sbod_embed_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_embed_bwd_workspace_bytes(n, v));
+  if (!workspace || workspace_bytes < sbod_embed_bwd_workspace_bytes(n, v, d)) {
+    set_error("sbod_embed_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_embed_bwd_workspace_bytes(n, v, d));
     return SBOD_E_WORKSPACE;
   }
   hipStream_t s = as_stream(stream);
@@ -261,7 +344,17 @@ extern "C" int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d,
   SBOD_LAUNCHED("k_embed_sort");
   const int w = column_group(d, dtype, grad, grad_table);
   const dim3 block = row_block(d / w);
-  SBOD_EMBED_LAUNCH(k_embed_grad, dtype, w, row_grid(v, block), block, grad, begin, sorted, v, d / w, scale, grad_table);
+  const int rows = piece_rows(n);
+  float *pieces = nullptr;
+  if (n > rows) {   // (else no label can have come more often)
+    const int64_t chunks = (n + rows - 1) / rows;
+    pieces = ws_at<float>(workspace, align_up((v + 1) * sizeof(int32_t)) + align_up(n * sizeof(int32_t)));
+    SBOD_EMBED_LAUNCH(k_embed_pieces, dtype, w, row_grid(chunks, block), block, grad, ids, ids64, begin, sorted, v, chunks,
+                      rows, d / w, pieces);
+    SBOD_LAUNCHED("k_embed_pieces");
+  }
+  SBOD_EMBED_LAUNCH(k_embed_grad, dtype, w, row_grid(v, block), block, grad, begin, sorted, v, rows, d / w, pieces, scale,
+                    grad_table);
   SBOD_LAUNCHED("k_embed_grad");
   return SBOD_OK;
 }
