@@ -7,6 +7,8 @@
 // that own a range of labels each, then each row of the table is summed by the threads that own its
 // columns, in 32 bits, and written once (zeros where no label came): no atomics on sums, no clearing pass.
 // A label that came often is summed in pieces first (k_embed_pieces), so that no thread walks a long run.
+#include <type_traits>
+
 #include "label_dev.h"
 
 namespace sbod {
@@ -22,40 +24,57 @@ __host__ __device__ inline int64_t sort_range(int64_t v) {
   return r < kSortRange ? r : kSortRange;
 }
 
+// Positions per flag bit of a wave's run of `per` positions: 64, or more so that a wave's flags fit
+// kSortFlags words (64 positions up to 4 M ids).
+constexpr int kSortFlags = 64;
+__host__ __device__ inline int flag_shift(int64_t per) {
+  int shift = 6;
+  while (per > (64ll * kSortFlags) << shift) ++shift;
+  return shift;
+}
+
 // Workgroup b: the positions of the labels [b range, (b + 1) range) in the order (label, position), and
-// where each label's begin.  Every workgroup reads all ids (they stay in its XCD's L2): once to count
-// its own labels and those below its range, once to place.  A wave owns a run of positions and a row of
-// counters, so its placing needs no other wave: the order is that of the positions.
-__global__ __launch_bounds__(kSortThreads) void k_embed_sort(const void *ids, int ids64, int64_t n, int64_t v,
-                                                             int64_t padding, int range, int32_t *__restrict__ begin,
-                                                             int32_t *__restrict__ sorted) {
-  extern __shared__ int32_t cnt[];   // [kSortWaves][range]
+// where each label's begin (an absent id has no place).  Every workgroup reads all ids (they stay in its
+// XCD's L2), counts its own labels and those below its range, and flags the stretches that hold one of
+// its own: only those are read again, to place.  A wave owns a run of positions and a row of counters, so
+// its placing needs no other wave: the order is that of the positions.
+template <typename ID>
+__global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID *__restrict__ ids, int64_t n, int64_t v, int range,
+                                                             int32_t *__restrict__ begin, int32_t *__restrict__ sorted) {
+  using U = std::make_unsigned_t<ID>;   // (a negative id is above every label)
+  extern __shared__ int32_t cnt[];      // [kSortWaves][range]
   __shared__ int32_t red[kSortWaves], low[kSortWaves];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * range;
-  const int mine = static_cast<int>(min(static_cast<int64_t>(range), v - lo));
+  __shared__ unsigned long long flags[kSortWaves][kSortFlags];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const U lo = static_cast<U>(static_cast<int64_t>(blockIdx.x) * range);
+  const int mine = static_cast<int>(min(static_cast<int64_t>(range), v - static_cast<int64_t>(lo)));
   for (int i = threadIdx.x; i < kSortWaves * range; i += kSortThreads) cnt[i] = 0;
+  flags[wv][lane] = 0;
   __syncthreads();
   const int64_t per = ((n + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
+  const int shift = flag_shift(per);
   const int64_t i0 = min(wv * per, n), i1 = min(i0 + per, n);
   int32_t *c = cnt + wv * range;
   int below = 0;
   constexpr int kU = 8;   // loads in flight per lane
   for (int64_t i = i0; i < i1; i += 64 * kU) {
-    int id[kU];
+    U id[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int64_t at = i + u * 64 + lane;
-      id[u] = at < i1 ? ld_id(ids, at, ids64, v) : -1;
+      id[u] = at < i1 ? static_cast<U>(ids[at]) : ~static_cast<U>(0);
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (id[u] < 0 || id[u] == padding) continue;
-      if (id[u] < lo) ++below;
-      else if (id[u] < lo + mine) atomicAdd(&c[id[u] - lo], 1);
+      below += __popcll(__ballot(id[u] < lo));
+      const U at = id[u] - lo;
+      const bool in = at < static_cast<U>(mine);
+      if (__ballot(in) == 0) continue;
+      if (in) atomicAdd(&c[static_cast<int>(at)], 1);
+      const int64_t f = (i + u * 64 - i0) >> shift;
+      if (lane == 0) flags[wv][f >> 6] |= 1ull << (f & 63);
     }
   }
-  below = wave_sum_i32(below);
   if (lane == 0) low[wv] = below;
   __syncthreads();
   // thread t: label lo + t; the labels' exclusive sums over the workgroup, then each wave's start in each
@@ -76,8 +95,9 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const void *ids, in
     if (w < wv) start += red[w];
   }
   if (static_cast<int>(threadIdx.x) < mine) {
-    begin[lo + threadIdx.x] = start;
-    if (lo + threadIdx.x == v - 1) begin[v] = start + tot;
+    const int64_t label = static_cast<int64_t>(lo) + threadIdx.x;
+    begin[label] = start;
+    if (label == v - 1) begin[v] = start + tot;
     int at = start;
     for (int w = 0; w < kSortWaves; ++w) {
       const int k = cnt[w * range + threadIdx.x];
@@ -89,31 +109,66 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const void *ids, in
   int bits = 0;
   while ((1 << bits) < mine) ++bits;
   volatile int32_t *place = c;
-  for (int64_t i = i0; i < i1; i += 64 * kU) {
-    int id[kU];
+  const int words = static_cast<int>((i1 - i0 + (64ll << shift) - 1) >> (shift + 6));   // of flags in use
+  for (int word = 0; word < words; ++word) {
+    // (read into scalar registers: the walk below is the same for every lane)
+    unsigned long long left = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(flags[wv][word] >> 32)));
+    left = left << 32 | static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(flags[wv][word])));
+    int64_t stretch = 0, end = 0;   // of a longer stretch: what is left of it
+    while (left || stretch < end) {
+      // the next kU groups of 64 positions, in order: their loads overlap
+      int64_t from[kU];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int64_t at = i + u * 64 + lane;
-      id[u] = at < i1 ? ld_id(ids, at, ids64, v) : -1;
-    }
+      for (int u = 0; u < kU; ++u) {
+        if (stretch >= end && left) {
+          stretch = i0 + ((static_cast<int64_t>(word) * 64 + __ffsll(left) - 1) << shift);
+          end = stretch + (1ll << shift);
+          left &= left - 1;
+        }
+        from[u] = stretch < end ? stretch : i1;
+        if (stretch < end) stretch += 64;
+      }
+      U id[kU];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const bool in = id[u] >= lo && id[u] < lo + mine && id[u] != padding;
-      unsigned long long same = __ballot(in);
-      if (same == 0) continue;
-      const int key = in ? static_cast<int>(id[u] - lo) : 0;
-      for (int b = 0; b < bits; ++b) {
-        const unsigned long long set = __ballot(key >> b & 1);
-        same &= key >> b & 1 ? set : ~set;
+      for (int u = 0; u < kU; ++u) {
+        const int64_t at = from[u] + lane;
+        id[u] = at < i1 ? static_cast<U>(ids[at]) : ~static_cast<U>(0);
       }
-      if (in) {
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        const int at = place[key];
-        sorted[at + rank] = static_cast<int32_t>(i + u * 64 + lane);
-        wave_lds_fence();
-        if (rank == 0) place[key] = at + __popcll(same);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const U at = id[u] - lo;
+        const bool in = at < static_cast<U>(mine);
+        unsigned long long todo = __ballot(in);
+        const int key = in ? static_cast<int>(at) : -1;
+        const int32_t pos = static_cast<int32_t>(from[u] + lane);
+        const unsigned long long before = (1ull << lane) - 1;
+        if (__popcll(todo) <= 16) {   // few of this workgroup's: label by label
+          while (todo) {
+            const int k0 = __builtin_amdgcn_readlane(key, __ffsll(todo) - 1);
+            const unsigned long long same = __ballot(key == k0);
+            const int first = place[k0];
+            if (key == k0) sorted[first + __popcll(same & before)] = pos;
+            wave_lds_fence();
+            if (lane == 0) place[k0] = first + __popcll(same);
+            wave_lds_fence();
+            todo &= ~same;
+          }
+        } else {   // many: the lanes of the same label by the bits of it
+          unsigned long long same = todo;
+          for (int b = 0; b < bits; ++b) {
+            const unsigned long long set = __ballot(key >> b & 1);
+            same &= key >> b & 1 ? set : ~set;
+          }
+          if (in) {
+            const int rank = __popcll(same & before);
+            const int first = place[key];
+            sorted[first + rank] = pos;
+            wave_lds_fence();
+            if (rank == 0) place[key] = first + __popcll(same);
+          }
+          wave_lds_fence();
+        }
       }
-      wave_lds_fence();
     }
   }
 }
@@ -140,28 +195,33 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const void *table, c
   }
 }
 
-// Rows of a run per piece: about half the square root of the positions, so that a run's pieces are no
-// more than the rows of one.
+// Rows of a run per piece: about a quarter of the square root of the positions, 16 at least and 1024 at
+// most, so that neither a piece's rows nor a run's pieces are many.
 __host__ __device__ inline int piece_rows(int64_t n) {
   int s = 16;
-  while (s < 1024 && 4ll * s * s < n) s *= 2;
+  while (s < 1024 && 16ll * s * s < n) s *= 2;
   return s;
 }
 
-// acc += the rows sorted[b .. e) of grad, in that order; kU of them in flight.
+// acc += the rows sorted[b .. e) of grad, in that order; kU of them in flight, and the next ones' numbers.
 template <typename T, int kV>
 __device__ __forceinline__ void add_rows(float (&acc)[kV], const T *grad, const int32_t *sorted, int b, int e, int64_t d,
                                          int64_t g) {
   using V = vec_t<T, kV>;
   constexpr int kU = 8;
-  for (int i = b; i < e; i += kU) {
-    int at[kU];
-    V s[kU];
+  if (b >= e) return;
+  int at[kU];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) at[u] = sorted[min(i + u, e - 1)];
+  for (int u = 0; u < kU; ++u) at[u] = sorted[min(b + u, e - 1)];
+  for (int i = b; i < e; i += kU) {
+    V s[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u)
       if (i + u < e) s[u] = reinterpret_cast<const V *>(grad + at[u] * d)[g];
+    if (i + kU < e) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) at[u] = sorted[min(i + kU + u, e - 1)];
+    }
 #pragma unroll
     for (int u = 0; u < kU; ++u)
       if (i + u < e) {
@@ -176,7 +236,8 @@ __device__ __forceinline__ void add_rows(float (&acc)[kV], const T *grad, const 
 template <int DT, int kV>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_pieces(const void *grad, const void *ids, int ids64,
                                                               const int32_t *begin, const int32_t *sorted, int64_t v,
-                                                              int64_t chunks, int rows, int64_t groups, float *pieces) {
+                                                              int64_t padding, int64_t chunks, int rows, int64_t groups,
+                                                              float *pieces) {
   using T = typename Elt<DT>::T;
   const int64_t d = groups * kV;
   const int total = begin[v];
@@ -190,8 +251,9 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_pieces(const void *grad, 
       const int label = side ? last : first;
       if (side && last == first) break;
       const int b = begin[label], e = begin[label + 1];
-      if (e - b <= rows) continue;
-      for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
+      if (e - b <= rows || label == padding) continue;
+      const int64_t g = blockIdx.y * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+      if (g < groups) {
         float acc[kV];
 #pragma unroll
         for (int j = 0; j < kV; ++j) acc[j] = 0.f;
@@ -205,24 +267,46 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_pieces(const void *grad, 
   }
 }
 
-// d table[v] from the sorted positions.  The same blocks over the table's rows.
-template <int DT, int kV>
+// d table[v] from the sorted positions.  The same blocks over the table's rows, kEmbRows of them per thread:
+// most labels came once or not at all, so a row is a chain of three loads (its places, their first row's
+// number, that row), and the rows' chains run side by side: 395 us with 4, 453 with 1 for 65,536 positions
+// into a table of 1 GB.
+template <int DT, int kV, int kEmbRows>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, const int32_t *begin,
-                                                            const int32_t *sorted, int64_t v, int rows, int64_t groups,
-                                                            const float *pieces, float scale, void *dtable) {
+                                                            const int32_t *sorted, int64_t v, int64_t padding, int rows,
+                                                            int64_t groups, const float *pieces, float scale,
+                                                            void *dtable) {
   using T = typename Elt<DT>::T;
   using V = vec_t<T, kV>;
   const int64_t d = groups * kV;
-  for (int64_t r = blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y; r < v;
-       r += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    const int b = begin[r], e = begin[r + 1];
-    V *dst = reinterpret_cast<V *>(static_cast<T *>(dtable) + r * d);
-    for (int64_t g = threadIdx.x; g < groups; g += blockDim.x) {
+  const int64_t g = blockIdx.y * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+  if (g >= groups) return;
+  const T *src = static_cast<const T *>(grad);
+  for (int64_t r0 = (blockIdx.x * static_cast<int64_t>(blockDim.y) + threadIdx.y) * kEmbRows; r0 < v;
+       r0 += static_cast<int64_t>(gridDim.x) * blockDim.y * kEmbRows) {
+    int at[kEmbRows + 1], first[kEmbRows];
+    V one[kEmbRows];
+#pragma unroll
+    for (int k = 0; k <= kEmbRows; ++k) at[k] = begin[min(r0 + k, v)];
+#pragma unroll
+    for (int k = 0; k < kEmbRows; ++k) first[k] = at[k] < at[k + 1] ? sorted[at[k]] : -1;
+#pragma unroll
+    for (int k = 0; k < kEmbRows; ++k)
+      if (first[k] >= 0) one[k] = reinterpret_cast<const V *>(src + first[k] * d)[g];
+#pragma unroll
+    for (int k = 0; k < kEmbRows; ++k) {
+      const int64_t r = r0 + k;
+      if (r >= v) break;
+      const int b = at[k], e = r == padding ? b : at[k + 1];
       float acc[kV];
 #pragma unroll
       for (int j = 0; j < kV; ++j) acc[j] = 0.f;
       if (e - b <= rows) {
-        add_rows<T, kV>(acc, static_cast<const T *>(grad), sorted, b, e, d, g);
+        if (b < e) {
+#pragma unroll
+          for (int j = 0; j < kV; ++j) acc[j] = static_cast<float>(one[k][j]);
+          add_rows<T, kV>(acc, src, sorted, b + 1, e, d, g);
+        }
       } else {
         constexpr int kU = 4;
         const int last = (e - 1) / rows;
@@ -230,8 +314,8 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, co
           vec_t<float, kV> s[kU];
 #pragma unroll
           for (int u = 0; u < kU; ++u) {
-            const int64_t at = min(c + u, last);
-            s[u] = reinterpret_cast<const vec_t<float, kV> *>(pieces + (2 * at + (at * rows < b)) * d)[g];
+            const int64_t p = min(c + u, last);
+            s[u] = reinterpret_cast<const vec_t<float, kV> *>(pieces + (2 * p + (p * rows < b)) * d)[g];
           }
 #pragma unroll
           for (int u = 0; u < kU; ++u)
@@ -244,10 +328,19 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, co
       V o;
 #pragma unroll
       for (int j = 0; j < kV; ++j) o[j] = static_cast<T>(acc[j] * scale);
-      dst[g] = o;
+      // (written once and not read here: past the caches, 505 against 535 us for a table of 1 GB)
+      __builtin_nontemporal_store(o, reinterpret_cast<V *>(static_cast<T *>(dtable) + r * d) + g);
     }
   }
 }
+
+template <int DT, int kV>
+constexpr auto k_embed_grad_wide = &k_embed_grad<DT, kV, 4>;
+template <int DT, int kV>
+constexpr auto k_embed_grad_narrow = &k_embed_grad<DT, kV, 1>;
+// Four rows per thread where that leaves every CU 512 threads; 6,400 positions into 21 rows of 256 take 36 us
+// so and 29 with one.
+bool wide_rows(int64_t v, int64_t groups) { return v * groups >= 4 * 256 * 512; }
 
 // The widest column group that every row of both tensors starts on a multiple of.
 int column_group(int64_t d, int dt, const void *p, const void *q) {
@@ -264,9 +357,9 @@ dim3 row_block(int64_t groups) {
   return dim3(x, kEmbThreads / x);
 }
 
-dim3 row_grid(int64_t rows, dim3 block) {
+dim3 row_grid(int64_t rows, dim3 block, int64_t tiles = 1) {
   const int64_t b = (rows + block.y - 1) / block.y;
-  return dim3(static_cast<unsigned>(b < 65536 ? b : 65536));
+  return dim3(static_cast<unsigned>(b < 65536 ? b : 65536), static_cast<unsigned>(tiles));
 }
 
 int check_embed(const char *what, int dt, int64_t n, int64_t v, int64_t d) {
@@ -338,23 +431,31 @@ extern "C" int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d,
   int32_t *begin = static_cast<int32_t *>(workspace);
   int32_t *sorted = ws_at<int32_t>(workspace, align_up((v + 1) * sizeof(int32_t)));
   const int range = static_cast<int>(sort_range(v));
-  hipLaunchKernelGGL(k_embed_sort, dim3(static_cast<unsigned>((v + range - 1) / range)), dim3(kSortThreads),
-                     static_cast<size_t>(range) * kSortWaves * sizeof(int32_t), s, ids, ids64, n, v, padding, range, begin,
-                     sorted);
+  const dim3 sgrid(static_cast<unsigned>((v + range - 1) / range)), sblock(kSortThreads);
+  const size_t lds = static_cast<size_t>(range) * kSortWaves * sizeof(int32_t);
+  if (ids64)
+    hipLaunchKernelGGL(k_embed_sort<int64_t>, sgrid, sblock, lds, s, static_cast<const int64_t *>(ids), n, v, range, begin, sorted);
+  else
+    hipLaunchKernelGGL(k_embed_sort<int32_t>, sgrid, sblock, lds, s, static_cast<const int32_t *>(ids), n, v, range, begin, sorted);
   SBOD_LAUNCHED("k_embed_sort");
   const int w = column_group(d, dtype, grad, grad_table);
   const dim3 block = row_block(d / w);
+  const int64_t tiles = (d / w + block.x - 1) / block.x;   // of a row's columns, a workgroup each
   const int rows = piece_rows(n);
   float *pieces = nullptr;
   if (n > rows) {   // (else no label can have come more often)
     const int64_t chunks = (n + rows - 1) / rows;
     pieces = ws_at<float>(workspace, align_up((v + 1) * sizeof(int32_t)) + align_up(n * sizeof(int32_t)));
-    SBOD_EMBED_LAUNCH(k_embed_pieces, dtype, w, row_grid(chunks, block), block, grad, ids, ids64, begin, sorted, v, chunks,
+    SBOD_EMBED_LAUNCH(k_embed_pieces, dtype, w, row_grid(chunks, block, tiles), block, grad, ids, ids64, begin, sorted, v, padding, chunks,
                       rows, d / w, pieces);
     SBOD_LAUNCHED("k_embed_pieces");
   }
-  SBOD_EMBED_LAUNCH(k_embed_grad, dtype, w, row_grid(v, block), block, grad, begin, sorted, v, rows, d / w, pieces, scale,
-                    grad_table);
+  if (wide_rows(v, d / w))
+    SBOD_EMBED_LAUNCH(k_embed_grad_wide, dtype, w, row_grid((v + 3) / 4, block, tiles), block, grad, begin, sorted, v,
+                      padding, rows, d / w, pieces, scale, grad_table);
+  else
+    SBOD_EMBED_LAUNCH(k_embed_grad_narrow, dtype, w, row_grid(v, block, tiles), block, grad, begin, sorted, v, padding,
+                      rows, d / w, pieces, scale, grad_table);
   SBOD_LAUNCHED("k_embed_grad");
   return SBOD_OK;
 }
