@@ -28,15 +28,18 @@ struct DistillArgs {
   const void *top;        // [n, k] of top_dt
   const float *lse;       // [n] or null
   const float *w;         // [n] or null
-  float *rows;            // [n] row losses (weighted), or for a reduction
-  double *rows64;         // in 64 bits: a mean holds where single rows are beyond float
+  float *rows;            // [n] row losses (weighted); for a reduction null, and
+  double *parts;          // what each row (k_distill_join) or workgroup adds to the loss, in 64 bits: a
+                          // mean holds where single rows are beyond float
+  const double *wparts;   // partial sums of the weights (k_distill_weights), or null
   float *stats;           // [n, kStats]
-  float *loss, *norm;     // the reduced loss, and the factor on each row's gradient; null: no reduction
+  float *loss, *norm;     // the reduced loss, and the factor on each row's gradient; null: 1
   float2 *part;           // [n, nchunk] {max, sum} of each chunk
   void *dx;               // [n, v], row stride lddx
   const float *up;        // upstream gradient, null for 1
   int64_t n, v, ldx, lddx, up_stride;
-  int k, ids64, top_dt, nchunk, reduction, skip_one;
+  int64_t nparts;
+  int k, ids64, top_dt, nchunk, nw, reduction, skip_one;
   float t, inv_t, s;      // temperature, 1 / T, log2(e) / T
   double inv_td;
 };
@@ -48,7 +51,7 @@ enum { kStM, kStL2s, kStMo, kStL2so, kStCoef, kStTb, kStTl, kStLive, kStats };
 __device__ __forceinline__ bool row_has_weight(const DistillArgs &a, int64_t r) { return !a.w || a.w[r] != 0.f; }
 
 __device__ __forceinline__ void put_row(const DistillArgs &a, int64_t r, double loss) {
-  if (a.rows64) a.rows64[r] = loss;
+  if (a.parts) a.parts[r] = loss;
   else a.rows[r] = static_cast<float>(loss);
 }
 
@@ -243,18 +246,33 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   }
 }
 
-// One block: {loss, norm} of the rows.  Sums in 64 bits, in a fixed order.
+// Partial sums of the row weights, in 64 bits and a fixed order.
+constexpr int kWeightParts = 64;
+__global__ __launch_bounds__(256) void k_distill_weights(const float *w, int64_t n, double *parts) {
+  __shared__ double red[16];
+  double sum = 0;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) sum += w[i];
+  sum = block_sum(sum, red);
+  if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+}
+
+// The factor on each row's gradient.  All lanes of a wave.
+__device__ __forceinline__ double norm_of(const DistillArgs &a) {
+  if (a.reduction != SBOD_REDUCE_MEAN) return 1.0;
+  if (!a.w) return 1.0 / static_cast<double>(a.n);
+  const int lane = threadIdx.x & 63;
+  const double w = wave_sum_f64(lane < a.nw ? a.wparts[lane] : 0.0);
+  return w == 0 ? 0.0 : 1.0 / w;
+}
+
+// One block: the reduced loss of its parts, and the norm for the gradient.
 __global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
   __shared__ double red[16];
-  double sum = 0, w = 0;
-  for (int64_t i = threadIdx.x; i < a.n; i += blockDim.x) {
-    sum += a.rows64[i];
-    if (a.w) w += a.w[i];
-  }
+  double sum = 0;
+  for (int64_t i = threadIdx.x; i < a.nparts; i += blockDim.x) sum += a.parts[i];
   sum = block_sum(sum, red);
-  w = a.w ? block_sum(w, red) : static_cast<double>(a.n);
+  const double norm = a.n == 0 ? 0.0 : norm_of(a);
   if (threadIdx.x == 0) {
-    const double norm = a.reduction == SBOD_REDUCE_MEAN ? (w == 0 ? 0.0 : 1.0 / w) : 1.0;
     *a.loss = static_cast<float>(norm == 0 ? 0.0 : sum * norm);
     *a.norm = static_cast<float>(norm);
   }
@@ -317,6 +335,203 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   }
 }
 
+// Reductions over a group of G lanes, valid in each of them.
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int m = G / 2; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, kWave));
+  return v;
+}
+template <int G, typename T>
+__device__ __forceinline__ T group_sum(T v) {
+#pragma unroll
+  for (int m = G / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ bool group_any(bool b) {
+  unsigned long long m = __ballot(b);
+  if (G < kWave) m = m >> ((threadIdx.x & 63) / G * G) & ((1ull << (G & 63)) - 1);
+  return m != 0;
+}
+
+// A vocabulary of at most G E labels: G lanes per row hold it in registers, label j G + lane in the lane's
+// slot j, so the logits are read once and the gradient written once, with the loss, in one launch.  The
+// teacher's masses lie in a table of the row in LDS (-1: not a kept label); a table is left as it was found.
+template <int DT, int G, int E, bool kBucket>
+__global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
+  using T = typename Elt<DT>::T;
+  constexpr int kRows = 256 / G;
+  extern __shared__ float tables[];   // [kRows][v]
+  __shared__ double red[16];
+  if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
+  const int lane = threadIdx.x % G, v = static_cast<int>(a.v), kk = a.k;
+  float *tab = tables + threadIdx.x / G * v;
+#pragma unroll
+  for (int j = 0; j < E; ++j)
+    if (j * G + lane < v) tab[j * G + lane] = -1.f;
+  const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
+  const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
+  double loss = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + threadIdx.x / G;
+  float w = a.w && r < a.n ? a.w[r] : 1.f;
+  for (; r < a.n; r += step) {
+    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+    T *drow = static_cast<T *>(a.dx) + r * a.lddx;
+    const float wr = w;
+    if (a.w && r + step < a.n) w = a.w[r + step];
+    bool live = wr != 0.f;
+    float f[E];
+    int id0 = -1;
+    float t0 = 0.f;
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[j] = j * G + lane < v ? static_cast<float>(row[j * G + lane]) : kNegInf;
+      if (lane < kk) {
+        id0 = ld_id(a.ids, r * kk + lane, a.ids64, a.v);
+        t0 = ld_any(a.top, r * kk + lane, a.top_dt);
+      }
+    }
+    const auto id_of = [&](int k) { return k < G ? id0 : ld_id(a.ids, r * kk + k, a.ids64, a.v); };
+    const auto top_of = [&](int k) { return k < G ? t0 : ld_any(a.top, r * kk + k, a.top_dt); };
+    // the teacher
+    float tb = 0.f, tl = 0.f;
+    if (live && kBucket) tl = a.lse[r];
+    if (!kBucket) {
+      float tm = kNegInf, sum = 0.f;
+      if (live)
+        for (int k = lane; k < kk; k += G)
+          if (id_of(k) >= 0) tm = fmaxf(tm, top_of(k));
+      tm = group_max<G>(tm);
+      tb = tm == kNegInf ? 0.f : tm;
+      if (live)
+        for (int k = lane; k < kk; k += G)
+          if (id_of(k) >= 0) sum += expf((top_of(k) - tb) * a.inv_t);
+      sum = group_sum<G>(sum);
+      live = live && !(sum == 0.f);
+      tl = logf(sum);
+    }
+    const auto logp_of = [&](int k) {
+      return static_cast<float>((static_cast<double>(top_of(k)) - tb) * a.inv_td - tl);
+    };
+    // its masses into the table; an entry whose label another entry took is found again
+    int *slot = reinterpret_cast<int *>(tab);
+    bool twice = false;
+    if (live)
+      for (int k = lane; k < kk; k += G)
+        if (id_of(k) >= 0) slot[id_of(k)] = k;
+    wave_lds_fence();
+    if (live)
+      for (int k = lane; k < kk; k += G) twice = twice || (id_of(k) >= 0 && slot[id_of(k)] != k);
+    twice = group_any<G>(twice);
+    wave_lds_fence();
+    double kl = 0;
+    float mass = 0.f;
+    if (live)
+      for (int k = lane; k < kk; k += G) {
+        const int id = id_of(k);
+        if (id < 0) continue;
+        const float logp = logp_of(k), p = expf(logp);
+        tab[id] = twice ? 0.f : p;
+        if (p != 0.f) kl += static_cast<double>(p) * logp;
+        mass += p;
+      }
+    wave_lds_fence();
+    if (twice)   // entry by entry: the sums' order is the list's
+      for (int k = 0; k < kk; ++k) {
+        if (k % G == lane && id_of(k) >= 0) tab[id_of(k)] += expf(logp_of(k));
+        wave_lds_fence();
+      }
+    // the student: maxima of the labels not kept (of all, without a bucket) and of the kept ones
+    float mo = kNegInf, mk = kNegInf;
+    bool others = false;
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const bool kept = kBucket && j * G + lane < v && !(tab[j * G + lane] < 0.f);
+        if (kept) mk = fmaxf(mk, f[j]);
+        else mo = fmaxf(mo, f[j]);
+        if (kBucket) others = others || (!kept && j * G + lane < v);
+      }
+    }
+    mo = group_max<G>(mo);
+    if (kBucket) {
+      mk = group_max<G>(mk);
+      others = group_any<G>(others);
+    }
+    const float m = fmaxf(mo, mk), base = m == kNegInf ? 0.f : m, obase = mo == kNegInf ? 0.f : mo;
+    float so = 0.f, sk = 0.f;
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const bool in = j * G + lane < v;
+        const float t = in ? tab[j * G + lane] : -1.f;
+        const bool kept = kBucket && !(t < 0.f);
+        if (in && !(t < 0.f) && t != 0.f)   // (in 64 bits: a label masked by the type's lowest value is finite)
+          kl -= static_cast<double>(t) * ((static_cast<double>(f[j]) - base) * a.inv_td);
+        f[j] = exp2_hw((f[j] - (kept ? base : obase)) * a.s);
+        if (kept) sk += f[j];
+        else so += f[j];
+      }
+    }
+    so = group_sum<G>(so);
+    if (kBucket) sk = group_sum<G>(sk);
+    const float sum = kBucket ? sk + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s)) : so;
+    // a row of -inf alone has no distribution: it is left out, as one of weight 0
+    live = live && !(m == kNegInf && sum == 0.f);
+    float coef = 1.f / so, rest = 0.f;   // what a label not kept takes of its exponential
+    if (live) {
+      const float logs = logf(sum);
+      mass = group_sum<G>(mass);
+      if (kBucket) {
+        rest = 1.f - mass;
+        // (no label outside the kept ones: what is left of the teacher's mass is rounding)
+        if (rest < 0.f || !others) rest = 0.f;
+        const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + logf(so) - logs;
+        if (lane == 0) kl += rest > 0.f ? rest * (logf(rest) - logo) : rest;
+        coef = so == 0.f ? 0.f : (expf(static_cast<float>(logo)) - rest) / so;
+      }
+      if (lane == 0) kl += static_cast<double>(mass) * logs;
+      kl *= static_cast<double>(a.t) * a.t * wr;
+    } else {
+      kl = 0;
+    }
+    if (a.rows) {
+      kl = group_sum<G>(kl);
+      if (lane == 0) a.rows[r] = static_cast<float>(kl);
+    }
+    loss += kl;
+    if (a.dx) {
+      float g = a.t * wr * norm * up;
+      if (a.up && a.up_stride) g *= a.up[r];
+      const float gs = g / sum;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        if (j * G + lane >= v) continue;
+        float d = 0.f;
+        if (live) {
+          const float t = tab[j * G + lane];
+          d = kBucket && t < 0.f ? g * (f[j] * coef) : t < 0.f ? f[j] * gs : g * (f[j] / sum - t);
+        }
+        drow[j * G + lane] = static_cast<T>(d);
+      }
+    }
+    wave_lds_fence();
+    if (wr != 0.f)
+      for (int k = lane; k < kk; k += G)
+        if (id_of(k) >= 0) tab[id_of(k)] = -1.f;
+    wave_lds_fence();
+  }
+  if (a.parts) {
+    loss = block_sum(loss, red);
+    if (threadIdx.x == 0) a.parts[blockIdx.x] = loss;
+  }
+}
+
+constexpr int kSmallMax = 2048;   // labels k_distill_small holds
+constexpr int kSmallBlocks = 2048;
+
 int distill_chunks(int64_t v, int dt) {
   const int64_t per = static_cast<int64_t>(kDistGran) * 16 / elt_bytes(dt);
   return static_cast<int>((v + 16 / elt_bytes(dt) - 1 + per - 1) / per);   // (a phase of P - 1 at most)
@@ -345,6 +560,56 @@ int launch_rows(const DistillArgs &a, hipStream_t s) {
   SBOD_LAUNCHED("k_distill_join");
   return SBOD_OK;
 }
+
+int64_t small_blocks(int64_t n, int g) {
+  const int64_t b = (n + 256 / g - 1) / (256 / g);
+  return b < kSmallBlocks ? b : kSmallBlocks;
+}
+int small_lanes(int64_t v) { return v <= 32 ? 8 : v <= 64 ? 16 : v <= 128 ? 32 : 64; }
+
+template <int DT, bool kBucket>
+int launch_small(const DistillArgs &a, hipStream_t s) {
+  const int g = small_lanes(a.v);
+  const dim3 grid(static_cast<unsigned>(small_blocks(a.n, g))), block(256);
+  const size_t lds = 256 / g * a.v * sizeof(float);
+#define SBOD_SMALL(G, E) hipLaunchKernelGGL((k_distill_small<DT, G, E, kBucket>), grid, block, lds, s, a)
+  if (a.v <= 32) SBOD_SMALL(8, 4);
+  else if (a.v <= 64) SBOD_SMALL(16, 4);
+  else if (a.v <= 128) SBOD_SMALL(32, 4);
+  else if (a.v <= 256) SBOD_SMALL(64, 4);
+  else if (a.v <= 512) SBOD_SMALL(64, 8);
+  else if (a.v <= 1024) SBOD_SMALL(64, 16);
+  else if (a.v <= 1536) SBOD_SMALL(64, 24);
+  else SBOD_SMALL(64, 32);
+#undef SBOD_SMALL
+  SBOD_LAUNCHED("k_distill_small");
+  return SBOD_OK;
+}
+
+// Which kernels take a call.
+enum Path { kSmall, kChunks };
+Path path_of(int64_t v) { return v <= kSmallMax ? kSmall : kChunks; }
+
+// The forward's, or with a.up the gradient's, launches of one type.
+template <int DT, bool kBucket>
+int launch_typed(const DistillArgs &a, hipStream_t s) {
+  if (path_of(a.v) == kSmall) return launch_small<DT, kBucket>(a, s);
+  if (!a.up) {
+    const int st = launch_rows<DT, kBucket>(a, s);
+    if (st != SBOD_OK) return st;
+  }
+  return SBOD_OK;
+}
+int launch_any(const DistillArgs &a, int dt, hipStream_t s) {
+  if (dt == SBOD_DT_F32) return a.lse ? launch_typed<SBOD_DT_F32, true>(a, s) : launch_typed<SBOD_DT_F32, false>(a, s);
+  if (dt == SBOD_DT_BF16) return a.lse ? launch_typed<SBOD_DT_BF16, true>(a, s) : launch_typed<SBOD_DT_BF16, false>(a, s);
+  return a.lse ? launch_typed<SBOD_DT_F16, true>(a, s) : launch_typed<SBOD_DT_F16, false>(a, s);
+}
+
+// The forward's workspace: partial weight sums | loss parts | chunk statistics.
+size_t parts_offset() { return kWeightParts * sizeof(double); }
+int64_t parts_count(int64_t n, int64_t v) { return path_of(v) == kSmall ? small_blocks(n, small_lanes(v)) : n; }
+size_t chunks_offset(int64_t n, int64_t v) { return align_up(parts_offset() + parts_count(n, v) * sizeof(double)); }
 
 int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, int64_t ldx, const void *ids,
                  const void *top, int top_dt, int k, float temperature, int reduction) {
@@ -375,8 +640,9 @@ using namespace sbod::label;
 extern "C" int sbod_distill_stat_floats(void) { return kStats; }
 
 extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int dtype) {
-  if (n <= 0 || v <= 0 || !known_dt(dtype)) return 0;
-  return align_up(static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2)) + static_cast<size_t>(n) * sizeof(double);
+  if (n < 0 || v <= 0 || !known_dt(dtype)) return 0;
+  const size_t chunks = path_of(v) == kChunks ? static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2) : 0;
+  return chunks_offset(n, v) + chunks;
 }
 
 extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -390,36 +656,37 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || (loss && norm), "sbod_distill_fwd: a reduction needs loss and norm");
   SBOD_REQUIRE(!grad || (grad_ld >= v && reduction != SBOD_REDUCE_NONE), "sbod_distill_fwd: gradient with row stride %lld, reduction %d",
                static_cast<long long>(grad_ld), reduction);
-  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, dtype) || (n > 0 && !workspace)) {
+  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, dtype) || !workspace) {
     set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, dtype));
     return SBOD_E_WORKSPACE;
   }
   hipStream_t s = as_stream(stream);
   DistillArgs a = {};
   a.x = logits, a.n = n, a.v = v, a.ldx = ld, a.ids = ids, a.ids64 = ids64, a.top = top, a.top_dt = top_dtype;
-  a.k = k, a.lse = lse, a.w = weights, a.rows = rows, a.stats = stats, a.reduction = reduction;
-  a.part = static_cast<float2 *>(workspace), a.nchunk = distill_chunks(v, dtype);
-  if (reduction != SBOD_REDUCE_NONE) {
-    a.loss = loss, a.norm = norm;
-    a.rows64 = ws_at<double>(workspace, align_up(static_cast<size_t>(n) * a.nchunk * sizeof(float2)));
-  }
+  a.k = k, a.lse = lse, a.w = weights, a.stats = stats, a.reduction = reduction;
+  a.rows = reduction == SBOD_REDUCE_NONE ? rows : nullptr;
+  a.part = ws_at<float2>(workspace, chunks_offset(n, v)), a.nchunk = distill_chunks(v, dtype);
   a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
+  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v);
+  if (reduction == SBOD_REDUCE_MEAN && weights) {
+    // (64 partial sums: each workgroup of the loss joins them)
+    a.wparts = static_cast<const double *>(workspace);
+    a.nw = static_cast<int>(n < kWeightParts * 256 ? (n + 255) / 256 : kWeightParts);
+    if (n > 0) {
+      hipLaunchKernelGGL(k_distill_weights, dim3(a.nw), dim3(256), 0, s, weights, n, static_cast<double *>(workspace));
+      SBOD_LAUNCHED("k_distill_weights");
+    }
+  }
   if (n > 0) {
-    int st;
-    if (dtype == SBOD_DT_F32)
-      st = lse ? launch_rows<SBOD_DT_F32, true>(a, s) : launch_rows<SBOD_DT_F32, false>(a, s);
-    else if (dtype == SBOD_DT_BF16)
-      st = lse ? launch_rows<SBOD_DT_BF16, true>(a, s) : launch_rows<SBOD_DT_BF16, false>(a, s);
-    else
-      st = lse ? launch_rows<SBOD_DT_F16, true>(a, s) : launch_rows<SBOD_DT_F16, false>(a, s);
+    const int st = launch_any(a, dtype, s);
     if (st != SBOD_OK) return st;
   }
-  if (a.loss) {
-    hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, s, a);
-    SBOD_LAUNCHED("k_distill_sum");
-  }
-  return grad && n > 0 ? launch_grad(a, dtype, s) : SBOD_OK;
+  if (reduction == SBOD_REDUCE_NONE) return SBOD_OK;
+  a.loss = loss, a.norm = norm;
+  hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, s, a);
+  SBOD_LAUNCHED("k_distill_sum");
+  return grad && n > 0 && path_of(v) == kChunks ? launch_grad(a, dtype, s) : SBOD_OK;
 }
 
 extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -441,5 +708,5 @@ extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_
   a.stats = const_cast<float *>(stats), a.up = upstream, a.up_stride = reduction == SBOD_REDUCE_NONE ? 1 : 0;
   a.nchunk = distill_chunks(v, dtype), a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
-  return launch_grad(a, dtype, as_stream(stream));
+  return path_of(v) == kSmall ? launch_any(a, dtype, as_stream(stream)) : launch_grad(a, dtype, as_stream(stream));
 }

@@ -213,15 +213,23 @@ __device__ __forceinline__ void add_rows(float (&acc)[kV], const T *grad, const 
   int at[kU];
 #pragma unroll
   for (int u = 0; u < kU; ++u) at[u] = sorted[min(b + u, e - 1)];
-  for (int i = b; i < e; i += kU) {
+  int i = b;
+  for (; i + kU <= e; i += kU) {   // whole batches: loads without a branch between them
+    V s[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) s[u] = reinterpret_cast<const V *>(grad + at[u] * d)[g];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) at[u] = sorted[min(i + kU + u, e - 1)];
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int j = 0; j < kV; ++j) acc[j] += static_cast<float>(s[u][j]);
+  }
+  if (i < e) {
     V s[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u)
       if (i + u < e) s[u] = reinterpret_cast<const V *>(grad + at[u] * d)[g];
-    if (i + kU < e) {
-#pragma unroll
-      for (int u = 0; u < kU; ++u) at[u] = sorted[min(i + kU + u, e - 1)];
-    }
 #pragma unroll
     for (int u = 0; u < kU; ++u)
       if (i + u < e) {
