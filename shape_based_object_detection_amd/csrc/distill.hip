@@ -335,70 +335,68 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   }
 }
 
-// Reductions over a group of G lanes, valid in each of them.
-template <int G>
-__device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int m = G / 2; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, kWave));
-  return v;
-}
-template <int G, typename T>
-__device__ __forceinline__ T group_sum(T v) {
-#pragma unroll
-  for (int m = G / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
-  return v;
-}
-template <int G>
-__device__ __forceinline__ bool group_any(bool b) {
-  unsigned long long m = __ballot(b);
-  if (G < kWave) m = m >> ((threadIdx.x & 63) / G * G) & ((1ull << (G & 63)) - 1);
-  return m != 0;
-}
-
 // A vocabulary of at most G E labels: G lanes per row hold it in registers, label j G + lane in the lane's
 // slot j, so the logits are read once and the gradient written once, with the loss, in one launch.  The
-// teacher's masses lie in a table of the row in LDS (-1: not a kept label); a table is left as it was found.
+// kept labels are K values beside it: lane k holds entry k (and k + G, ...), its logit gathered from the row.
+// With a bucket they leave the row by a bit mask per lane; their gradients overwrite the row's.
 template <int DT, int G, int E, bool kBucket>
 __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
   using T = typename Elt<DT>::T;
   constexpr int kRows = 256 / G;
-  extern __shared__ float tables[];   // [kRows][v]
+  __shared__ uint32_t masks[256];   // bit j of a lane's word: its slot j is a kept label
   __shared__ double red[16];
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int lane = threadIdx.x % G, v = static_cast<int>(a.v), kk = a.k;
-  float *tab = tables + threadIdx.x / G * v;
-#pragma unroll
-  for (int j = 0; j < E; ++j)
-    if (j * G + lane < v) tab[j * G + lane] = -1.f;
+  uint32_t *mask = masks + threadIdx.x / G * G;
+  mask[lane] = 0;
   const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
   const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
   double loss = 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
-  int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + threadIdx.x / G;
-  float w = a.w && r < a.n ? a.w[r] : 1.f;
+  int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + (G == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G);
+  // a row's weight and first G entries are loaded a row ahead
+  float w_next = 1.f, t_next = 0.f;
+  int id_next = -1;
+  const auto ahead = [&](int64_t q) {
+    if (q >= a.n) return;
+    if (a.w) w_next = a.w[q];
+    if (lane < kk) {
+      id_next = ld_id(a.ids, q * kk + lane, a.ids64, a.v);
+      t_next = ld_any(a.top, q * kk + lane, a.top_dt);
+    }
+  };
+  ahead(r);
   for (; r < a.n; r += step) {
     const T *row = static_cast<const T *>(a.x) + r * a.ldx;
-    T *drow = static_cast<T *>(a.dx) + r * a.lddx;
-    const float wr = w;
-    if (a.w && r + step < a.n) w = a.w[r + step];
-    bool live = wr != 0.f;
-    float f[E];
-    int id0 = -1;
-    float t0 = 0.f;
+    const float w = w_next, t0 = t_next;
+    const int id0 = id_next;
+    bool live = w != 0.f;
+    // (loads first, conversions behind them: a conversion next to its load would wait for it)
+    T raw[E];
+    T xraw = static_cast<T>(0.f);
+#pragma unroll
+    for (int j = 0; j < E; ++j) raw[j] = static_cast<T>(kNegInf);
     if (live) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) f[j] = j * G + lane < v ? static_cast<float>(row[j * G + lane]) : kNegInf;
-      if (lane < kk) {
-        id0 = ld_id(a.ids, r * kk + lane, a.ids64, a.v);
-        t0 = ld_any(a.top, r * kk + lane, a.top_dt);
+      for (int j = 0; j < E; ++j) {
+        if ((j + 1) * G <= v) raw[j] = row[j * G + lane];
+        else if (j * G + lane < v) raw[j] = row[j * G + lane];
       }
+      if (id0 >= 0) xraw = row[id0];
     }
+    ahead(r + step);
+    float f[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = static_cast<float>(raw[j]);
+    const float x0 = static_cast<float>(xraw);
     const auto id_of = [&](int k) { return k < G ? id0 : ld_id(a.ids, r * kk + k, a.ids64, a.v); };
     const auto top_of = [&](int k) { return k < G ? t0 : ld_any(a.top, r * kk + k, a.top_dt); };
+    const auto x_of = [&](int k, int id) { return k < G ? x0 : static_cast<float>(row[id]); };
     // the teacher
     float tb = 0.f, tl = 0.f;
-    if (live && kBucket) tl = a.lse[r];
-    if (!kBucket) {
+    if (kBucket) {
+      if (live) tl = a.lse[r];
+    } else {
       float tm = kNegInf, sum = 0.f;
       if (live)
         for (int k = lane; k < kk; k += G)
@@ -407,53 +405,40 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
       tb = tm == kNegInf ? 0.f : tm;
       if (live)
         for (int k = lane; k < kk; k += G)
-          if (id_of(k) >= 0) sum += expf((top_of(k) - tb) * a.inv_t);
+          if (id_of(k) >= 0) sum += exp_hw((top_of(k) - tb) * a.inv_t);
       sum = group_sum<G>(sum);
       live = live && !(sum == 0.f);
-      tl = logf(sum);
+      tl = log_hw(sum);
     }
-    const auto logp_of = [&](int k) {
-      return static_cast<float>((static_cast<double>(top_of(k)) - tb) * a.inv_td - tl);
-    };
-    // its masses into the table; an entry whose label another entry took is found again
-    int *slot = reinterpret_cast<int *>(tab);
+    const auto logp_at = [&](float t) { return static_cast<float>((static_cast<double>(t) - tb) * a.inv_td - tl); };
+    // the kept labels' bits; a label that is there already is listed twice
     bool twice = false;
-    if (live)
-      for (int k = lane; k < kk; k += G)
-        if (id_of(k) >= 0) slot[id_of(k)] = k;
-    wave_lds_fence();
-    if (live)
-      for (int k = lane; k < kk; k += G) twice = twice || (id_of(k) >= 0 && slot[id_of(k)] != k);
-    twice = group_any<G>(twice);
-    wave_lds_fence();
-    double kl = 0;
-    float mass = 0.f;
+    float mk = kNegInf;
     if (live)
       for (int k = lane; k < kk; k += G) {
         const int id = id_of(k);
         if (id < 0) continue;
-        const float logp = logp_of(k), p = expf(logp);
-        tab[id] = twice ? 0.f : p;
-        if (p != 0.f) kl += static_cast<double>(p) * logp;
-        mass += p;
+        const uint32_t bit = 1u << (id / G);
+        twice = (atomicOr(&mask[id % G], bit) & bit) || twice;
+        if (kBucket) mk = fmaxf(mk, x_of(k, id));
       }
+    twice = group_any<G>(twice);
     wave_lds_fence();
-    if (twice)   // entry by entry: the sums' order is the list's
-      for (int k = 0; k < kk; ++k) {
-        if (k % G == lane && id_of(k) >= 0) tab[id_of(k)] += expf(logp_of(k));
-        wave_lds_fence();
-      }
-    // the student: maxima of the labels not kept (of all, without a bucket) and of the kept ones
-    float mo = kNegInf, mk = kNegInf;
+    const uint32_t mine = mask[lane];
+    wave_lds_fence();
+    mask[lane] = 0;
+    // the student: the row's labels, with a bucket those not kept
+    float mo = kNegInf;
     bool others = false;
-    if (live) {
+    if (kBucket) {
+      // (slots of the lane that hold a label: j G + lane < v)
+      const int held = v > lane ? (v - lane + G - 1) / G : 0;
+      others = held > 0 && (~mine & (0xffffffffu >> (32 - held))) != 0;
+    }
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const bool kept = kBucket && j * G + lane < v && !(tab[j * G + lane] < 0.f);
-        if (kept) mk = fmaxf(mk, f[j]);
-        else mo = fmaxf(mo, f[j]);
-        if (kBucket) others = others || (!kept && j * G + lane < v);
-      }
+    for (int j = 0; j < E; ++j) {
+      if (kBucket && (mine >> j & 1)) f[j] = kNegInf;
+      mo = fmaxf(mo, f[j]);
     }
     mo = group_max<G>(mo);
     if (kBucket) {
@@ -462,66 +447,83 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     }
     const float m = fmaxf(mo, mk), base = m == kNegInf ? 0.f : m, obase = mo == kNegInf ? 0.f : mo;
     float so = 0.f, sk = 0.f;
-    if (live) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const bool in = j * G + lane < v;
-        const float t = in ? tab[j * G + lane] : -1.f;
-        const bool kept = kBucket && !(t < 0.f);
-        if (in && !(t < 0.f) && t != 0.f)   // (in 64 bits: a label masked by the type's lowest value is finite)
-          kl -= static_cast<double>(t) * ((static_cast<double>(f[j]) - base) * a.inv_td);
-        f[j] = exp2_hw((f[j] - (kept ? base : obase)) * a.s);
-        if (kept) sk += f[j];
-        else so += f[j];
-      }
+    for (int j = 0; j < E; ++j) {
+      f[j] = exp2_hw((f[j] - obase) * a.s);
+      so += f[j];
     }
     so = group_sum<G>(so);
-    if (kBucket) sk = group_sum<G>(sk);
-    const float sum = kBucket ? sk + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s)) : so;
+    // an entry's place among those of its label: the sums' order is the list's
+    const auto earlier = [&](int k, int id) {
+      for (int i = 0; i < k; ++i)
+        if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) return true;
+      return false;
+    };
+    float sum = so, mass = 0.f;
+    if (kBucket) {
+      if (live)
+        for (int k = lane; k < kk; k += G) {
+          const int id = id_of(k);
+          if (id < 0) continue;
+          if (!twice || !earlier(k, id)) sk += exp2_hw((x_of(k, id) - base) * a.s);
+          mass += exp_hw(logp_at(top_of(k)));
+        }
+      sk = group_sum<G>(sk);
+      mass = group_sum<G>(mass);
+      sum = sk + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
+    }
     // a row of -inf alone has no distribution: it is left out, as one of weight 0
     live = live && !(m == kNegInf && sum == 0.f);
-    float coef = 1.f / so, rest = 0.f;   // what a label not kept takes of its exponential
+    const float logs = log_hw(sum);
+    float coef = 1.f / sum;   // what a label not kept takes of its exponential
+    double kl = 0;
     if (live) {
-      const float logs = logf(sum);
-      mass = group_sum<G>(mass);
+      // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
+      for (int k = lane; k < kk; k += G) {
+        const int id = id_of(k);
+        if (id < 0) continue;
+        const float logp = logp_at(top_of(k)), p = exp_hw(logp);
+        if (p != 0.f) kl += p * (logp - ((static_cast<double>(x_of(k, id)) - base) * a.inv_td - logs));
+      }
       if (kBucket) {
-        rest = 1.f - mass;
+        float rest = 1.f - mass;
         // (no label outside the kept ones: what is left of the teacher's mass is rounding)
         if (rest < 0.f || !others) rest = 0.f;
-        const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + logf(so) - logs;
-        if (lane == 0) kl += rest > 0.f ? rest * (logf(rest) - logo) : rest;
-        coef = so == 0.f ? 0.f : (expf(static_cast<float>(logo)) - rest) / so;
+        const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + log_hw(so) - logs;
+        if (lane == 0) kl += rest > 0.f ? rest * (log_hw(rest) - logo) : rest;
+        coef = so == 0.f ? 0.f : (exp_hw(static_cast<float>(logo)) - rest) / so;
       }
-      if (lane == 0) kl += static_cast<double>(mass) * logs;
-      kl *= static_cast<double>(a.t) * a.t * wr;
-    } else {
-      kl = 0;
+      kl *= static_cast<double>(a.t) * a.t * w;
     }
     if (a.rows) {
       kl = group_sum<G>(kl);
       if (lane == 0) a.rows[r] = static_cast<float>(kl);
     }
     loss += kl;
-    if (a.dx) {
-      float g = a.t * wr * norm * up;
-      if (a.up && a.up_stride) g *= a.up[r];
-      const float gs = g / sum;
+    if (!a.dx) continue;
+    T *drow = static_cast<T *>(a.dx) + r * a.lddx;
+    float g = a.t * w * norm * up;
+    if (a.up && a.up_stride) g *= a.up[r];
+    const float gc = g * coef;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        if (j * G + lane >= v) continue;
-        float d = 0.f;
-        if (live) {
-          const float t = tab[j * G + lane];
-          d = kBucket && t < 0.f ? g * (f[j] * coef) : t < 0.f ? f[j] * gs : g * (f[j] / sum - t);
-        }
-        drow[j * G + lane] = static_cast<T>(d);
-      }
+    for (int j = 0; j < E; ++j) {
+      const T d = static_cast<T>(live ? f[j] * gc : 0.f);
+      if ((j + 1) * G <= v) drow[j * G + lane] = d;
+      else if (j * G + lane < v) drow[j * G + lane] = d;
     }
-    wave_lds_fence();
-    if (wr != 0.f)
-      for (int k = lane; k < kk; k += G)
-        if (id_of(k) >= 0) tab[id_of(k)] = -1.f;
-    wave_lds_fence();
+    wave_lds_fence();   // (the same addresses again, by the lanes that hold the entries)
+    if (live)
+      for (int k = lane; k < kk; k += G) {
+        const int id = id_of(k);
+        if (id < 0) continue;
+        float p = exp_hw(logp_at(top_of(k)));
+        if (twice) {
+          p = 0.f;
+          for (int i = 0; i < kk; ++i)
+            if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) p += exp_hw(logp_at(ld_any(a.top, r * kk + i, a.top_dt)));
+        }
+        drow[id] = static_cast<T>(g * (exp2_hw((x_of(k, id) - base) * a.s) / sum - p));
+      }
   }
   if (a.parts) {
     loss = block_sum(loss, red);
@@ -571,8 +573,7 @@ template <int DT, bool kBucket>
 int launch_small(const DistillArgs &a, hipStream_t s) {
   const int g = small_lanes(a.v);
   const dim3 grid(static_cast<unsigned>(small_blocks(a.n, g))), block(256);
-  const size_t lds = 256 / g * a.v * sizeof(float);
-#define SBOD_SMALL(G, E) hipLaunchKernelGGL((k_distill_small<DT, G, E, kBucket>), grid, block, lds, s, a)
+#define SBOD_SMALL(G, E) hipLaunchKernelGGL((k_distill_small<DT, G, E, kBucket>), grid, block, 0, s, a)
   if (a.v <= 32) SBOD_SMALL(8, 4);
   else if (a.v <= 64) SBOD_SMALL(16, 4);
   else if (a.v <= 128) SBOD_SMALL(32, 4);

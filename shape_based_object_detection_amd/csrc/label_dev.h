@@ -94,14 +94,62 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, kWave));
+// Reductions over aligned groups of G lanes (a power of two), valid in each lane, without LDS: quad swaps
+// and mirrors inside a row of 16 (DPP), then gfx950's row and half swaps: permlane16_swap of v with itself
+// gives {row 0, row 0, row 2, row 2} and {row 1, row 1, row 3, row 3}, permlane32_swap the halves likewise.
+// All lanes of a group take part; other groups of the wave need not.
+template <int kCtrl>
+__device__ __forceinline__ float dpp_row(float v) {
+  const int x = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(x, x, kCtrl, 0xf, 0xf, false));
+}
+template <int G, typename Op>
+__device__ __forceinline__ float group_reduce(float v, Op op) {
+  if (G >= 2) v = op(v, dpp_row<0xB1>(v));     // quad_perm [1,0,3,2]
+  if (G >= 4) v = op(v, dpp_row<0x4E>(v));     // quad_perm [2,3,0,1]
+  if (G >= 8) v = op(v, dpp_row<0x141>(v));    // row_half_mirror
+  if (G >= 16) v = op(v, dpp_row<0x140>(v));   // row_mirror
+  if (G >= 32) {
+    const unsigned x = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const unsigned a = r[0], b = r[1];   // (a bit cast of a vector's element takes its first one)
+    v = op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+  }
+  if (G >= 64) {
+    const unsigned x = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const unsigned a = r[0], b = r[1];   // (a bit cast of a vector's element takes its first one)
+    v = op(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+  }
   return v;
 }
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+  return group_reduce<G>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+  return group_reduce<G>(v, [](float a, float b) { return a + b; });
+}
+template <int G>
+__device__ __forceinline__ double group_sum(double v) {
+#pragma unroll
+  for (int m = G / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ bool group_any(bool b) {
+  unsigned long long m = __ballot(b);
+  if (G < kWave) m = m >> ((threadIdx.x & 63) / G * G) & ((1ull << (G & 63)) - 1);
+  return m != 0;
+}
+__device__ __forceinline__ float wave_max_f32(float v) { return group_max<kWave>(v); }
 
 // 2^x by the hardware instruction (1 ulp; results below 2^-126 are 0).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+// e^x and log x from it and from the hardware's log2 (1 ulp): e^x is off by |x| half steps more.
+__device__ __forceinline__ float exp_hw(float x) { return exp2_hw(x * 1.44269504088896340736f); }
+__device__ __forceinline__ float log_hw(float x) { return __builtin_amdgcn_logf(x) * 0.693147180559945309417f; }
 
 }  // namespace label
 }  // namespace sbod
