@@ -41,7 +41,7 @@ struct DistillArgs {
   int64_t nparts;
   int k, ids64, top_dt, nchunk, nw, reduction, skip_one;
   float t, inv_t, s;      // temperature, 1 / T, log2(e) / T
-  double inv_td;
+  double inv_td, tt;      // 1 / T, T^2
 };
 
 // What a row leaves for its gradient: q_v = 2^((x - m) s - l2s); another label than the kept ones
@@ -248,10 +248,16 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
 
 // Partial sums of the row weights, in 64 bits and a fixed order.
 constexpr int kWeightParts = 64;
-__global__ __launch_bounds__(256) void k_distill_weights(const float *w, int64_t n, double *parts) {
+__global__ __launch_bounds__(1024) void k_distill_weights(const float *w, int64_t n, double *parts) {
   __shared__ double red[16];
   double sum = 0;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) sum += w[i];
+  const int64_t step = gridDim.x * 1024ll;
+  int64_t i = blockIdx.x * 1024ll + threadIdx.x;
+  for (; i + 3 * step < n; i += 4 * step) {
+    const float a = w[i], b = w[i + step], c = w[i + 2 * step], d = w[i + 3 * step];
+    sum += static_cast<double>(a) + b + (static_cast<double>(c) + d);
+  }
+  for (; i < n; i += step) sum += w[i];
   sum = block_sum(sum, red);
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
@@ -337,103 +343,122 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
 
 // A vocabulary of at most G E labels: G lanes per row hold it in registers, label j G + lane in the lane's
 // slot j, so the logits are read once and the gradient written once, with the loss, in one launch.  The
-// kept labels are K values beside it: lane k holds entry k (and k + G, ...), its logit gathered from the row.
-// With a bucket they leave the row by a bit mask per lane; their gradients overwrite the row's.
-template <int DT, int G, int E, bool kBucket>
+// kept labels are K values beside it: lane k holds entry k (kMore: entries from G on are taken up again where
+// they are needed; their code costs the others registers), its logit gathered from the row.  A bit mask per lane says which of its slots are kept
+// labels: with a bucket they leave the row's sum, and their gradients come by a table in LDS.
+// Slots that every vocabulary of a (G, E) fills are read and written without a test.
+template <int DT, int G, int E, bool kBucket, bool kMore>
 __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
   using T = typename Elt<DT>::T;
-  constexpr int kRows = 256 / G;
+  constexpr int kRows = 256 / G, kFull = E > 8 ? E - 8 : E == 8 ? 4 : 0;   // (launch_small)
   __shared__ uint32_t masks[256];   // bit j of a lane's word: its slot j is a kept label
+  __shared__ float kept[256 * E];   // the gradients of the kept labels, at their places in the row
   __shared__ double red[16];
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int lane = threadIdx.x % G, v = static_cast<int>(a.v), kk = a.k;
   uint32_t *mask = masks + threadIdx.x / G * G;
+  float *own = kept + threadIdx.x / G * (G * E);
   mask[lane] = 0;
   const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
   const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
   double loss = 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
-  int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + (G == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G);
+  int64_t r = blockIdx.x * static_cast<int64_t>(kRows) +
+              (G == kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G);
   // a row's weight and first G entries are loaded a row ahead
-  float w_next = 1.f, t_next = 0.f;
-  int id_next = -1;
+  float w_next = 1.f;
+  RawAny t_next = {};
+  RawId id_next = {~0u, ~0u};
   const auto ahead = [&](int64_t q) {
     if (q >= a.n) return;
     if (a.w) w_next = a.w[q];
-    if (lane < kk) {
-      id_next = ld_id(a.ids, q * kk + lane, a.ids64, a.v);
-      t_next = ld_any(a.top, q * kk + lane, a.top_dt);
-    }
+    const int64_t at = q * kk + min(lane, kk - 1);
+    id_next = ld_raw_id(a.ids, at, a.ids64);
+    t_next = ld_raw_any(a.top, at, a.top_dt);
   };
   ahead(r);
-  for (; r < a.n; r += step) {
-    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
-    const float w = w_next, t0 = t_next;
-    const int id0 = id_next;
+  const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+  T *drow = static_cast<T *>(a.dx) + r * a.lddx;
+  for (; r < a.n; r += step, row += step * a.ldx, drow += step * a.lddx) {
+    const float w = w_next, t0 = any_of(t_next, a.top_dt);
+    const int id0 = lane < kk ? id_of(id_next, a.ids64, a.v) : -1;
     bool live = w != 0.f;
-    // (loads first, conversions behind them: a conversion next to its load would wait for it)
-    T raw[E];
-    T xraw = static_cast<T>(0.f);
-#pragma unroll
-    for (int j = 0; j < E; ++j) raw[j] = static_cast<T>(kNegInf);
+    // (all loads in one block and none used in it: they are in flight together)
+    uint32_t raw[E], xraw = 0;
     if (live) {
+      const auto bits = [&](int i) {   // (a 32-bit offset from the row's base)
+        return *reinterpret_cast<const bits_t<DT> *>(reinterpret_cast<const char *>(row) +
+                                                     static_cast<uint32_t>(i) * static_cast<uint32_t>(sizeof(T)));
+      };
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        if ((j + 1) * G <= v) raw[j] = row[j * G + lane];
-        else if (j * G + lane < v) raw[j] = row[j * G + lane];
-      }
-      if (id0 >= 0) xraw = row[id0];
+      for (int j = 0; j < E; ++j) raw[j] = bits(j < kFull ? j * G + lane : min(j * G + lane, v - 1));
+      xraw = bits(max(id0, 0));
     }
     ahead(r + step);
     float f[E];
+    if (__ballot(live) == 0) {   // no row of this wave has a weight
+      if (a.rows && lane == 0) a.rows[r] = 0.f;
+      if (a.dx)
 #pragma unroll
-    for (int j = 0; j < E; ++j) f[j] = static_cast<float>(raw[j]);
-    const float x0 = static_cast<float>(xraw);
-    const auto id_of = [&](int k) { return k < G ? id0 : ld_id(a.ids, r * kk + k, a.ids64, a.v); };
-    const auto top_of = [&](int k) { return k < G ? t0 : ld_any(a.top, r * kk + k, a.top_dt); };
-    const auto x_of = [&](int k, int id) { return k < G ? x0 : static_cast<float>(row[id]); };
+        for (int j = 0; j < E; ++j)
+          if (j < kFull || j * G + lane < v) drow[j * G + lane] = static_cast<T>(0.f);
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = live && (j < kFull || j * G + lane < v) ? bits_value<DT>(raw[j]) : kNegInf;
+    const float x0 = bits_value<DT>(xraw);
+    const bool has0 = live && id0 >= 0;
+    // the entries from G on, of a live row: f(id, teacher's logit, student's)
+    const auto more = [&](auto &&f) {
+      if (kMore && live)
+        for (int k = lane + G; k < kk; k += G) {
+          const int id = ld_id(a.ids, r * kk + k, a.ids64, a.v);
+          if (id >= 0) f(k, id, ld_any(a.top, r * kk + k, a.top_dt), static_cast<float>(row[id]));
+        }
+    };
     // the teacher
     float tb = 0.f, tl = 0.f;
     if (kBucket) {
       if (live) tl = a.lse[r];
     } else {
-      float tm = kNegInf, sum = 0.f;
-      if (live)
-        for (int k = lane; k < kk; k += G)
-          if (id_of(k) >= 0) tm = fmaxf(tm, top_of(k));
+      float tm = has0 ? t0 : kNegInf, sum;
+      more([&](int, int, float t, float) { tm = fmaxf(tm, t); });
       tm = group_max<G>(tm);
       tb = tm == kNegInf ? 0.f : tm;
-      if (live)
-        for (int k = lane; k < kk; k += G)
-          if (id_of(k) >= 0) sum += exp_hw((top_of(k) - tb) * a.inv_t);
+      sum = has0 ? exp_hw((t0 - tb) * a.inv_t) : 0.f;
+      more([&](int, int, float t, float) { sum += exp_hw((t - tb) * a.inv_t); });
       sum = group_sum<G>(sum);
       live = live && !(sum == 0.f);
       tl = log_hw(sum);
     }
+    // (the difference in 64 bits: with lse, t / T and lse are large against it)
     const auto logp_at = [&](float t) { return static_cast<float>((static_cast<double>(t) - tb) * a.inv_td - tl); };
+    const float logp0 = logp_at(t0), p0 = has0 ? exp_hw(logp0) : 0.f;
     // the kept labels' bits; a label that is there already is listed twice
     bool twice = false;
-    float mk = kNegInf;
-    if (live)
-      for (int k = lane; k < kk; k += G) {
-        const int id = id_of(k);
-        if (id < 0) continue;
-        const uint32_t bit = 1u << (id / G);
-        twice = (atomicOr(&mask[id % G], bit) & bit) || twice;
-        if (kBucket) mk = fmaxf(mk, x_of(k, id));
-      }
+    if (has0) {
+      const uint32_t bit = 1u << (id0 / G);
+      twice = atomicOr(&mask[id0 % G], bit) & bit;
+    }
+    more([&](int, int id, float, float) {
+      const uint32_t bit = 1u << (id / G);
+      twice = (atomicOr(&mask[id % G], bit) & bit) || twice;
+    });
     twice = group_any<G>(twice);
     wave_lds_fence();
     const uint32_t mine = mask[lane];
     wave_lds_fence();
     mask[lane] = 0;
     // the student: the row's labels, with a bucket those not kept
-    float mo = kNegInf;
+    float mo = kNegInf, mk = kNegInf;
     bool others = false;
     if (kBucket) {
       // (slots of the lane that hold a label: j G + lane < v)
       const int held = v > lane ? (v - lane + G - 1) / G : 0;
-      others = held > 0 && (~mine & (0xffffffffu >> (32 - held))) != 0;
+      others = group_any<G>(held > 0 && (~mine & (0xffffffffu >> (32 - held))) != 0);
+      if (has0) mk = x0;
+      more([&](int, int, float, float x) { mk = fmaxf(mk, x); });
+      mk = group_max<G>(mk);
     }
 #pragma unroll
     for (int j = 0; j < E; ++j) {
@@ -441,89 +466,79 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
       mo = fmaxf(mo, f[j]);
     }
     mo = group_max<G>(mo);
-    if (kBucket) {
-      mk = group_max<G>(mk);
-      others = group_any<G>(others);
-    }
     const float m = fmaxf(mo, mk), base = m == kNegInf ? 0.f : m, obase = mo == kNegInf ? 0.f : mo;
-    float so = 0.f, sk = 0.f;
+    float so = 0.f;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       f[j] = exp2_hw((f[j] - obase) * a.s);
       so += f[j];
     }
     so = group_sum<G>(so);
-    // an entry's place among those of its label: the sums' order is the list's
-    const auto earlier = [&](int k, int id) {
-      for (int i = 0; i < k; ++i)
-        if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) return true;
-      return false;
-    };
+    const float e0 = has0 ? exp2_hw((x0 - base) * a.s) : 0.f;
     float sum = so, mass = 0.f;
     if (kBucket) {
-      if (live)
-        for (int k = lane; k < kk; k += G) {
-          const int id = id_of(k);
-          if (id < 0) continue;
-          if (!twice || !earlier(k, id)) sk += exp2_hw((x_of(k, id) - base) * a.s);
-          mass += exp_hw(logp_at(top_of(k)));
-        }
+      // (a label listed twice counts once, at its first entry: the sums' order is the list's)
+      const auto first = [&](int k, int id) {
+        for (int i = 0; i < k; ++i)
+          if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) return false;
+        return true;
+      };
+      float sk = has0 && (!twice || first(lane, id0)) ? e0 : 0.f;
+      mass = p0;
+      more([&](int k, int id, float t, float x) {
+        if (!twice || first(k, id)) sk += exp2_hw((x - base) * a.s);
+        mass += exp_hw(logp_at(t));
+      });
       sk = group_sum<G>(sk);
       mass = group_sum<G>(mass);
       sum = sk + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
     }
     // a row of -inf alone has no distribution: it is left out, as one of weight 0
     live = live && !(m == kNegInf && sum == 0.f);
-    const float logs = log_hw(sum);
-    float coef = 1.f / sum;   // what a label not kept takes of its exponential
-    double kl = 0;
-    if (live) {
-      // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
-      for (int k = lane; k < kk; k += G) {
-        const int id = id_of(k);
-        if (id < 0) continue;
-        const float logp = logp_at(top_of(k)), p = exp_hw(logp);
-        if (p != 0.f) kl += p * (logp - ((static_cast<double>(x_of(k, id)) - base) * a.inv_td - logs));
-      }
-      if (kBucket) {
-        float rest = 1.f - mass;
-        // (no label outside the kept ones: what is left of the teacher's mass is rounding)
-        if (rest < 0.f || !others) rest = 0.f;
-        const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + log_hw(so) - logs;
-        if (lane == 0) kl += rest > 0.f ? rest * (log_hw(rest) - logo) : rest;
-        coef = so == 0.f ? 0.f : (exp_hw(static_cast<float>(logo)) - rest) / so;
-      }
-      kl *= static_cast<double>(a.t) * a.t * w;
+    const float logs = log_hw(sum), inv = 1.f / sum;
+    float coef = inv;   // what a label not kept takes of its exponential
+    // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
+    const auto term = [&](float p, float logp, float x) {   // 0 log 0 = 0
+      return p == 0.f ? 0.0 : p * (logp - ((static_cast<double>(x) - base) * a.inv_td - logs));
+    };
+    double kl = has0 ? term(p0, logp0, x0) : 0.0;
+    more([&](int, int, float t, float x) { kl += term(exp_hw(logp_at(t)), logp_at(t), x); });
+    if (kBucket) {
+      float rest = 1.f - mass;
+      // (no label outside the kept ones: what is left of the teacher's mass is rounding)
+      if (rest < 0.f || !others) rest = 0.f;
+      const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + log_hw(so) - logs;
+      if (lane == 0) kl += rest > 0.f ? rest * (log_hw(rest) - logo) : rest;
+      coef = so == 0.f ? 0.f : (exp_hw(static_cast<float>(logo)) - rest) / so;
     }
+    kl = live ? kl * a.tt * w : 0.0;
     if (a.rows) {
       kl = group_sum<G>(kl);
       if (lane == 0) a.rows[r] = static_cast<float>(kl);
     }
     loss += kl;
     if (!a.dx) continue;
-    T *drow = static_cast<T *>(a.dx) + r * a.lddx;
     float g = a.t * w * norm * up;
     if (a.up && a.up_stride) g *= a.up[r];
+    const auto mass_of = [&](int id, float p) {
+      if (!twice) return p;
+      p = 0.f;
+      for (int i = 0; i < kk; ++i)
+        if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) p += exp_hw(logp_at(ld_any(a.top, r * kk + i, a.top_dt)));
+      return p;
+    };
+    if (has0) own[id0] = g * (e0 * inv - mass_of(id0, p0));
+    more([&](int, int id, float t, float x) {
+      own[id] = g * (exp2_hw((x - base) * a.s) * inv - mass_of(id, exp_hw(logp_at(t))));
+    });
+    wave_lds_fence();
     const float gc = g * coef;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const T d = static_cast<T>(live ? f[j] * gc : 0.f);
-      if ((j + 1) * G <= v) drow[j * G + lane] = d;
-      else if (j * G + lane < v) drow[j * G + lane] = d;
+      const float at = own[j * G + lane], d = mine >> j & 1 ? at : f[j] * gc;
+      if (j < kFull || j * G + lane < v) drow[j * G + lane] = static_cast<T>(live ? d : 0.f);
     }
-    wave_lds_fence();   // (the same addresses again, by the lanes that hold the entries)
-    if (live)
-      for (int k = lane; k < kk; k += G) {
-        const int id = id_of(k);
-        if (id < 0) continue;
-        float p = exp_hw(logp_at(top_of(k)));
-        if (twice) {
-          p = 0.f;
-          for (int i = 0; i < kk; ++i)
-            if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) p += exp_hw(logp_at(ld_any(a.top, r * kk + i, a.top_dt)));
-        }
-        drow[id] = static_cast<T>(g * (exp2_hw((x_of(k, id) - base) * a.s) / sum - p));
-      }
+    wave_lds_fence();
   }
   if (a.parts) {
     loss = block_sum(loss, red);
@@ -532,7 +547,7 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
 }
 
 constexpr int kSmallMax = 2048;   // labels k_distill_small holds
-constexpr int kSmallBlocks = 2048;
+constexpr int kSmallBlocks = 1280;
 
 int distill_chunks(int64_t v, int dt) {
   const int64_t per = static_cast<int64_t>(kDistGran) * 16 / elt_bytes(dt);
@@ -567,21 +582,29 @@ int64_t small_blocks(int64_t n, int g) {
   const int64_t b = (n + 256 / g - 1) / (256 / g);
   return b < kSmallBlocks ? b : kSmallBlocks;
 }
-int small_lanes(int64_t v) { return v <= 32 ? 8 : v <= 64 ? 16 : v <= 128 ? 32 : 64; }
+// Lanes per row: enough for its labels four a lane, and for its entries one a lane.
+int small_lanes(int64_t v, int k) {
+  int g = v <= 32 ? 8 : v <= 64 ? 16 : v <= 128 ? 32 : 64;
+  while (g < 64 && g < k) g *= 2;
+  return g;
+}
 
 template <int DT, bool kBucket>
 int launch_small(const DistillArgs &a, hipStream_t s) {
-  const int g = small_lanes(a.v);
+  const int g = small_lanes(a.v, a.k);
   const dim3 grid(static_cast<unsigned>(small_blocks(a.n, g))), block(256);
-#define SBOD_SMALL(G, E) hipLaunchKernelGGL((k_distill_small<DT, G, E, kBucket>), grid, block, 0, s, a)
-  if (a.v <= 32) SBOD_SMALL(8, 4);
-  else if (a.v <= 64) SBOD_SMALL(16, 4);
-  else if (a.v <= 128) SBOD_SMALL(32, 4);
-  else if (a.v <= 256) SBOD_SMALL(64, 4);
-  else if (a.v <= 512) SBOD_SMALL(64, 8);
-  else if (a.v <= 1024) SBOD_SMALL(64, 16);
-  else if (a.v <= 1536) SBOD_SMALL(64, 24);
-  else SBOD_SMALL(64, 32);
+#define SBOD_SMALL(G, E, MORE) hipLaunchKernelGGL((k_distill_small<DT, G, E, kBucket, MORE>), grid, block, 0, s, a)
+#define SBOD_SMALL64(E) \
+  do { if (a.k > 64) SBOD_SMALL(64, E, true); else SBOD_SMALL(64, E, false); } while (0)
+  if (g == 8) SBOD_SMALL(8, 4, false);
+  else if (g == 16) SBOD_SMALL(16, 4, false);
+  else if (g == 32) SBOD_SMALL(32, 4, false);
+  else if (a.v <= 256) SBOD_SMALL64(4);
+  else if (a.v <= 512) SBOD_SMALL64(8);
+  else if (a.v <= 1024) SBOD_SMALL64(16);
+  else if (a.v <= 1536) SBOD_SMALL64(24);
+  else SBOD_SMALL64(32);
+#undef SBOD_SMALL64
 #undef SBOD_SMALL
   SBOD_LAUNCHED("k_distill_small");
   return SBOD_OK;
@@ -609,8 +632,8 @@ int launch_any(const DistillArgs &a, int dt, hipStream_t s) {
 
 // The forward's workspace: partial weight sums | loss parts | chunk statistics.
 size_t parts_offset() { return kWeightParts * sizeof(double); }
-int64_t parts_count(int64_t n, int64_t v) { return path_of(v) == kSmall ? small_blocks(n, small_lanes(v)) : n; }
-size_t chunks_offset(int64_t n, int64_t v) { return align_up(parts_offset() + parts_count(n, v) * sizeof(double)); }
+int64_t parts_count(int64_t n, int64_t v, int k) { return path_of(v) == kSmall ? small_blocks(n, small_lanes(v, k)) : n; }
+size_t chunks_offset(int64_t n, int64_t v, int k) { return align_up(parts_offset() + parts_count(n, v, k) * sizeof(double)); }
 
 int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, int64_t ldx, const void *ids,
                  const void *top, int top_dt, int k, float temperature, int reduction) {
@@ -628,6 +651,7 @@ int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, 
 void set_temperature(DistillArgs &a, float t) {
   a.t = t;
   a.inv_td = 1.0 / t;
+  a.tt = static_cast<double>(t) * t;
   a.inv_t = static_cast<float>(a.inv_td);
   a.s = static_cast<float>(a.inv_td * 1.44269504088896340736);
 }
@@ -640,10 +664,10 @@ using namespace sbod::label;
 
 extern "C" int sbod_distill_stat_floats(void) { return kStats; }
 
-extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int dtype) {
-  if (n < 0 || v <= 0 || !known_dt(dtype)) return 0;
+extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int dtype) {
+  if (n < 0 || v <= 0 || k <= 0 || !known_dt(dtype)) return 0;
   const size_t chunks = path_of(v) == kChunks ? static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2) : 0;
-  return chunks_offset(n, v) + chunks;
+  return chunks_offset(n, v, k) + chunks;
 }
 
 extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -657,8 +681,8 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || (loss && norm), "sbod_distill_fwd: a reduction needs loss and norm");
   SBOD_REQUIRE(!grad || (grad_ld >= v && reduction != SBOD_REDUCE_NONE), "sbod_distill_fwd: gradient with row stride %lld, reduction %d",
                static_cast<long long>(grad_ld), reduction);
-  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, dtype) || !workspace) {
-    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, dtype));
+  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, k, dtype) || !workspace) {
+    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, k, dtype));
     return SBOD_E_WORKSPACE;
   }
   hipStream_t s = as_stream(stream);
@@ -666,16 +690,16 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   a.x = logits, a.n = n, a.v = v, a.ldx = ld, a.ids = ids, a.ids64 = ids64, a.top = top, a.top_dt = top_dtype;
   a.k = k, a.lse = lse, a.w = weights, a.stats = stats, a.reduction = reduction;
   a.rows = reduction == SBOD_REDUCE_NONE ? rows : nullptr;
-  a.part = ws_at<float2>(workspace, chunks_offset(n, v)), a.nchunk = distill_chunks(v, dtype);
+  a.part = ws_at<float2>(workspace, chunks_offset(n, v, k)), a.nchunk = distill_chunks(v, dtype);
   a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
-  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v);
+  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v, k);
   if (reduction == SBOD_REDUCE_MEAN && weights) {
     // (64 partial sums: each workgroup of the loss joins them)
     a.wparts = static_cast<const double *>(workspace);
-    a.nw = static_cast<int>(n < kWeightParts * 256 ? (n + 255) / 256 : kWeightParts);
+    a.nw = static_cast<int>(n < kWeightParts * 1024 ? (n + 1023) / 1024 : kWeightParts);
     if (n > 0) {
-      hipLaunchKernelGGL(k_distill_weights, dim3(a.nw), dim3(256), 0, s, weights, n, static_cast<double *>(workspace));
+      hipLaunchKernelGGL(k_distill_weights, dim3(a.nw), dim3(1024), 0, s, weights, n, static_cast<double *>(workspace));
       SBOD_LAUNCHED("k_distill_weights");
     }
   }

@@ -2,6 +2,8 @@
 // types, and rows that start anywhere read and written in aligned 16-byte granules.
 #pragma once
 
+#include <type_traits>
+
 #include "sbod_common.h"
 
 namespace sbod {
@@ -41,8 +43,47 @@ __device__ __forceinline__ float ld_any(const void *p, int64_t i, int dt) {
 
 // A label id as the caller holds it (int32 or int64); -1 for anything outside [0, v).
 __device__ __forceinline__ int ld_id(const void *ids, int64_t i, bool wide, int64_t v) {
-  const int64_t id = wide ? static_cast<const int64_t *>(ids)[i] : static_cast<const int32_t *>(ids)[i];
-  return id >= 0 && id < v ? static_cast<int>(id) : -1;
+  if (wide) {
+    const uint64_t id = static_cast<const uint64_t *>(ids)[i];   // (a negative id is above every label)
+    return id < static_cast<uint64_t>(v) ? static_cast<int>(id) : -1;
+  }
+  const uint32_t id = static_cast<const uint32_t *>(ids)[i];
+  return id < static_cast<uint64_t>(v) ? static_cast<int>(id) : -1;
+}
+
+// The same two in halves: loads without a branch between them or a use behind them, so that they stay in
+// flight until the value is asked for.
+struct RawId {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ RawId ld_raw_id(const void *ids, int64_t i, bool wide) {
+  const uint32_t *p = static_cast<const uint32_t *>(ids) + (wide ? 2 * i : i);
+  return RawId{p[0], p[wide ? 1 : 0]};
+}
+__device__ __forceinline__ int id_of(RawId r, bool wide, int64_t v) {
+  const uint64_t id = (wide ? static_cast<uint64_t>(r.hi) << 32 : 0) | r.lo;
+  return id < static_cast<uint64_t>(v) ? static_cast<int>(id) : -1;
+}
+struct RawAny {
+  uint16_t lo, hi;
+};
+__device__ __forceinline__ RawAny ld_raw_any(const void *q, int64_t i, int dt) {
+  const uint16_t *p = static_cast<const uint16_t *>(q) + (dt == SBOD_DT_F32 ? 2 * i : i);
+  return RawAny{p[0], p[dt == SBOD_DT_F32 ? 1 : 0]};
+}
+__device__ __forceinline__ float any_of(RawAny r, int dt) {
+  if (dt == SBOD_DT_F32) return __uint_as_float(static_cast<uint32_t>(r.hi) << 16 | r.lo);
+  if (dt == SBOD_DT_BF16) return __uint_as_float(static_cast<uint32_t>(r.lo) << 16);
+  return static_cast<float>(__builtin_bit_cast(_Float16, r.lo));
+}
+// An element's bits, and its value.
+template <int DT>
+using bits_t = std::conditional_t<DT == SBOD_DT_F32, uint32_t, uint16_t>;
+template <int DT>
+__device__ __forceinline__ float bits_value(uint32_t b) {
+  if (DT == SBOD_DT_F32) return __uint_as_float(b);
+  if (DT == SBOD_DT_BF16) return __uint_as_float(b << 16);
+  return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(b)));
 }
 
 // Elements between the 16-byte boundary at or below p and p itself: granule g of a row at p holds
