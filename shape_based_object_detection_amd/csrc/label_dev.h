@@ -93,6 +93,17 @@ __device__ __forceinline__ int row_phase(const T *p) {
   return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
 }
 
+// A granule's 16 bytes, and their P values.
+typedef uint32_t raw16_t __attribute__((ext_vector_type(4)));
+template <int DT>
+__device__ __forceinline__ void raw_values(raw16_t r, float (&f)[Elt<DT>::P]) {
+#pragma unroll
+  for (int j = 0; j < Elt<DT>::P; ++j) {
+    if (DT == SBOD_DT_F32) f[j] = __uint_as_float(r[j]);
+    else f[j] = bits_value<DT>(r[j >> 1] >> (16 * (j & 1)) & 0xffff);
+  }
+}
+
 // The elements [e, e + P) of a row of v at p; those outside the row read as `fill`.  p + e is
 // 16-byte aligned (row_phase), so a granule inside the row is one load, and nothing outside the row
 // is touched.

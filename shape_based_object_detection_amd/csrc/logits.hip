@@ -11,9 +11,11 @@
 namespace sbod {
 namespace label {
 
-constexpr int kLogThreads = 256;
-constexpr int kLogTile = 4096;            // labels per item: their counts and listed biases in LDS, 32 KB
-constexpr uint32_t kSeen = 0x80000000u;   // in the history's given part; the low bits count the answers
+constexpr int kLogTile = 8192;      // labels per item
+constexpr int kLogThreads = 512;
+// A label's word in the table: seen in the history's given part, with a listed bias, with two; and below
+// them how often it was answered.
+constexpr uint32_t kSeen = 1u << 31, kBiased = 1u << 30, kTwice = 1u << 29, kCount = kTwice - 1;
 
 struct LogitsArgs {
   const void *x;
@@ -27,85 +29,165 @@ struct LogitsArgs {
   const void *mask;             // bits: int32 words; bytes: truth values; row stride ldm in elements
   int64_t n, v, ldx, ldo, ldh, ldb, ldi, ldv, ldm;
   int64_t len;
-  int m, hist64, ids64, bias_dt, mask_kind, ntile;
+  int m, hist64, ids64, bias_dt, mask_kind, ntile, tile;   // tile: labels of an item, a multiple of 8
   float rep_s, pres_s, freq_s;
 };
 
-template <int DT>
+// One label's value: x with the history's word of it, its listed biases, its bias and its mask.
+__device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int64_t v, float x, uint32_t word, int entry,
+                                        float rep, float pres, float freq) {
+  if (word & (kSeen | kCount)) {
+    x = x > 0.f ? x / rep : x * rep;
+    const uint32_t answered = word & kCount;
+    x = x - freq * static_cast<float>(answered);
+    if (answered) x -= pres;
+  }
+  if (a.bias) x += ld_any(a.bias, r * a.ldb + v, a.bias_dt);
+  if (word & kTwice) {   // in the order listed
+    float s = 0.f;
+    for (int i = 0; i < a.m; ++i)
+      if (ld_id(a.bias_ids, r * a.ldi + i, a.ids64, a.v) == v) s += a.bias_val[r * a.ldv + i];
+    x += s;
+  } else if (word & kBiased) {
+    x += a.bias_val[r * a.ldv + entry];
+  }
+  return x;
+}
+
+template <int kMask>
+__device__ __forceinline__ bool forbidden(const LogitsArgs &a, int64_t r, int64_t v) {
+  if (kMask == SBOD_MASK_BITS) return !(static_cast<const uint32_t *>(a.mask)[r * a.ldm + (v >> 5)] >> (v & 31) & 1);
+  if (kMask == SBOD_MASK_BYTES) return static_cast<const uint8_t *>(a.mask)[r * a.ldm + v] == 0;
+  return false;
+}
+
+// P mask bits of the labels [e, e + P), all inside the row.
+template <int kMask, int P>
+__device__ __forceinline__ uint32_t mask_of(const LogitsArgs &a, int64_t r, int64_t e) {
+  if (kMask == SBOD_MASK_BITS) {
+    const uint32_t *w = static_cast<const uint32_t *>(a.mask) + r * a.ldm;
+    const uint64_t two = static_cast<uint64_t>(w[(e + P - 1) >> 5]) << 32 | w[e >> 5];
+    return static_cast<uint32_t>(two >> (e & 31));   // (one word twice where they are the same: its upper copy is not reached)
+  }
+  if (kMask == SBOD_MASK_BYTES) {
+    const uint8_t *b = static_cast<const uint8_t *>(a.mask) + r * a.ldm + e;
+    uint32_t bits = 0;
+    uint32_t word[P / 4];
+    __builtin_memcpy(word, b, P);   // (a load at any address)
+#pragma unroll
+    for (int j = 0; j < P; ++j) bits |= (word[j / 4] >> (8 * (j % 4)) & 0xff) != 0 ? 1u << j : 0;
+    return bits;
+  }
+  return ~0u;
+}
+
+// An item is a row's tile of up to kLogTile labels.  Its logits are on their way while the history is read:
+// the answers' counts and the listed biases go to a table of the tile in LDS (integer atomics), and the
+// tile then passes through registers once, a granule with a touched label label by label.
+template <int DT, int kMask>
 __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
   using T = typename Elt<DT>::T;
-  constexpr int P = Elt<DT>::P;
-  __shared__ uint32_t cnt[kLogTile];
-  __shared__ float add[kLogTile];
+  constexpr int P = Elt<DT>::P, kPer = kLogTile / P / kLogThreads;
+  extern __shared__ uint32_t table[];   // [a.tile] words, then [a.tile] 16-bit entries
+  uint16_t *entry = reinterpret_cast<uint16_t *>(table + a.tile);
+  const int nt = blockDim.x;
   const int64_t items = a.n * a.ntile;
+  const bool build = a.len > 0 || a.m > 0;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t r = it / a.ntile;
+    const int64_t r = a.ntile == 1 ? it : it / a.ntile;
     const T *row = static_cast<const T *>(a.x) + r * a.ldx;
     T *orow = static_cast<T *>(a.out) + r * a.ldo;
     const int phase = row_phase(row);
     const bool aligned = row_phase(orow) == phase;
     const int64_t e0 = (it - r * a.ntile) * kLogTile - phase;
-    int64_t len = a.len;
-    if (a.hist_len) len = min(len, static_cast<int64_t>(max(a.hist_len[r], 0)));
-    const int64_t given = a.prompt_len ? a.prompt_len[r] : 0;
-    for (int i = threadIdx.x; i < kLogTile; i += kLogThreads) {
-      cnt[i] = 0;
-      add[i] = 0.f;
-    }
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < len; i += kLogThreads) {
-      const int id = ld_id(a.hist, r * a.ldh + i, a.hist64, a.v);
-      const int64_t at = id - e0;
-      if (id < 0 || at < 0 || at >= kLogTile) continue;
-      if (i < given)
-        atomicOr(&cnt[at], kSeen);
-      else
-        atomicAdd(&cnt[at], 1u);
-    }
-    for (int i = threadIdx.x; i < a.m; i += kLogThreads) {
-      const int id = ld_id(a.bias_ids, r * a.ldi + i, a.ids64, a.v);
-      const int64_t at = id - e0;
-      if (id < 0 || at < 0 || at >= kLogTile) continue;
-      // the first of a repeated label's entries adds them all, in order
-      bool first = true;
-      for (int j = 0; j < i && first; ++j) first = ld_id(a.bias_ids, r * a.ldi + j, a.ids64, a.v) != id;
-      if (!first) continue;
-      float s = 0.f;
-      for (int j = i; j < a.m; ++j)
-        if (ld_id(a.bias_ids, r * a.ldi + j, a.ids64, a.v) == id) s += a.bias_val[r * a.ldv + j];
-      add[at] = s;
-    }
-    __syncthreads();
-    const float rep = a.rep ? a.rep[r] : a.rep_s, pres = a.pres ? a.pres[r] : a.pres_s,
-                freq = a.freq ? a.freq[r] : a.freq_s;
-    for (int g = threadIdx.x; g < kLogTile / P; g += kLogThreads) {
-      const int64_t e = e0 + static_cast<int64_t>(g) * P;
-      if (e >= a.v) break;
-      float f[P];
-      ld_granule<DT>(row, e, a.v, 0.f, f);
+    raw16_t raw[kPer];
+    uint32_t ok[kPer];
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        if (e + j < 0 || e + j >= a.v) continue;
-        const uint32_t c = cnt[g * P + j];
-        if (c) {
-          f[j] = f[j] > 0.f ? f[j] / rep : f[j] * rep;
-          const uint32_t answered = c & ~kSeen;
-          f[j] = f[j] - freq * static_cast<float>(answered);
-          if (answered) f[j] -= pres;
-        }
-        if (a.bias) f[j] += ld_any(a.bias, r * a.ldb + e + j, a.bias_dt);
-        f[j] += add[g * P + j];
-        bool ok = true;
-        if (a.mask_kind == SBOD_MASK_BITS)
-          ok = static_cast<const uint32_t *>(a.mask)[r * a.ldm + ((e + j) >> 5)] >> ((e + j) & 31) & 1;
-        else if (a.mask_kind == SBOD_MASK_BYTES)
-          ok = static_cast<const uint8_t *>(a.mask)[r * a.ldm + e + j] != 0;
-        if (!ok) f[j] = -__builtin_inff();
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t e = e0 + static_cast<int64_t>(i * nt + threadIdx.x) * P;
+      if (i * nt + static_cast<int>(threadIdx.x) < a.tile / P && e >= 0 && e + P <= a.v) {
+        raw[i] = *reinterpret_cast<const raw16_t *>(row + e);
+        ok[i] = mask_of<kMask, P>(a, r, e);
       }
-      st_granule<DT>(orow, e, a.v, aligned, f);
     }
-    __syncthreads();
+    float rep = 1.f, pres = 0.f, freq = 0.f;
+    if (build) {
+      for (int i = threadIdx.x; i < a.tile / 4; i += nt) reinterpret_cast<raw16_t *>(table)[i] = raw16_t{0, 0, 0, 0};
+      rep = a.rep ? a.rep[r] : a.rep_s, pres = a.pres ? a.pres[r] : a.pres_s, freq = a.freq ? a.freq[r] : a.freq_s;
+      int64_t len = a.len;
+      if (a.hist_len) len = min(len, static_cast<int64_t>(max(a.hist_len[r], 0)));
+      const int64_t given = a.prompt_len ? a.prompt_len[r] : 0;
+      __syncthreads();
+      constexpr int kU = 4;   // loads in flight
+      for (int64_t i = threadIdx.x; i < len; i += kU * nt) {
+        RawId id[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) id[u] = ld_raw_id(a.hist, r * a.ldh + min(i + u * nt, len - 1), a.hist64);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int label = id_of(id[u], a.hist64, a.v);
+          const int64_t at = label - e0;
+          if (i + u * nt >= len || label < 0 || at < 0 || at >= a.tile) continue;
+          if (i + u * nt < given) atomicOr(&table[at], kSeen);
+          else atomicAdd(&table[at], 1u);
+        }
+      }
+      for (int i = threadIdx.x; i < a.m; i += nt) {
+        const int label = ld_id(a.bias_ids, r * a.ldi + i, a.ids64, a.v);
+        const int64_t at = label - e0;
+        if (label < 0 || at < 0 || at >= a.tile) continue;
+        if (atomicOr(&table[at], kBiased) & kBiased) atomicOr(&table[at], kTwice);
+        entry[at] = static_cast<uint16_t>(i);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g = i * nt + threadIdx.x;
+      const int64_t e = e0 + static_cast<int64_t>(g) * P;
+      if (g >= a.tile / P || e >= a.v) break;
+      float f[P];
+      if (e >= 0 && e + P <= a.v) {
+        raw_values<DT>(raw[i], f);
+        uint32_t word[P], any = 0;
+        if (build) {
+#pragma unroll
+          for (int j = 0; j < P; j += 4) {
+            const raw16_t w = reinterpret_cast<const raw16_t *>(table)[(g * P + j) / 4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) any |= word[j + c] = w[c];
+          }
+        }
+        if (any) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) f[j] = adjust(a, r, e + j, f[j], word[j], word[j] & kBiased ? entry[g * P + j] : 0, rep, pres, freq);
+        } else if (a.bias) {
+#pragma unroll
+          for (int j = 0; j < P; ++j) f[j] += ld_any(a.bias, r * a.ldb + e + j, a.bias_dt);
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (kMask != SBOD_MASK_NONE && !(ok[i] >> j & 1)) f[j] = -__builtin_inff();
+        st_granule<DT>(orow, e, a.v, aligned, f);
+      } else {   // a granule that the row's start or end cuts
+        for (int j = 0; j < P; ++j) {
+          if (e + j < 0 || e + j >= a.v) continue;
+          const uint32_t word = build ? table[g * P + j] : 0;
+          float x = adjust(a, r, e + j, static_cast<float>(row[e + j]), word, word & kBiased ? entry[g * P + j] : 0, rep, pres, freq);
+          if (forbidden<kMask>(a, r, e + j)) x = -__builtin_inff();
+          orow[e + j] = static_cast<T>(x);
+        }
+      }
+    }
+    if (build) __syncthreads();
   }
+}
+
+template <int DT>
+void launch_logits(const LogitsArgs &a, dim3 grid, dim3 block, size_t lds, hipStream_t s) {
+  if (a.mask_kind == SBOD_MASK_BITS) hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_BITS>), grid, block, lds, s, a);
+  else if (a.mask_kind == SBOD_MASK_BYTES) hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_BYTES>), grid, block, lds, s, a);
+  else hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_NONE>), grid, block, lds, s, a);
 }
 
 }  // namespace label
@@ -126,7 +208,7 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
   SBOD_REQUIRE(n >= 0 && v >= 1 && v < (1ll << 31) - 65536 && ld >= v && out_ld >= v && n < (1ll << 40) / v,
                "sbod_logits_process: logits [%lld, %lld], row strides %lld / %lld", static_cast<long long>(n),
                static_cast<long long>(v), static_cast<long long>(ld), static_cast<long long>(out_ld));
-  SBOD_REQUIRE(history_cols >= 0 && history_cols < (1ll << 31) && bias_cols >= 0 && history_ld >= 0 && bias_ld >= 0 &&
+  SBOD_REQUIRE(history_cols >= 0 && history_cols <= kCount && bias_cols >= 0 && bias_cols < 65536 && history_ld >= 0 && bias_ld >= 0 &&
                    bias_ids_ld >= 0 && bias_values_ld >= 0 && mask_ld >= 0,
                "sbod_logits_process: negative size or stride");
   SBOD_REQUIRE(mask_kind == SBOD_MASK_NONE || ((mask_kind == SBOD_MASK_BITS || mask_kind == SBOD_MASK_BYTES) && mask),
@@ -144,16 +226,18 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
   a.bias = bias, a.bias_dt = bias_dtype, a.ldb = bias_ld, a.bias_ids = bias_ids, a.ids64 = bias_ids64;
   a.bias_val = bias_values, a.m = bias_cols, a.ldi = bias_ids_ld, a.ldv = bias_values_ld;
   a.mask = mask, a.mask_kind = mask_kind, a.ldm = mask_ld;
-  a.ntile = static_cast<int>((v + 16 / elt_bytes(dtype) - 1 + kLogTile - 1) / kLogTile);
+  const int64_t most = v + 16 / static_cast<int64_t>(elt_bytes(dtype)) - 1;   // (from a 16-byte boundary on)
+  a.ntile = static_cast<int>((most + kLogTile - 1) / kLogTile);
+  a.tile = static_cast<int>(most < kLogTile ? (most + 7) / 8 * 8 : kLogTile);
+  // threads for the tile's granules, two (four of float32) each
+  const dim3 block(a.tile <= 1024 + 8 ? 128 : a.tile <= kLogTile / 2 ? 256 : kLogThreads);
   const int64_t items = n * a.ntile;
-  const dim3 grid(static_cast<unsigned>(items < 65536 ? items : 65536)), block(kLogThreads);
+  const dim3 grid(static_cast<unsigned>(items < 65536 ? items : 65536));
+  const size_t lds = a.len > 0 || a.m > 0 ? a.tile * (sizeof(uint32_t) + sizeof(uint16_t)) : 0;
   hipStream_t s = as_stream(stream);
-  if (dtype == SBOD_DT_F32)
-    hipLaunchKernelGGL(k_logits<SBOD_DT_F32>, grid, block, 0, s, a);
-  else if (dtype == SBOD_DT_BF16)
-    hipLaunchKernelGGL(k_logits<SBOD_DT_BF16>, grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL(k_logits<SBOD_DT_F16>, grid, block, 0, s, a);
+  if (dtype == SBOD_DT_F32) launch_logits<SBOD_DT_F32>(a, grid, block, lds, s);
+  else if (dtype == SBOD_DT_BF16) launch_logits<SBOD_DT_BF16>(a, grid, block, lds, s);
+  else launch_logits<SBOD_DT_F16>(a, grid, block, lds, s);
   SBOD_LAUNCHED("k_logits");
   return SBOD_OK;
 }
