@@ -33,16 +33,16 @@ struct LogitsArgs {
   float rep_s, pres_s, freq_s;
 };
 
-// One label's value: x with the history's word of it, its listed biases, its bias and its mask.
+// One label's value: x with the history's word of it, its bias and its listed biases.
 __device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int64_t v, float x, uint32_t word, int entry,
-                                        float rep, float pres, float freq) {
+                                        float bias, float rep, float pres, float freq) {
   if (word & (kSeen | kCount)) {
     x = x > 0.f ? x / rep : x * rep;
     const uint32_t answered = word & kCount;
     x = x - freq * static_cast<float>(answered);
     if (answered) x -= pres;
   }
-  if (a.bias) x += ld_any(a.bias, r * a.ldb + v, a.bias_dt);
+  x += bias;
   if (word & kTwice) {   // in the order listed
     float s = 0.f;
     for (int i = 0; i < a.m; ++i)
@@ -52,6 +52,26 @@ __device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int64_t 
     x += a.bias_val[r * a.ldv + entry];
   }
   return x;
+}
+
+// P biases of type BT of the labels [e, e + P), all inside the row: in flight until bias_values.
+template <int BT, int P>
+struct RawBias {
+  static constexpr int kWords = P * (BT == SBOD_DT_F32 ? 4 : 2) / 4;
+  uint32_t w[kWords];
+};
+template <int BT, int P>
+__device__ __forceinline__ void ld_raw_bias(RawBias<BT, P> &b, const LogitsArgs &a, int64_t r, int64_t e) {
+  typedef uint32_t words_t __attribute__((ext_vector_type(RawBias<BT, P>::kWords), aligned(sizeof(typename Elt<BT>::T))));
+  const words_t v = *reinterpret_cast<const words_t *>(static_cast<const typename Elt<BT>::T *>(a.bias) + r * a.ldb + e);
+#pragma unroll
+  for (int i = 0; i < RawBias<BT, P>::kWords; ++i) b.w[i] = v[i];   // (a load at any address)
+}
+template <int BT, int P>
+__device__ __forceinline__ void bias_values(const RawBias<BT, P> &b, float (&f)[P]) {
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+    f[j] = BT == SBOD_DT_F32 ? __uint_as_float(b.w[j]) : bits_value<BT>(b.w[j / 2] >> (16 * (j & 1)) & 0xffff);
 }
 
 template <int kMask>
@@ -84,9 +104,10 @@ __device__ __forceinline__ uint32_t mask_of(const LogitsArgs &a, int64_t r, int6
 // An item is a row's tile of up to kLogTile labels.  Its logits are on their way while the history is read:
 // the answers' counts and the listed biases go to a table of the tile in LDS (integer atomics), and the
 // tile then passes through registers once, a granule with a touched label label by label.
-template <int DT, int kMask>
+template <int DT, int kMask, int kBias>
 __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
   using T = typename Elt<DT>::T;
+  constexpr int BT = kBias < 0 ? SBOD_DT_F32 : kBias;
   constexpr int P = Elt<DT>::P, kPer = kLogTile / P / kLogThreads;
   extern __shared__ uint32_t table[];   // [a.tile] words, then [a.tile] 16-bit entries
   uint16_t *entry = reinterpret_cast<uint16_t *>(table + a.tile);
@@ -100,14 +121,17 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
     const int phase = row_phase(row);
     const bool aligned = row_phase(orow) == phase;
     const int64_t e0 = (it - r * a.ntile) * kLogTile - phase;
+    if (e0 >= a.v) continue;   // (a last tile that only other rows' starts reach into)
     raw16_t raw[kPer];
     uint32_t ok[kPer];
+    RawBias<BT, P> rb[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int64_t e = e0 + static_cast<int64_t>(i * nt + threadIdx.x) * P;
       if (i * nt + static_cast<int>(threadIdx.x) < a.tile / P && e >= 0 && e + P <= a.v) {
         raw[i] = *reinterpret_cast<const raw16_t *>(row + e);
         ok[i] = mask_of<kMask, P>(a, r, e);
+        if (kBias >= 0) ld_raw_bias<BT, P>(rb[i], a, r, e);
       }
     }
     float rep = 1.f, pres = 0.f, freq = 0.f;
@@ -158,12 +182,15 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
             for (int c = 0; c < 4; ++c) any |= word[j + c] = w[c];
           }
         }
+        float bias[P] = {};
+        if (kBias >= 0) bias_values<BT, P>(rb[i], bias);
         if (any) {
 #pragma unroll
-          for (int j = 0; j < P; ++j) f[j] = adjust(a, r, e + j, f[j], word[j], word[j] & kBiased ? entry[g * P + j] : 0, rep, pres, freq);
-        } else if (a.bias) {
+          for (int j = 0; j < P; ++j)
+            f[j] = adjust(a, r, e + j, f[j], word[j], word[j] & kBiased ? entry[g * P + j] : 0, bias[j], rep, pres, freq);
+        } else if (kBias >= 0) {
 #pragma unroll
-          for (int j = 0; j < P; ++j) f[j] += ld_any(a.bias, r * a.ldb + e + j, a.bias_dt);
+          for (int j = 0; j < P; ++j) f[j] += bias[j];
         }
 #pragma unroll
         for (int j = 0; j < P; ++j)
@@ -173,7 +200,9 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
         for (int j = 0; j < P; ++j) {
           if (e + j < 0 || e + j >= a.v) continue;
           const uint32_t word = build ? table[g * P + j] : 0;
-          float x = adjust(a, r, e + j, static_cast<float>(row[e + j]), word, word & kBiased ? entry[g * P + j] : 0, rep, pres, freq);
+          const float bias = kBias >= 0 ? ld_any(a.bias, r * a.ldb + e + j, BT) : 0.f;
+          float x = adjust(a, r, e + j, static_cast<float>(row[e + j]), word, word & kBiased ? entry[g * P + j] : 0, bias,
+                           rep, pres, freq);
           if (forbidden<kMask>(a, r, e + j)) x = -__builtin_inff();
           orow[e + j] = static_cast<T>(x);
         }
@@ -183,11 +212,17 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
   }
 }
 
+template <int DT, int kBias>
+void launch_logits(const LogitsArgs &a, dim3 grid, dim3 block, size_t lds, hipStream_t s) {
+  if (a.mask_kind == SBOD_MASK_BITS) hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_BITS, kBias>), grid, block, lds, s, a);
+  else if (a.mask_kind == SBOD_MASK_BYTES) hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_BYTES, kBias>), grid, block, lds, s, a);
+  else hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_NONE, kBias>), grid, block, lds, s, a);
+}
 template <int DT>
 void launch_logits(const LogitsArgs &a, dim3 grid, dim3 block, size_t lds, hipStream_t s) {
-  if (a.mask_kind == SBOD_MASK_BITS) hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_BITS>), grid, block, lds, s, a);
-  else if (a.mask_kind == SBOD_MASK_BYTES) hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_BYTES>), grid, block, lds, s, a);
-  else hipLaunchKernelGGL((k_logits<DT, SBOD_MASK_NONE>), grid, block, lds, s, a);
+  if (!a.bias) launch_logits<DT, -1>(a, grid, block, lds, s);
+  else if (a.bias_dt == SBOD_DT_F32) launch_logits<DT, SBOD_DT_F32>(a, grid, block, lds, s);
+  else launch_logits<DT, DT>(a, grid, block, lds, s);
 }
 
 }  // namespace label
@@ -204,7 +239,7 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
                                    const void *bias_ids, int bias_ids64, const float *bias_values, int bias_cols,
                                    int64_t bias_ids_ld, int64_t bias_values_ld, const void *mask, int mask_kind,
                                    int64_t mask_ld, void *out, int64_t out_ld, void *stream) {
-  SBOD_REQUIRE(known_dt(dtype) && (!bias || known_dt(bias_dtype)), "sbod_logits_process: dtype %d / %d", dtype, bias_dtype);
+  SBOD_REQUIRE(known_dt(dtype) && (!bias || bias_dtype == SBOD_DT_F32 || bias_dtype == dtype), "sbod_logits_process: dtype %d / %d", dtype, bias_dtype);
   SBOD_REQUIRE(n >= 0 && v >= 1 && v < (1ll << 31) - 65536 && ld >= v && out_ld >= v && n < (1ll << 40) / v,
                "sbod_logits_process: logits [%lld, %lld], row strides %lld / %lld", static_cast<long long>(n),
                static_cast<long long>(v), static_cast<long long>(ld), static_cast<long long>(out_ld));
@@ -226,7 +261,9 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
   a.bias = bias, a.bias_dt = bias_dtype, a.ldb = bias_ld, a.bias_ids = bias_ids, a.ids64 = bias_ids64;
   a.bias_val = bias_values, a.m = bias_cols, a.ldi = bias_ids_ld, a.ldv = bias_values_ld;
   a.mask = mask, a.mask_kind = mask_kind, a.ldm = mask_ld;
-  const int64_t most = v + 16 / static_cast<int64_t>(elt_bytes(dtype)) - 1;   // (from a 16-byte boundary on)
+  // a row's labels from the 16-byte boundary below it on
+  const bool even = (reinterpret_cast<uintptr_t>(logits) | ld * elt_bytes(dtype)) % 16 == 0;
+  const int64_t most = even ? v : v + 16 / static_cast<int64_t>(elt_bytes(dtype)) - 1;
   a.ntile = static_cast<int>((most + kLogTile - 1) / kLogTile);
   a.tile = static_cast<int>(most < kLogTile ? (most + 7) / 8 * 8 : kLogTile);
   // threads for the tile's granules, two (four of float32) each
