@@ -13,6 +13,7 @@ namespace label {
 
 constexpr int kLogTile = 8192;      // labels per item
 constexpr int kLogThreads = 512;
+constexpr int kMaxBiases = 4096;    // listed per row: 32 of the fewest threads' (sbod_logits_process)
 // A label's word in the table: seen in the history's given part, with a listed bias, with two; and below
 // them how often it was answered.
 constexpr uint32_t kSeen = 1u << 31, kBiased = 1u << 30, kTwice = 1u << 29, kCount = kTwice - 1;
@@ -29,26 +30,28 @@ struct LogitsArgs {
   const void *mask;             // bits: int32 words; bytes: truth values; row stride ldm in elements
   int64_t n, v, ldx, ldo, ldh, ldb, ldi, ldv, ldm;
   int64_t len;
-  int m, hist64, ids64, bias_dt, mask_kind, ntile, tile;   // tile: labels of an item, a multiple of 8
+  int m, hist64, ids64, bias_dt, mask_kind, ntile, tile;   // tile: labels of an item, a multiple of 32
   float rep_s, pres_s, freq_s;
 };
 
-// One label's value: x with the history's word of it, its bias and its listed biases.
-__device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int64_t v, float x, uint32_t word, int entry,
-                                        float bias, float rep, float pres, float freq) {
+// A touched label's value but for its mask: x with the history's word of it, its bias, and the listed bias
+// `entry` (-1: none).
+template <int kBias>
+__device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int v, float x, uint32_t word, int entry,
+                                        float rep, float pres, float freq) {
   if (word & (kSeen | kCount)) {
     x = x > 0.f ? x / rep : x * rep;
     const uint32_t answered = word & kCount;
     x = x - freq * static_cast<float>(answered);
     if (answered) x -= pres;
   }
-  x += bias;
+  if (kBias >= 0) x += ld_any(a.bias, r * a.ldb + v, kBias);
   if (word & kTwice) {   // in the order listed
     float s = 0.f;
     for (int i = 0; i < a.m; ++i)
       if (ld_id(a.bias_ids, r * a.ldi + i, a.ids64, a.v) == v) s += a.bias_val[r * a.ldv + i];
     x += s;
-  } else if (word & kBiased) {
+  } else if (entry >= 0) {
     x += a.bias_val[r * a.ldv + entry];
   }
   return x;
@@ -102,16 +105,20 @@ __device__ __forceinline__ uint32_t mask_of(const LogitsArgs &a, int64_t r, int6
 }
 
 // An item is a row's tile of up to kLogTile labels.  Its logits are on their way while the history is read:
-// the answers' counts and the listed biases go to a table of the tile in LDS (integer atomics), and the
-// tile then passes through registers once, a granule with a touched label label by label.
+// the answers' counts go to a table of the tile in LDS (integer atomics), the first touch of a label puts it
+// on a list, and the first of its listed biases' threads owns it.  Each touched label is then computed by one
+// thread, its value taking its word's place in the table, and the tile passes through registers once, the
+// touched labels (a bit each) from the table.
 template <int DT, int kMask, int kBias>
 __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
   using T = typename Elt<DT>::T;
   constexpr int BT = kBias < 0 ? SBOD_DT_F32 : kBias;
   constexpr int P = Elt<DT>::P, kPer = kLogTile / P / kLogThreads;
-  extern __shared__ uint32_t table[];   // [a.tile] words, then [a.tile] 16-bit entries
-  uint16_t *entry = reinterpret_cast<uint16_t *>(table + a.tile);
-  const int nt = blockDim.x;
+  extern __shared__ __attribute__((aligned(16))) uint32_t table[];   // [a.tile] words, then values; [a.tile] listed labels; [a.tile] bits
+  __shared__ int listed;
+  uint16_t *list = reinterpret_cast<uint16_t *>(table + a.tile);
+  uint8_t *touched = reinterpret_cast<uint8_t *>(list + a.tile);
+  const int nt = blockDim.x, lane = threadIdx.x;
   const int64_t items = a.n * a.ntile;
   const bool build = a.len > 0 || a.m > 0;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
@@ -127,70 +134,100 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
     RawBias<BT, P> rb[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int64_t e = e0 + static_cast<int64_t>(i * nt + threadIdx.x) * P;
-      if (i * nt + static_cast<int>(threadIdx.x) < a.tile / P && e >= 0 && e + P <= a.v) {
+      const int64_t e = e0 + static_cast<int64_t>(i * nt + lane) * P;
+      if (i * nt + lane < a.tile / P && e >= 0 && e + P <= a.v) {
         raw[i] = *reinterpret_cast<const raw16_t *>(row + e);
         ok[i] = mask_of<kMask, P>(a, r, e);
         if (kBias >= 0) ld_raw_bias<BT, P>(rb[i], a, r, e);
       }
     }
-    float rep = 1.f, pres = 0.f, freq = 0.f;
     if (build) {
-      for (int i = threadIdx.x; i < a.tile / 4; i += nt) reinterpret_cast<raw16_t *>(table)[i] = raw16_t{0, 0, 0, 0};
-      rep = a.rep ? a.rep[r] : a.rep_s, pres = a.pres ? a.pres[r] : a.pres_s, freq = a.freq ? a.freq[r] : a.freq_s;
+      // what the row brings is asked for at once: the first kU entries per thread before the history's
+      // length is known
+      constexpr int kU = 2;
+      RawId id[kU], bid = {};
       int64_t len = a.len;
-      if (a.hist_len) len = min(len, static_cast<int64_t>(max(a.hist_len[r], 0)));
-      const int64_t given = a.prompt_len ? a.prompt_len[r] : 0;
-      __syncthreads();
-      constexpr int kU = 4;   // loads in flight
-      for (int64_t i = threadIdx.x; i < len; i += kU * nt) {
-        RawId id[kU];
+      if (a.len > 0) {
 #pragma unroll
-        for (int u = 0; u < kU; ++u) id[u] = ld_raw_id(a.hist, r * a.ldh + min(i + u * nt, len - 1), a.hist64);
+        for (int u = 0; u < kU; ++u) id[u] = ld_raw_id(a.hist, r * a.ldh + min(static_cast<int64_t>(u * nt + lane), a.len - 1), a.hist64);
+      }
+      if (a.m > 0) bid = ld_raw_id(a.bias_ids, r * a.ldi + min(lane, a.m - 1), a.ids64);
+      const int32_t lim = a.hist_len ? a.hist_len[r] : 0, prompt = a.prompt_len ? a.prompt_len[r] : 0;
+      const float rep = a.rep ? a.rep[r] : a.rep_s, pres = a.pres ? a.pres[r] : a.pres_s,
+                  freq = a.freq ? a.freq[r] : a.freq_s;
+      for (int i = lane; i < a.tile / 4; i += nt) reinterpret_cast<raw16_t *>(table)[i] = raw16_t{0, 0, 0, 0};
+      for (int i = lane; i < a.tile / 32; i += nt) reinterpret_cast<uint32_t *>(touched)[i] = 0;
+      if (lane == 0) listed = 0;
+      if (a.hist_len) len = min(len, static_cast<int64_t>(max(lim, 0)));
+      __syncthreads();
+      const auto mark = [&](int at) { atomicOr(reinterpret_cast<uint32_t *>(touched) + (at >> 5), 1u << (at & 31)); };
+      for (int64_t i = lane;; i += kU * nt) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
           const int label = id_of(id[u], a.hist64, a.v);
           const int64_t at = label - e0;
           if (i + u * nt >= len || label < 0 || at < 0 || at >= a.tile) continue;
-          if (i + u * nt < given) atomicOr(&table[at], kSeen);
-          else atomicAdd(&table[at], 1u);
+          const uint32_t was = i + u * nt < prompt ? atomicOr(&table[at], kSeen) : atomicAdd(&table[at], 1u);
+          if (was == 0) {
+            list[atomicAdd(&listed, 1)] = static_cast<uint16_t>(at);
+            mark(static_cast<int>(at));
+          }
+        }
+        if (i + kU * nt >= len) break;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) id[u] = ld_raw_id(a.hist, r * a.ldh + min(i + (kU + u) * nt, len - 1), a.hist64);
+      }
+      uint32_t own = 0;   // which of this thread's listed biases own their labels (at most 32: launch)
+      const auto biased = [&](int i) -> int {
+        const int label = id_of(i == lane ? bid : ld_raw_id(a.bias_ids, r * a.ldi + i, a.ids64), a.ids64, a.v);
+        const int64_t at = label - e0;
+        return label < 0 || at < 0 || at >= a.tile ? -1 : static_cast<int>(at);
+      };
+      for (int i = lane, c = 0; i < a.m; i += nt, ++c) {
+        const int at = biased(i);
+        if (at < 0) continue;
+        if (atomicOr(&table[at], kBiased) & kBiased) {
+          atomicOr(&table[at], kTwice);
+        } else {
+          own |= 1u << c;
+          mark(at);
         }
       }
-      for (int i = threadIdx.x; i < a.m; i += nt) {
-        const int label = ld_id(a.bias_ids, r * a.ldi + i, a.ids64, a.v);
-        const int64_t at = label - e0;
-        if (label < 0 || at < 0 || at >= a.tile) continue;
-        if (atomicOr(&table[at], kBiased) & kBiased) atomicOr(&table[at], kTwice);
-        entry[at] = static_cast<uint16_t>(i);
-      }
       __syncthreads();
+      const auto settle = [&](int at, int entry) {
+        const int v = static_cast<int>(e0 + at);
+        const float x = adjust<kBias>(a, r, v, static_cast<float>(row[v]), table[at], entry, rep, pres, freq);
+        table[at] = __float_as_uint(x);
+      };
+      for (int i = lane; i < listed; i += nt)
+        if (!(table[list[i]] & kBiased)) settle(list[i], -1);
+      __syncthreads();   // (an owned label's word is a value from here on)
+      for (int i = lane, c = 0; i < a.m; i += nt, ++c)
+        if (own >> c & 1) settle(biased(i), i);
+      if (a.m > 0) __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int g = i * nt + threadIdx.x;
+      const int g = i * nt + lane;
       const int64_t e = e0 + static_cast<int64_t>(g) * P;
       if (g >= a.tile / P || e >= a.v) break;
-      float f[P];
+      const uint32_t bits = !build ? 0 : P == 8 ? touched[g] : touched[g / 2] >> (4 * (g & 1)) & 15;
       if (e >= 0 && e + P <= a.v) {
+        float f[P];
         raw_values<DT>(raw[i], f);
-        uint32_t word[P], any = 0;
-        if (build) {
+        if (kBias >= 0) {
+          float bias[P];
+          bias_values<BT, P>(rb[i], bias);
+#pragma unroll
+          for (int j = 0; j < P; ++j) f[j] += bias[j];
+        }
+        if (bits) {
 #pragma unroll
           for (int j = 0; j < P; j += 4) {
             const raw16_t w = reinterpret_cast<const raw16_t *>(table)[(g * P + j) / 4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) any |= word[j + c] = w[c];
+            for (int c = 0; c < 4; ++c) f[j + c] = bits >> (j + c) & 1 ? __uint_as_float(w[c]) : f[j + c];
           }
-        }
-        float bias[P] = {};
-        if (kBias >= 0) bias_values<BT, P>(rb[i], bias);
-        if (any) {
-#pragma unroll
-          for (int j = 0; j < P; ++j)
-            f[j] = adjust(a, r, e + j, f[j], word[j], word[j] & kBiased ? entry[g * P + j] : 0, bias[j], rep, pres, freq);
-        } else if (kBias >= 0) {
-#pragma unroll
-          for (int j = 0; j < P; ++j) f[j] += bias[j];
         }
 #pragma unroll
         for (int j = 0; j < P; ++j)
@@ -199,10 +236,9 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
       } else {   // a granule that the row's start or end cuts
         for (int j = 0; j < P; ++j) {
           if (e + j < 0 || e + j >= a.v) continue;
-          const uint32_t word = build ? table[g * P + j] : 0;
-          const float bias = kBias >= 0 ? ld_any(a.bias, r * a.ldb + e + j, BT) : 0.f;
-          float x = adjust(a, r, e + j, static_cast<float>(row[e + j]), word, word & kBiased ? entry[g * P + j] : 0, bias,
-                           rep, pres, freq);
+          float x = static_cast<float>(row[e + j]);
+          if (bits >> j & 1) x = __uint_as_float(table[g * P + j]);
+          else if (kBias >= 0) x += ld_any(a.bias, r * a.ldb + e + j, BT);
           if (forbidden<kMask>(a, r, e + j)) x = -__builtin_inff();
           orow[e + j] = static_cast<T>(x);
         }
@@ -243,7 +279,7 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
   SBOD_REQUIRE(n >= 0 && v >= 1 && v < (1ll << 31) - 65536 && ld >= v && out_ld >= v && n < (1ll << 40) / v,
                "sbod_logits_process: logits [%lld, %lld], row strides %lld / %lld", static_cast<long long>(n),
                static_cast<long long>(v), static_cast<long long>(ld), static_cast<long long>(out_ld));
-  SBOD_REQUIRE(history_cols >= 0 && history_cols <= kCount && bias_cols >= 0 && bias_cols < 65536 && history_ld >= 0 && bias_ld >= 0 &&
+  SBOD_REQUIRE(history_cols >= 0 && history_cols <= kCount && bias_cols >= 0 && bias_cols <= kMaxBiases && history_ld >= 0 && bias_ld >= 0 &&
                    bias_ids_ld >= 0 && bias_values_ld >= 0 && mask_ld >= 0,
                "sbod_logits_process: negative size or stride");
   SBOD_REQUIRE(mask_kind == SBOD_MASK_NONE || ((mask_kind == SBOD_MASK_BITS || mask_kind == SBOD_MASK_BYTES) && mask),
@@ -265,12 +301,12 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
   const bool even = (reinterpret_cast<uintptr_t>(logits) | ld * elt_bytes(dtype)) % 16 == 0;
   const int64_t most = even ? v : v + 16 / static_cast<int64_t>(elt_bytes(dtype)) - 1;
   a.ntile = static_cast<int>((most + kLogTile - 1) / kLogTile);
-  a.tile = static_cast<int>(most < kLogTile ? (most + 7) / 8 * 8 : kLogTile);
+  a.tile = static_cast<int>(most < kLogTile ? (most + 31) / 32 * 32 : kLogTile);
   // threads for the tile's granules, two (four of float32) each
-  const dim3 block(a.tile <= 1024 + 8 ? 128 : a.tile <= kLogTile / 2 ? 256 : kLogThreads);
+  const dim3 block(a.tile <= 1024 ? 128 : a.tile <= kLogTile / 2 ? 256 : kLogThreads);
   const int64_t items = n * a.ntile;
   const dim3 grid(static_cast<unsigned>(items < 65536 ? items : 65536));
-  const size_t lds = a.len > 0 || a.m > 0 ? a.tile * (sizeof(uint32_t) + sizeof(uint16_t)) : 0;
+  const size_t lds = a.len > 0 || a.m > 0 ? a.tile * (sizeof(uint32_t) + sizeof(uint16_t)) + a.tile / 8 : 0;
   hipStream_t s = as_stream(stream);
   if (dtype == SBOD_DT_F32) launch_logits<SBOD_DT_F32>(a, grid, block, lds, s);
   else if (dtype == SBOD_DT_BF16) launch_logits<SBOD_DT_BF16>(a, grid, block, lds, s);
