@@ -549,6 +549,238 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
 constexpr int kSmallMax = 2048;   // labels k_distill_small holds
 constexpr int kSmallBlocks = 1280;
 
+// A vocabulary that a workgroup's registers hold: NT threads with NG 16-byte granules each keep the row from
+// its one read to its gradient's one write, and ask for the next row's granules as those of this one fall
+// free, so that loads, exponentials and stores of a CU overlap though it holds one row at a time.  Thread k
+// has kept entry k (K <= NT).  The elements before the row's first 16-byte boundary and behind its last
+// granule are one value each of the first 2 P threads.
+// With a bucket the kept labels leave the registers by a bit each in LDS, looked up a granule at a time.
+template <int DT, bool kBucket, int NT, int NG>
+__global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
+  using T = typename Elt<DT>::T;
+  constexpr int P = Elt<DT>::P, NW = NT / kWave;
+  constexpr uint32_t kInfBits = DT == SBOD_DT_F32 ? 0xff800000u : DT == SBOD_DT_BF16 ? 0xff80u : 0xfc00u;
+  // bit e - head + P: element e is kept (head: the elements before the first granule)
+  __shared__ uint32_t bits[kBucket ? NT * NG * P / 32 + 1 : 1];
+  __shared__ int ids_s[NT];
+  __shared__ float top_s[NT], red[2][NW], sums[3][NW];
+  __shared__ double red64[16];
+  if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
+  const int tid = threadIdx.x, wave = tid >> 6, v = static_cast<int>(a.v), kk = a.k;
+  if (kBucket)
+    for (int i = tid; i < NT * NG * P / 32 + 1; i += NT) bits[i] = 0;
+  const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
+  const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
+  double loss = 0;
+  const bool entry = tid < kk;
+  raw16_t raw[NG];
+  uint32_t xraw = 0;
+  RawId idr = {};
+  RawAny tr = {};
+  // where a row's granules lie, and which single element this thread has (-1: none)
+  const auto head_of = [&](const T *row) { return min((P - row_phase(row)) % P, v); };
+  const auto single = [&](int head) {
+    const int in = (v - head) / P, tail = v - head - in * P;
+    return tid < head ? tid : tid >= P && tid < P + tail ? head + in * P + tid - P : -1;
+  };
+  // (a granule's address is a scalar base and the thread's own offset, the same for all of them)
+  const uint32_t mine = static_cast<uint32_t>(tid) * 16;
+  const auto base_of = [&](const T *row, int head) { return reinterpret_cast<const char *>(row + head); };
+  const auto step_on = [&](const char *&at) {   // (one base that moves on, not one per granule kept)
+    at += NT * 16;
+    asm volatile("" : "+s"(at));
+  };
+  const auto fetch = [&](int i, const char *at, int granules) {
+    if (i * NT + tid < granules) raw[i] = *reinterpret_cast<const raw16_t *>(at + mine);
+  };
+  // The registers hold the row as it was read, a granule's work at a time.  Without this the compiler widens
+  // each element once and keeps twice the registers from pass to pass.
+  const auto as_read = [&](int i) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(raw[i]));
+  };
+  const auto fetch_rest = [&](int64_t r, const T *row, int head) {
+    const int e = single(head);
+    if (e >= 0) xraw = reinterpret_cast<const bits_t<DT> *>(row)[e];
+    if (entry) {
+      idr = ld_raw_id(a.ids, r * kk + tid, a.ids64);
+      tr = ld_raw_any(a.top, r * kk + tid, a.top_dt);
+    }
+  };
+  int64_t r = blockIdx.x;
+  float w_next = a.w && r < a.n ? a.w[r] : 1.f;
+  if (r < a.n && w_next != 0.f) {
+    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+    const int head = head_of(row);
+    const char *at = base_of(row, head);
+#pragma unroll
+    for (int i = 0; i < NG; ++i, step_on(at)) fetch(i, at, (v - head) / P);
+    fetch_rest(r, row, head);
+  }
+  for (; r < a.n; r += gridDim.x) {
+    const T *row = static_cast<const T *>(a.x) + r * a.ldx;
+    T *drow = static_cast<T *>(a.dx) + r * a.lddx;
+    const int head = head_of(row), inner = (v - head) / P, e1 = single(head);
+    const bool aligned = row_phase(drow) == row_phase(row);
+    const int64_t rn = r + gridDim.x;
+    const T *next = static_cast<const T *>(a.x) + rn * a.ldx;
+    const float w = w_next;
+    w_next = a.w && rn < a.n ? a.w[rn] : 1.f;
+    const bool ahead = rn < a.n && w_next != 0.f;
+    const int nhead = ahead ? head_of(next) : 0, ninner = ahead ? (v - nhead) / P : 0;
+    bool live = w != 0.f;
+    float mo = kNegInf, so = 0.f, base = 0.f, coef = 0.f, inv = 0.f, ek = 0.f, pk = 0.f, obase = 0.f;
+    int id = -1;
+    if (live) {
+      id = entry ? id_of(idr, a.ids64, a.v) : -1;
+      const float t = any_of(tr, a.top_dt);
+      uint32_t xk_raw = 0;
+      if (id >= 0) xk_raw = reinterpret_cast<const bits_t<DT> *>(row)[id];
+      const int place = id - head + P;
+      if (entry) ids_s[tid] = id, top_s[tid] = t;
+      if (kBucket && id >= 0) atomicOr(&bits[place >> 5], 1u << (place & 31));
+      __syncthreads();
+      float x1 = e1 >= 0 ? bits_value<DT>(xraw) : kNegInf;
+      if (kBucket && e1 >= 0 && bits[(e1 - head + P) >> 5] >> ((e1 - head + P) & 31) & 1) x1 = kNegInf;
+      mo = x1;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int g = i * NT + tid;
+        as_read(i);
+        // (by masks: a branch would hold the row twice where it joins)
+        uint32_t b = 0;
+        if (kBucket) {
+          int at = P == 8 ? g + 1 : (g + 1) >> 1;
+          asm volatile("" : "+v"(at));   // (looked up here, not ahead for all granules)
+          const uint32_t byte = reinterpret_cast<const uint8_t *>(bits)[at];
+          b = P == 8 ? byte : byte >> (4 * ((g + 1) & 1)) & 15;
+        }
+        b = g >= inner ? ~0u : b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const auto bit = [&](int k) { return static_cast<uint32_t>(static_cast<int32_t>(b << (31 - k)) >> 31); };
+          const uint32_t m = DT == SBOD_DT_F32 ? bit(j) : (bit(2 * j) & 0xffffu) | bit(2 * j + 1) << 16;
+          raw[i][j] = (raw[i][j] & ~m) | (m & (DT == SBOD_DT_F32 ? kInfBits : kInfBits << 16 | kInfBits));
+        }
+        as_read(i);
+        float f[P];
+        raw_values<DT>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) mo = fmaxf(mo, f[j]);
+      }
+      const float xk = bits_value<DT>(xk_raw);
+      float other = id < 0 ? kNegInf : kBucket ? xk : t;   // the kept logits, or the teacher's
+      mo = wave_max_f32(mo);
+      other = wave_max_f32(other);
+      if ((tid & 63) == 0) red[0][wave] = mo, red[1][wave] = other;
+      __syncthreads();
+      mo = group_max<NW>(red[0][tid % NW]), other = group_max<NW>(red[1][tid % NW]);
+      if (kBucket && id >= 0) bits[place >> 5] = 0;   // (read for the last time above)
+      obase = mo == kNegInf ? 0.f : mo;
+      const float m = kBucket ? fmaxf(mo, other) : mo;
+      base = m == kNegInf ? 0.f : m;
+      const float tb = kBucket || other == kNegInf ? 0.f : other;
+      float tl = kBucket ? a.lse[r] : 0.f;
+      const auto logp_at = [&](float q) { return static_cast<float>((static_cast<double>(q) - tb) * a.inv_td - tl); };
+      // listed before?  then the label counts at its first entry, and its masses are added in the list's order
+      bool first = id >= 0, again = false;
+      if (id >= 0)
+        for (int j = 0; j < kk; ++j)
+          if (j != tid && ids_s[j] == id) again = true, first = first && j > tid;
+      ek = id >= 0 ? exp2_hw((xk - base) * a.s) : 0.f;
+      float s1, s2 = 0.f;   // the teacher's normaliser; with a bucket the kept labels' sum and their mass
+      if (kBucket) {
+        pk = id >= 0 ? exp_hw(logp_at(t)) : 0.f;
+        s1 = first ? ek : 0.f;
+        s2 = pk;
+      } else {
+        s1 = id >= 0 ? exp_hw((t - tb) * a.inv_t) : 0.f;
+      }
+      so = exp2_hw((x1 - obase) * a.s);
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        float f[P];
+        as_read(i);
+        raw_values<DT>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) so += exp2_hw((f[j] - obase) * a.s);
+      }
+      so = group_sum<kWave>(so), s1 = group_sum<kWave>(s1);
+      if (kBucket) s2 = group_sum<kWave>(s2);
+      if ((tid & 63) == 0) sums[0][wave] = so, sums[1][wave] = s1, sums[2][wave] = s2;
+      __syncthreads();
+      so = group_sum<NW>(sums[0][tid % NW]), s1 = group_sum<NW>(sums[1][tid % NW]);
+      if (kBucket) s2 = group_sum<NW>(sums[2][tid % NW]);
+      const float sum = kBucket ? s1 + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s)) : so;
+      // a row of -inf alone has no distribution, a teacher without mass nothing to say: left out, as of weight 0
+      live = !(m == kNegInf && sum == 0.f) && (kBucket || !(s1 == 0.f));
+      const float logs = log_hw(sum);
+      if (!kBucket) {
+        tl = log_hw(s1);
+        pk = id >= 0 ? exp_hw(logp_at(t)) : 0.f;
+      }
+      inv = 1.f / sum;
+      coef = inv;
+      // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
+      double kl = pk == 0.f ? 0.0 : pk * (logp_at(t) - ((static_cast<double>(xk) - base) * a.inv_td - logs));
+      if (kBucket) {
+        float rest = 1.f - s2;
+        if (rest < 0.f) rest = 0.f;   // (K < V here: there is a label that is not kept)
+        const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + log_hw(so) - logs;
+        if (tid == 0) kl += rest > 0.f ? rest * (log_hw(rest) - logo) : rest;
+        coef = so == 0.f ? 0.f : (exp_hw(static_cast<float>(logo)) - rest) / so;
+      }
+      if (again) {
+        pk = 0.f;
+        for (int j = 0; j < kk; ++j)
+          if (ids_s[j] == id) pk += exp_hw(logp_at(top_s[j]));
+      }
+      kl = live ? kl * a.tt * w : 0.0;
+      loss += kl;
+      if (a.rows) {
+        kl = block_sum(kl, red64);
+        if (tid == 0) a.rows[r] = static_cast<float>(kl);
+      }
+    } else if (a.rows && tid == 0) {
+      a.rows[r] = 0.f;
+    }
+    float g = a.t * w * norm * up;
+    if (a.up && a.up_stride) g *= a.up[r];
+    const float gc = g * coef;
+    if (a.dx && e1 >= 0) drow[e1] = static_cast<T>(live && !(kBucket && so == 0.f) ? gc * exp2_hw((bits_value<DT>(xraw) - obase) * a.s) : 0.f);
+    const char *from = base_of(next, nhead), *to = base_of(drow, head);
+#pragma unroll
+    for (int i = 0; i < NG; ++i, step_on(from), step_on(to)) {
+      if (a.dx && i * NT + tid < inner) {
+        float f[P];
+        as_read(i);
+        raw_values<DT>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[j] = live ? gc * exp2_hw((f[j] - obase) * a.s) : 0.f;
+        T *at = reinterpret_cast<T *>(const_cast<char *>(to) + mine);
+        if (aligned) {
+          vec_t<T, P> o;
+#pragma unroll
+          for (int j = 0; j < P; ++j) o[j] = static_cast<T>(f[j]);
+          *reinterpret_cast<vec_t<T, P> *>(at) = o;
+        } else {
+#pragma unroll
+          for (int j = 0; j < P; ++j) at[j] = static_cast<T>(f[j]);
+        }
+      }
+      fetch(i, from, ninner);
+    }
+    __syncthreads();
+    // the kept labels, over what the row's pass wrote there
+    if (a.dx && live && id >= 0) drow[id] = static_cast<T>(g * (ek * inv - pk));
+    if (ahead) fetch_rest(rn, next, nhead);
+  }
+  if (a.parts) {
+    loss = block_sum(loss, red64);
+    if (tid == 0) a.parts[blockIdx.x] = loss;
+  }
+}
+
 int distill_chunks(int64_t v, int dt) {
   const int64_t per = static_cast<int64_t>(kDistGran) * 16 / elt_bytes(dt);
   return static_cast<int>((v + 16 / elt_bytes(dt) - 1 + per - 1) / per);   // (a phase of P - 1 at most)
@@ -610,14 +842,48 @@ int launch_small(const DistillArgs &a, hipStream_t s) {
   return SBOD_OK;
 }
 
+// Threads and granules of k_distill_row for a row, smallest first, and the workgroups that the device holds at
+// once.  With a bucket the longest rows' lookups do not fit the registers beside them (-1: k_distill_part and
+// the kernels behind it).
+struct RowShape {
+  int nt, ng, groups;
+};
+constexpr RowShape kRowShapes[] = {{256, 4, 1280}, {256, 8, 1024}, {256, 16, 1024}, {512, 16, 512}, {1024, 16, 256}};
+int row_shape(int64_t v, int k, int dt, bool bucket) {
+  const int64_t granules = v / static_cast<int64_t>(16 / elt_bytes(dt));
+  for (int i = 0; i < (bucket ? 4 : 5); ++i)
+    if (kRowShapes[i].nt >= k && static_cast<int64_t>(kRowShapes[i].nt) * kRowShapes[i].ng >= granules) return i;
+  return -1;
+}
+
 // Which kernels take a call.
-enum Path { kSmall, kChunks };
-Path path_of(int64_t v) { return v <= kSmallMax ? kSmall : kChunks; }
+enum Path { kSmall, kRow, kChunks };
+Path path_of(int64_t v, int k, int dt, bool bucket) {
+  return v <= kSmallMax ? kSmall : row_shape(v, k, dt, bucket) >= 0 ? kRow : kChunks;
+}
+int64_t row_blocks(int64_t n, int shape) { return n < kRowShapes[shape].groups ? n : kRowShapes[shape].groups; }
+
+template <int DT, bool kBucket>
+int launch_row(const DistillArgs &a, hipStream_t s) {
+  const int shape = row_shape(a.v, a.k, DT, kBucket);
+  const dim3 grid(static_cast<unsigned>(row_blocks(a.n, shape))), block(kRowShapes[shape].nt);
+#define SBOD_ROW(I) hipLaunchKernelGGL((k_distill_row<DT, kBucket, kRowShapes[I].nt, kRowShapes[I].ng>), grid, block, 0, s, a)
+  if (shape == 0) SBOD_ROW(0);
+  else if (shape == 1) SBOD_ROW(1);
+  else if (shape == 2) SBOD_ROW(2);
+  else if (shape == 3) SBOD_ROW(3);
+  else if constexpr (!kBucket) SBOD_ROW(4);
+#undef SBOD_ROW
+  SBOD_LAUNCHED("k_distill_row");
+  return SBOD_OK;
+}
 
 // The forward's, or with a.up the gradient's, launches of one type.
 template <int DT, bool kBucket>
 int launch_typed(const DistillArgs &a, hipStream_t s) {
-  if (path_of(a.v) == kSmall) return launch_small<DT, kBucket>(a, s);
+  const Path p = path_of(a.v, a.k, DT, kBucket);
+  if (p == kSmall) return launch_small<DT, kBucket>(a, s);
+  if (p == kRow) return launch_row<DT, kBucket>(a, s);
   if (!a.up) {
     const int st = launch_rows<DT, kBucket>(a, s);
     if (st != SBOD_OK) return st;
@@ -632,8 +898,13 @@ int launch_any(const DistillArgs &a, int dt, hipStream_t s) {
 
 // The forward's workspace: partial weight sums | loss parts | chunk statistics.
 size_t parts_offset() { return kWeightParts * sizeof(double); }
-int64_t parts_count(int64_t n, int64_t v, int k) { return path_of(v) == kSmall ? small_blocks(n, small_lanes(v, k)) : n; }
-size_t chunks_offset(int64_t n, int64_t v, int k) { return align_up(parts_offset() + parts_count(n, v, k) * sizeof(double)); }
+int64_t parts_count(int64_t n, int64_t v, int k, int dt, bool bucket) {
+  const Path p = path_of(v, k, dt, bucket);
+  return p == kSmall ? small_blocks(n, small_lanes(v, k)) : p == kRow ? row_blocks(n, row_shape(v, k, dt, bucket)) : n;
+}
+size_t chunks_offset(int64_t n, int64_t v, int k, int dt, bool bucket) {
+  return align_up(parts_offset() + parts_count(n, v, k, dt, bucket) * sizeof(double));
+}
 
 int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, int64_t ldx, const void *ids,
                  const void *top, int top_dt, int k, float temperature, int reduction) {
@@ -664,10 +935,10 @@ using namespace sbod::label;
 
 extern "C" int sbod_distill_stat_floats(void) { return kStats; }
 
-extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int dtype) {
-  if (n < 0 || v <= 0 || k <= 0 || !known_dt(dtype)) return 0;
-  const size_t chunks = path_of(v) == kChunks ? static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2) : 0;
-  return chunks_offset(n, v, k) + chunks;
+extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int has_lse, int dtype) {
+  if (n < 0 || v <= 0 || k <= 0 || k > kMaxTop || !known_dt(dtype)) return 0;
+  const size_t chunks = path_of(v, k, dtype, has_lse) == kChunks ? static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2) : 0;
+  return chunks_offset(n, v, k, dtype, has_lse) + chunks;
 }
 
 extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -681,8 +952,8 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || (loss && norm), "sbod_distill_fwd: a reduction needs loss and norm");
   SBOD_REQUIRE(!grad || (grad_ld >= v && reduction != SBOD_REDUCE_NONE), "sbod_distill_fwd: gradient with row stride %lld, reduction %d",
                static_cast<long long>(grad_ld), reduction);
-  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, k, dtype) || !workspace) {
-    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, k, dtype));
+  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, k, lse != nullptr, dtype) || !workspace) {
+    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, k, lse != nullptr, dtype));
     return SBOD_E_WORKSPACE;
   }
   hipStream_t s = as_stream(stream);
@@ -690,10 +961,10 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   a.x = logits, a.n = n, a.v = v, a.ldx = ld, a.ids = ids, a.ids64 = ids64, a.top = top, a.top_dt = top_dtype;
   a.k = k, a.lse = lse, a.w = weights, a.stats = stats, a.reduction = reduction;
   a.rows = reduction == SBOD_REDUCE_NONE ? rows : nullptr;
-  a.part = ws_at<float2>(workspace, chunks_offset(n, v, k)), a.nchunk = distill_chunks(v, dtype);
+  a.part = ws_at<float2>(workspace, chunks_offset(n, v, k, dtype, lse)), a.nchunk = distill_chunks(v, dtype);
   a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
-  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v, k);
+  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v, k, dtype, lse);
   if (reduction == SBOD_REDUCE_MEAN && weights) {
     // (64 partial sums: each workgroup of the loss joins them)
     a.wparts = static_cast<const double *>(workspace);
@@ -711,7 +982,7 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   a.loss = loss, a.norm = norm;
   hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, s, a);
   SBOD_LAUNCHED("k_distill_sum");
-  return grad && n > 0 && path_of(v) == kChunks ? launch_grad(a, dtype, s) : SBOD_OK;
+  return grad && n > 0 && path_of(v, k, dtype, lse) == kChunks ? launch_grad(a, dtype, s) : SBOD_OK;
 }
 
 extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -733,5 +1004,5 @@ extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_
   a.stats = const_cast<float *>(stats), a.up = upstream, a.up_stride = reduction == SBOD_REDUCE_NONE ? 1 : 0;
   a.nchunk = distill_chunks(v, dtype), a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
-  return path_of(v) == kSmall ? launch_any(a, dtype, as_stream(stream)) : launch_grad(a, dtype, as_stream(stream));
+  return path_of(v, k, dtype, lse) != kChunks ? launch_any(a, dtype, as_stream(stream)) : launch_grad(a, dtype, as_stream(stream));
 }
