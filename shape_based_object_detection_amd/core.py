@@ -1180,6 +1180,19 @@ def deform_conv2d(x, offset, mask_logits, weight, ks=3, padding=1, stride=1):
 
 
 # ----------------------------------------------------------------------------- label vocabularies
+def differentiable_once(backward):
+    """Decorator of an autograd backward that only kernels compute: differentiating its (first) gradient raises,
+    whatever the upstream gradient is."""
+    def run(ctx, g):
+        with torch.no_grad():
+            out = backward(ctx, g)
+        if not torch.is_grad_enabled() or out[0] is None:
+            return out
+        late = torch._C._functions.DelayedError(b'trying to differentiate twice a function that is differentiable once', 1)
+        return (late(out[0].detach().requires_grad_(True)),) + tuple(out[1:])
+    return run
+
+
 def _on_device(t):
     """Context that makes ``t``'s device current for launches (nothing to do when it is)."""
     if t.get_device() == torch.cuda.current_device():
@@ -1226,6 +1239,23 @@ def _empty_rows(t):
     if shift == 0 and ld == v:
         return torch.empty_like(t, memory_format=torch.contiguous_format)
     return torch.empty(n * ld + shift, dtype=t.dtype, device=t.device).as_strided((n, v), (ld, 1), shift)
+
+
+def label_call(name, t, *args):
+    """A label-vocabulary call in C++ (_sbodhost, csrc/host_label.h): its result, or None when it needs this module's
+    path (CPU tensors, conversions, errors, no extension, or a caller that records the sbod_* calls)."""
+    ext = L.host_ext
+    if ext is None or L._recorder or not t.is_cuda:
+        return None
+    r = getattr(ext, name)(*args, L._raw_stream(t.get_device()))
+    if type(r) is int:
+        raise L.SbodError('%s failed (%d): %s' % (name, r, L.lib().sbod_last_error().decode(errors='replace')))
+    return r
+
+
+def unit_pointer(t):
+    u = _UNIT.get(t.device)
+    return None if u is None else u.data_ptr()
 
 
 def distill_arguments(logits, ids, top, lse, weights, temperature, reduction):
@@ -1282,7 +1312,7 @@ class _TopKDistill(torch.autograd.Function):
         return loss if red else rows
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiable_once
     def backward(ctx, g):
         none = (None,) * 7
         if g is None:
@@ -1458,6 +1488,8 @@ def process_logits(logits, history, history_len, prompt_len, repetition, presenc
                int(bias_ids is not None and bias_ids.dtype == torch.int64), L.ptr(bias_values),
                0 if bias_ids is None else bias_ids.shape[-1], ldi, ldv, L.ptr(allowed), kind, ldm, L.ptr(dst),
                _row_stride(dst), L.stream_of(x))
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
     return result
 
 
@@ -1493,7 +1525,7 @@ class _ScaledEmbedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @differentiable_once
     def backward(ctx, g):
         (ids,) = ctx.saved_tensors
         v, d, wide, scale, pad = ctx.args

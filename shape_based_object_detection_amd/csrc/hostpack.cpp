@@ -30,6 +30,7 @@
 #include <cstdint>
 #include <vector>
 
+#include "host_label.h"
 #include "sbod.h"
 
 namespace {
@@ -568,6 +569,12 @@ PyObject *criterion_focal_fast(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
+    {"label_distill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::label_distill)),
+     METH_FASTCALL, "operators.Loss.topk_distill_loss on device tensors (host_label.h)."},
+    {"label_embed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::label_embed)),
+     METH_FASTCALL, "operators.Embedding.scaled_embedding on device tensors (host_label.h)."},
+    {"label_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::label_logits)),
+     METH_FASTCALL, "operators.Logits.process_logits on device tensors (host_label.h)."},
     {"criterion_focal_fast",
      reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(criterion_focal_fast)),
      METH_FASTCALL, "GT packing + sbod_criterion_focal + a C++ autograd node for the loss."},

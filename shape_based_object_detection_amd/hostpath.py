@@ -17,7 +17,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import host
+from . import core, host
 
 # ----------------------------------------------------------------------------- aligned overlaps
 
@@ -493,7 +493,7 @@ class _TopKDistill(torch.autograd.Function):
         return (temperature * temperature * kl).masked_fill(~live, 0.0)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @core.differentiable_once
     def backward(ctx, g):
         (grad,) = ctx.saved_tensors
         g = g.masked_fill(~ctx.live, 0.0)
@@ -570,7 +570,7 @@ class _ScaledEmbedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @core.differentiable_once
     def backward(ctx, g):
         flat, live = ctx.saved_tensors
         shape, scale, wide = ctx.args

@@ -28,6 +28,10 @@ def process_logits(logits, history=None, history_len=None, prompt_len=None, repe
     ``repetition`` (> 0), ``presence``, ``frequency``: numbers, or float tensors [N].  An id outside [0, V) is
     absent (padding).  Not differentiable: logits that require a gradient are refused while gradients are on.
     """
+    r = core.label_call('label_logits', logits, logits, history, history_len, prompt_len, repetition, presence, frequency,
+                        bias, bias_ids, bias_values, allowed, out)
+    if r is not None:
+        return r
     args = core.logits_arguments(logits, history, history_len, prompt_len, repetition, presence, frequency, bias,
                                  bias_ids, bias_values, allowed, out)
     if on_host(*[t for t in args if hasattr(t, 'is_cuda')]):

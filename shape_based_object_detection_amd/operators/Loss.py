@@ -10,6 +10,7 @@ from torch import nn
 
 from .. import core
 from .. import hostpath
+from .._lib import REDUCE
 from ..metrics import on_host
 from .iou_utils import bbox_overlaps_ciou, bbox_overlaps_diou, bbox_overlaps_giou, bbox_overlaps_iou
 
@@ -125,6 +126,11 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, wei
     is 0), 'sum' adds, 'none' returns the weighted row losses [...].  Loss in float32, gradient in the logits'
     type.  A row of weight 0, without an entry that has mass, or whose logits are all -inf gives loss 0 and a zero
     gradient.  The teacher's tensors and the weights are constants: one that requires a gradient is refused."""
+    if reduction in REDUCE and torch.is_tensor(logits):
+        r = core.label_call('label_distill', logits, logits, teacher_ids, teacher_logits, teacher_lse, weights,
+                            float(temperature), REDUCE[reduction], core.unit_pointer(logits))
+        if r is not None:
+            return r
     core.distill_arguments(logits, teacher_ids, teacher_logits, teacher_lse, weights, temperature, reduction)
     on = on_host(*[t for t in (logits, teacher_ids, teacher_logits, teacher_lse, weights) if t is not None])
     run = hostpath.topk_distill if on else core.topk_distill

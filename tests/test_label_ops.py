@@ -181,6 +181,16 @@ def test_entry_points_refuse_before_any_launch():
             L.call(name, *args)
 
 
+def test_gradients_are_not_differentiable_again():
+    x, ids, top, _ = C.distill_inputs(3, 7, 2, torch.float32, 0)
+    x.requires_grad_(True)
+    table = torch.randn(7, 4, requires_grad=True)
+    for out, leaf in ((topk_distill_loss(x, ids, top), x), (scaled_embedding(ids, table).sum(), table)):
+        g, = torch.autograd.grad(out, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match='twice'):
+            g.square().sum().backward()
+
+
 def test_module_holds_its_settings():
     x, ids, top, _ = C.distill_inputs(3, 7, 2, torch.float32, 0)
     m = TopKDistillLoss(temperature=2.0, reduction='sum')
