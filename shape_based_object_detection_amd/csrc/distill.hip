@@ -80,19 +80,25 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_part(DistillArgs a) {
     if (!row_has_weight(a, r)) continue;
     const T *row = static_cast<const T *>(a.x) + r * a.ldx;
     const int64_t e0 = (it - r * a.nchunk) * kDistGran * P - row_phase(row);
+    // (whole granules are asked for together; the two that the row's ends cut, element by element)
+    raw16_t raw[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int64_t e = e0 + static_cast<int64_t>(i * kDistThreads + threadIdx.x) * P;
+      if (e >= 0 && e + P <= a.v) raw[i] = *reinterpret_cast<const raw16_t *>(row + e);
+    }
     if (kBucket) mark_kept(a, r, e0, bits, kDistGran * P / 32);
     float f[kPer][P], m = kNegInf;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      ld_granule<DT>(row, e0 + static_cast<int64_t>(i * kDistThreads + threadIdx.x) * P, a.v, kNegInf, f[i]);
-#pragma unroll
     for (int i = 0; i < kPer; ++i) {
+      const int g = i * kDistThreads + threadIdx.x;
+      const int64_t e = e0 + static_cast<int64_t>(g) * P;
+      if (e >= 0 && e + P <= a.v) raw_values<DT>(raw[i], f[i]);
+      else ld_granule<DT>(row, e, a.v, kNegInf, f[i]);
       if (kBucket) {
-        const int g = i * kDistThreads + threadIdx.x;
         const uint32_t b = bits[g * P >> 5] >> (g * P & 31);
 #pragma unroll
-        for (int j = 0; j < P; ++j)
-          if (b >> j & 1) f[i][j] = kNegInf;
+        for (int j = 0; j < P; ++j) f[i][j] = b >> j & 1 ? kNegInf : f[i][j];
       }
 #pragma unroll
       for (int j = 0; j < P; ++j) m = fmaxf(m, f[i][j]);
@@ -190,8 +196,9 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
       float sk = 0.f;
       for (int k = lane; k < a.k; k += kWave) {
         const int id = ids_s[wv][k];
-        bool first = id >= 0;
-        for (int j = 0; j < k && first; ++j) first = ids_s[wv][j] != id;
+        bool first = id >= 0;   // (no early end: the reads are in flight together)
+#pragma unroll 8
+        for (int j = 0; j < k; ++j) first = first && ids_s[wv][j] != id;
         if (first) {
           sk += exp2_hw((static_cast<float>(row[id]) - base) * a.s);
           ++kept;
@@ -285,7 +292,8 @@ __global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
 }
 
 // dx of one chunk of a row from the row's statistics.  The kept labels are written a second time,
-// behind a barrier, by a thread each.
+// behind a barrier, by a thread each.  The rows are taken from the last to the first: the ones that
+// k_distill_part read last are still in the Infinity Cache (256 MB), and the gradient is stored past it.
 template <int DT>
 __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -294,8 +302,8 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   __shared__ float p_s[kMaxTop];
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int64_t items = a.n * a.nchunk;
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t r = it / a.nchunk;
+  for (int64_t at = blockIdx.x; at < items; at += gridDim.x) {
+    const int64_t it = items - 1 - at, r = it / a.nchunk;
     const T *row = static_cast<const T *>(a.x) + r * a.ldx;
     T *drow = static_cast<T *>(a.dx) + r * a.lddx;
     const int phase = row_phase(row);
@@ -326,7 +334,7 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
       ld_granule<DT>(row, e, a.v, kNegInf, f);
 #pragma unroll
       for (int j = 0; j < P; ++j) f[j] = gc * exp2_hw((f[j] - mo) * a.s - l2so);
-      st_granule<DT>(drow, e, a.v, aligned, f);
+      st_granule<DT, true>(drow, e, a.v, aligned, f);
     }
     __syncthreads();
     for (int k = threadIdx.x; k < a.k; k += kDistThreads) {

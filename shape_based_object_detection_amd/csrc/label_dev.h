@@ -122,8 +122,9 @@ __device__ __forceinline__ void ld_granule(const typename Elt<DT>::T *p, int64_t
   }
 }
 
-// The same elements written.  `aligned`: p + e is 16-byte aligned; else element by element.
-template <int DT>
+// The same elements written.  `aligned`: p + e is 16-byte aligned; else element by element.  kStream: past
+// the caches.
+template <int DT, bool kStream = false>
 __device__ __forceinline__ void st_granule(typename Elt<DT>::T *p, int64_t e, int64_t v, bool aligned,
                                            const float (&f)[Elt<DT>::P]) {
   using T = typename Elt<DT>::T;
@@ -132,7 +133,8 @@ __device__ __forceinline__ void st_granule(typename Elt<DT>::T *p, int64_t e, in
     vec_t<T, P> r;
 #pragma unroll
     for (int j = 0; j < P; ++j) r[j] = static_cast<T>(f[j]);
-    *reinterpret_cast<vec_t<T, P> *>(p + e) = r;
+    if (kStream) __builtin_nontemporal_store(r, reinterpret_cast<vec_t<T, P> *>(p + e));
+    else *reinterpret_cast<vec_t<T, P> *>(p + e) = r;
   } else {
 #pragma unroll
     for (int j = 0; j < P; ++j)
