@@ -156,9 +156,34 @@ __device__ __forceinline__ bool teacher_norm(const DistillArgs &a, int64_t r, in
   return !(sum == 0.f);
 }
 
-// (the difference in 64 bits: with lse, t / T and lse are large against it)
-__device__ __forceinline__ float teacher_logp(const DistillArgs &a, int64_t i, float tb, float tl) {
-  return static_cast<float>((static_cast<double>(ld_any(a.top, i, a.top_dt)) - tb) * a.inv_td - tl);
+// The bucket of a row: the teacher's mass outside the kept labels, 1 - mass, against the student's, q_o.
+// term: its part of the KL; coef: q_o - rest.  Both sides are near 1 where the kept labels hold little, so
+// their logarithms and their difference are then taken from what the kept labels hold (P - Q = q_o - rest);
+// `mass` comes in 64 bits, for where they hold nearly all.  others: there is a label that is not kept (else
+// what is left of the teacher's mass is rounding).
+struct Bucket {
+  double term;
+  float coef;
+};
+__device__ __forceinline__ Bucket bucket_of(const DistillArgs &a, double mass, float kept, float sum, float so, float mo,
+                                            float base, bool others) {
+  double rest = 1.0 - mass;
+  if (rest < 0 || !others) rest = 0;
+  const float q = kept / sum;
+  const bool little = q < 0.5f;
+  const double logr = mass < 0.5 ? log1pf(static_cast<float>(-mass)) : logf(static_cast<float>(rest));
+  const double logo = so == 0.f ? kNegInf
+                      : little  ? log1pf(-q)
+                                : (static_cast<double>(mo) - base) * a.inv_td + logf(so) - logf(sum);
+  Bucket b;
+  b.term = rest > 0 ? rest * (logr - logo) : rest;
+  b.coef = little && mass < 1 && others ? static_cast<float>(mass - q) : static_cast<float>(expf(static_cast<float>(logo)) - rest);
+  return b;
+}
+
+// (in 64 bits: with lse, t / T and lse are large against their difference)
+__device__ __forceinline__ double teacher_logp(const DistillArgs &a, int64_t i, float tb, float tl) {
+  return (static_cast<double>(ld_any(a.top, i, a.top_dt)) - tb) * a.inv_td - tl;
 }
 
 // One wave per row: the chunks joined, the teacher's side, the row's loss and statistics.
@@ -182,7 +207,7 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
       so = wave_sum_f32(so);
     }
     const T *row = static_cast<const T *>(a.x) + r * a.ldx;
-    float m = mo, sum = so;
+    float m = mo, sum = so, ksum = 0.f;
     int kept = 0;   // different labels kept
     if (live && kBucket) {
       for (int k = lane; k < a.k; k += kWave) {
@@ -205,7 +230,8 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
         }
       }
       kept = wave_sum_i32(kept);
-      sum = wave_sum_f32(sk) + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
+      ksum = wave_sum_f32(sk);
+      sum = ksum + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
       wave_lds_fence();
     }
     // a row of -inf alone has no distribution: it is left out, as one of weight 0
@@ -217,12 +243,12 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
     }
     const float logs = logf(sum);
     // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
-    double kl = 0;
-    float mass = 0.f;
+    double kl = 0, mass = 0;
     for (int k = lane; k < a.k; k += kWave) {
       const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
       if (id < 0) continue;
-      const float logp = teacher_logp(a, r * a.k + k, tb, tl), p = expf(logp);
+      const double logp = teacher_logp(a, r * a.k + k, tb, tl);
+      const float p = expf(static_cast<float>(logp));
       const double logq = (static_cast<double>(row[id]) - m) * a.inv_td - logs;
       if (p != 0.f) kl += p * (logp - logq);   // 0 log 0 = 0
       mass += p;
@@ -230,13 +256,9 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
     kl = wave_sum_f64(kl);
     float coef = 1.f;
     if (kBucket) {
-      mass = wave_sum_f32(mass);
-      float rest = 1.f - mass;
-      // (no label outside the kept ones: what is left of the teacher's mass is rounding)
-      if (rest < 0.f || kept == a.v) rest = 0.f;
-      const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - m) * a.inv_td + logf(so) - logs;
-      kl += rest > 0.f ? rest * (logf(rest) - logo) : rest;
-      coef = expf(static_cast<float>(logo)) - rest;
+      const Bucket b = bucket_of(a, wave_sum_f64(mass), ksum, sum, so, mo, m, kept < a.v);
+      kl += b.term;
+      coef = b.coef;
     }
     if (lane == 0) {
       st[kStM] = m;
@@ -326,7 +348,7 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
     for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
       const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
       ids_s[k] = id;
-      p_s[k] = id >= 0 ? expf(teacher_logp(a, r * a.k + k, tb, tl)) : 0.f;
+      p_s[k] = id >= 0 ? expf(static_cast<float>(teacher_logp(a, r * a.k + k, tb, tl))) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -441,7 +463,9 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     }
     // (the difference in 64 bits: with lse, t / T and lse are large against it)
     const auto logp_at = [&](float t) { return static_cast<float>((static_cast<double>(t) - tb) * a.inv_td - tl); };
-    const float logp0 = logp_at(t0), p0 = has0 ? exp_hw(logp0) : 0.f;
+    // (with a bucket the masses' sum counts to the last bit: bucket_of)
+    const auto p_at = [&](float logp) { return kBucket ? expf(logp) : exp_hw(logp); };
+    const float logp0 = logp_at(t0), p0 = has0 ? p_at(logp0) : 0.f;
     // the kept labels' bits; a label that is there already is listed twice
     bool twice = false;
     if (has0) {
@@ -483,7 +507,8 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     }
     so = group_sum<G>(so);
     const float e0 = has0 ? exp2_hw((x0 - base) * a.s) : 0.f;
-    float sum = so, mass = 0.f;
+    float sum = so, ksum = 0.f;
+    double mass = 0;
     if (kBucket) {
       // (a label listed twice counts once, at its first entry: the sums' order is the list's)
       const auto first = [&](int k, int id) {
@@ -495,9 +520,9 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
       mass = p0;
       more([&](int k, int id, float t, float x) {
         if (!twice || first(k, id)) sk += exp2_hw((x - base) * a.s);
-        mass += exp_hw(logp_at(t));
+        mass += p_at(logp_at(t));
       });
-      sk = group_sum<G>(sk);
+      ksum = sk = group_sum<G>(sk);
       mass = group_sum<G>(mass);
       sum = sk + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
     }
@@ -507,17 +532,14 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     float coef = inv;   // what a label not kept takes of its exponential
     // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
     const auto term = [&](float p, float logp, float x) {   // 0 log 0 = 0
-      return p == 0.f ? 0.0 : p * (logp - ((static_cast<double>(x) - base) * a.inv_td - logs));
+      return p == 0 ? 0.0 : p * (logp - ((static_cast<double>(x) - base) * a.inv_td - logs));
     };
     double kl = has0 ? term(p0, logp0, x0) : 0.0;
-    more([&](int, int, float t, float x) { kl += term(exp_hw(logp_at(t)), logp_at(t), x); });
+    more([&](int, int, float t, float x) { kl += term(p_at(logp_at(t)), logp_at(t), x); });
     if (kBucket) {
-      float rest = 1.f - mass;
-      // (no label outside the kept ones: what is left of the teacher's mass is rounding)
-      if (rest < 0.f || !others) rest = 0.f;
-      const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + log_hw(so) - logs;
-      if (lane == 0) kl += rest > 0.f ? rest * (log_hw(rest) - logo) : rest;
-      coef = so == 0.f ? 0.f : (exp_hw(static_cast<float>(logo)) - rest) / so;
+      const Bucket b = bucket_of(a, mass, ksum, sum, so, mo, base, others);
+      if (lane == 0) kl += b.term;
+      coef = so == 0.f ? 0.f : b.coef / so;
     }
     kl = live ? kl * a.tt * w : 0.0;
     if (a.rows) {
@@ -532,12 +554,13 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
       if (!twice) return p;
       p = 0.f;
       for (int i = 0; i < kk; ++i)
-        if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) p += exp_hw(logp_at(ld_any(a.top, r * kk + i, a.top_dt)));
+        if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id)
+          p += p_at(logp_at(ld_any(a.top, r * kk + i, a.top_dt)));
       return p;
     };
     if (has0) own[id0] = g * (e0 * inv - mass_of(id0, p0));
     more([&](int, int id, float t, float x) {
-      own[id] = g * (exp2_hw((x - base) * a.s) * inv - mass_of(id, exp_hw(logp_at(t))));
+      own[id] = g * (exp2_hw((x - base) * a.s) * inv - mass_of(id, p_at(logp_at(t))));
     });
     wave_lds_fence();
     const float gc = g * coef;
@@ -571,8 +594,8 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   // bit e - head + P: element e is kept (head: the elements before the first granule)
   __shared__ uint32_t bits[kBucket ? NT * NG * P / 32 + 1 : 1];
   __shared__ int ids_s[NT];
-  __shared__ float top_s[NT], red[2][NW], sums[3][NW];
-  __shared__ double red64[16];
+  __shared__ float top_s[NT], red[2][NW], sums[2][NW];
+  __shared__ double red64[16], masses[NW];
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int tid = threadIdx.x, wave = tid >> 6, v = static_cast<int>(a.v), kk = a.k;
   if (kBucket)
@@ -690,17 +713,18 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       const float tb = kBucket || other == kNegInf ? 0.f : other;
       float tl = kBucket ? a.lse[r] : 0.f;
       const auto logp_at = [&](float q) { return static_cast<float>((static_cast<double>(q) - tb) * a.inv_td - tl); };
+      const auto p_at = [&](float logp) { return kBucket ? expf(logp) : exp_hw(logp); };
       // listed before?  then the label counts at its first entry, and its masses are added in the list's order
       bool first = id >= 0, again = false;
       if (id >= 0)
         for (int j = 0; j < kk; ++j)
           if (j != tid && ids_s[j] == id) again = true, first = first && j > tid;
       ek = id >= 0 ? exp2_hw((xk - base) * a.s) : 0.f;
-      float s1, s2 = 0.f;   // the teacher's normaliser; with a bucket the kept labels' sum and their mass
+      float s1;         // the teacher's normaliser; with a bucket the kept labels' sum,
+      double s2 = 0;    // and their mass, in 64 bits (bucket_of)
       if (kBucket) {
-        pk = id >= 0 ? exp_hw(logp_at(t)) : 0.f;
+        s2 = pk = id >= 0 ? p_at(logp_at(t)) : 0.f;
         s1 = first ? ek : 0.f;
-        s2 = pk;
       } else {
         s1 = id >= 0 ? exp_hw((t - tb) * a.inv_t) : 0.f;
       }
@@ -715,33 +739,31 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       }
       so = group_sum<kWave>(so), s1 = group_sum<kWave>(s1);
       if (kBucket) s2 = group_sum<kWave>(s2);
-      if ((tid & 63) == 0) sums[0][wave] = so, sums[1][wave] = s1, sums[2][wave] = s2;
+      if ((tid & 63) == 0) sums[0][wave] = so, sums[1][wave] = s1, masses[wave] = s2;
       __syncthreads();
       so = group_sum<NW>(sums[0][tid % NW]), s1 = group_sum<NW>(sums[1][tid % NW]);
-      if (kBucket) s2 = group_sum<NW>(sums[2][tid % NW]);
+      if (kBucket) s2 = group_sum<NW>(masses[tid % NW]);
       const float sum = kBucket ? s1 + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s)) : so;
       // a row of -inf alone has no distribution, a teacher without mass nothing to say: left out, as of weight 0
       live = !(m == kNegInf && sum == 0.f) && (kBucket || !(s1 == 0.f));
       const float logs = log_hw(sum);
       if (!kBucket) {
         tl = log_hw(s1);
-        pk = id >= 0 ? exp_hw(logp_at(t)) : 0.f;
+        pk = id >= 0 ? p_at(logp_at(t)) : 0.f;
       }
       inv = 1.f / sum;
       coef = inv;
       // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
       double kl = pk == 0.f ? 0.0 : pk * (logp_at(t) - ((static_cast<double>(xk) - base) * a.inv_td - logs));
       if (kBucket) {
-        float rest = 1.f - s2;
-        if (rest < 0.f) rest = 0.f;   // (K < V here: there is a label that is not kept)
-        const double logo = so == 0.f ? kNegInf : (static_cast<double>(mo) - base) * a.inv_td + log_hw(so) - logs;
-        if (tid == 0) kl += rest > 0.f ? rest * (log_hw(rest) - logo) : rest;
-        coef = so == 0.f ? 0.f : (exp_hw(static_cast<float>(logo)) - rest) / so;
+        const Bucket b = bucket_of(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
+        if (tid == 0) kl += b.term;
+        coef = so == 0.f ? 0.f : b.coef / so;
       }
       if (again) {
         pk = 0.f;
         for (int j = 0; j < kk; ++j)
-          if (ids_s[j] == id) pk += exp_hw(logp_at(top_s[j]));
+          if (ids_s[j] == id) pk += p_at(logp_at(top_s[j]));
       }
       kl = live ? kl * a.tt * w : 0.0;
       loss += kl;

@@ -138,6 +138,31 @@ def test_distill_backward_forms(dt, v):
     assert torch.allclose(x.grad[3:9].float(), 2 * g1[3:9].float(), rtol=4 * C.half_step(dt), atol=1e-6)
 
 
+@DT
+@pytest.mark.parametrize('v', [700, 30011, 90001])
+def test_distill_bucket_that_holds_nearly_all(dt, v):
+    """Kept labels with little mass on both sides: rest and q_o are 1 but for it, and the loss is far below the rounding
+    of 1.  It is off by what its terms are, each a share P (teacher) or Q (student) of the mass."""
+    n, k, T = 6, 4, 4.0
+    x, ids, top, lse = C.distill_inputs(n, v, k, dt, 21, True, spread=1.0)
+    top = (0.2 * top.float()).to(dt)
+    lse = torch.full((n,), 11.0)
+    loss, grad = run_distill(*dev(x, ids, top, lse), T=T, reduction='none', upstream=torch.ones(n, device=DEV))
+    want, gwant, _ = R.distill(x.double().numpy(), ids.numpy(), top.double().numpy(), lse.double().numpy(), None, T, 'none')
+    z = x.double().numpy() / T
+    q = np.exp(z - z.max(1, keepdims=True))
+    q /= q.sum(1, keepdims=True)
+    P = np.exp(top.double().numpy() / T - 11.0).sum(1)
+    Q = np.take_along_axis(q, ids.numpy(), 1).sum(1)
+    A, B = np.ptp(z, axis=1), 11.0 + np.abs(top.double().numpy()).max(1) / T
+    rel = C.STEP * (105 + 4 * A + 4 * B + k + 4 * math.log(v + 1.0))
+    assert (P < 1e-3).all() and (Q < 0.02).all()
+    assert np.all(np.abs(loss.detach().double().cpu().numpy() - want) <= T * T * rel * (2 + A + B) * 2 * (P + Q) + C.STEP * want)
+    # others: share (P - Q), each of P and Q off by rel of itself
+    tol = C.half_step(dt) * 1.001 * np.abs(gwant) + C.smallest(dt) + T * rel[:, None] * 4 * (np.abs(gwant) / T + q * (P + Q)[:, None])
+    assert np.all(np.abs(grad.double().cpu().numpy() - gwant) <= tol)
+
+
 def test_distill_half_gradients_do_not_underflow():
     """Half precision's mean over many rows is below its smallest value until the loss scale reaches it."""
     x, ids, top, _ = dev(*C.distill_inputs(2048, 640, 4, torch.float16, 2, spread=0.1))
