@@ -476,7 +476,7 @@ int sbod_map_f32(const float *det_boxes, const int64_t *det_labels, const float 
  * call gives the same bits.  A workspace belongs to one call at a time. */
 
 /* Distillation from a teacher's K kept logits per row (ids, top [N, K] contiguous, 1 <= K <= 1024),
- * at temperature T:  p = softmax(top / T) over a row's entries, or with lse [N] (the teacher's
+ * at temperature T (1e-30 to 1e30):  p = softmax(top / T) over a row's entries, or with lse [N] (the teacher's
  * log sum exp(logits / T) over its whole vocabulary) p = exp(top / T - lse) and one bucket for the
  * mass outside the kept labels;  row = weights_row T^2 KL(p || softmax(logits / T)).  An entry listed
  * twice adds its masses.  A row of weight 0, without an entry, or whose logits are all -inf gives
@@ -517,7 +517,7 @@ int sbod_logits_process(const void *logits, int dtype, int64_t n, int64_t v, int
                         const float *bias_values, int bias_cols, int64_t bias_ids_ld, int64_t bias_values_ld,
                         const void *mask, int mask_kind, int64_t mask_ld, void *out, int64_t out_ld, void *stream);
 
-/* out [N, D] = scale table[ids] (an absent id: zeros), and d table [V, D] = scale sum of grad's rows of
+/* out [N, D < 2^23] = scale table[ids] (an absent id: zeros), and d table [V, D] = scale sum of grad's rows of
  * each label, added in 32 bits in ascending position, zeros where none came; `padding` (-1: none) is a
  * label that gets no gradient.  table, out, grad, grad_table are contiguous. */
 int sbod_embed_fwd(const void *table, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,

@@ -1247,6 +1247,10 @@ def label_call(name, t, *args):
     ext = L.host_ext
     if ext is None or L._recorder or not t.is_cuda:
         return None
+    if t.requires_grad and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing() and ext.foreign_leaves(t):
+        # captured, the backward pass would take the other stream into the graph, and the capture's end stops the process
+        raise RuntimeError('%s: a graph from before the capture still holds gradient nodes of these leaves, made on another '
+                           'stream: release its result first' % name)
     r = getattr(ext, name)(*args, L._raw_stream(t.get_device()))
     if type(r) is int:
         raise L.SbodError('%s failed (%d): %s' % (name, r, L.lib().sbod_last_error().decode(errors='replace')))
@@ -1274,8 +1278,8 @@ def distill_arguments(logits, ids, top, lse, weights, temperature, reduction):
     for name, t in (('teacher_lse', lse), ('weights', weights)):
         if t is not None and t.shape != logits.shape[:-1]:
             raise ValueError('%s: %s %s for logits %s' % (what, name, tuple(t.shape), tuple(logits.shape)))
-    if not 0.0 < float(temperature) < float('inf'):
-        raise ValueError('%s: temperature %s' % (what, temperature))
+    if not 1e-30 <= float(temperature) <= 1e30:
+        raise ValueError('%s: temperature %s (1e-30 to 1e30)' % (what, temperature))
     if reduction not in L.REDUCE:
         raise ValueError('%s: reduction %r (mean, sum or none)' % (what, reduction))
     _constant(what, 'teacher_logits', top)
@@ -1370,6 +1374,8 @@ def logits_arguments(logits, history, history_len, prompt_len, repetition, prese
     if history is not None:
         _integral(what, 'history', history)
         rows('history', history)
+        if history.shape[-1] >= 1 << 29:
+            raise ValueError('%s: history %s (fewer than 2^29 entries per row)' % (what, tuple(history.shape)))
     for name, t in (('history_len', history_len), ('prompt_len', prompt_len)):
         if t is None:
             continue
@@ -1395,6 +1401,8 @@ def logits_arguments(logits, history, history_len, prompt_len, repetition, prese
     if bias_ids is not None:
         _integral(what, 'bias_ids', bias_ids)
         rows('bias_ids', bias_ids)
+        if bias_ids.shape[-1] > 4096:
+            raise ValueError('%s: bias_ids %s (at most 4096 per row)' % (what, tuple(bias_ids.shape)))
         if bias_values.dtype != torch.float32:
             raise TypeError('%s: bias_values of %s (float32)' % (what, bias_values.dtype))
         rows('bias_values', bias_values, bias_ids.shape[-1])
@@ -1470,7 +1478,9 @@ def process_logits(logits, history, history_len, prompt_len, repetition, presenc
         return (t.to(torch.float32).contiguous(), 0.0) if torch.is_tensor(t) else (None, float(t))
 
     def lens(t):
-        return None if t is None else t.to(torch.int32).contiguous()
+        if t is not None and t.dtype != torch.int32:
+            t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+        return None if t is None else t.contiguous()
 
     history, ldh = per_row(history)
     bias, ldb = per_row(bias)

@@ -943,7 +943,7 @@ int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, 
                what, static_cast<long long>(n), static_cast<long long>(v), static_cast<long long>(ldx));
   SBOD_REQUIRE(k >= 1 && k <= kMaxTop, "%s: %d kept labels per row (1..%d)", what, k, kMaxTop);
   SBOD_REQUIRE(n < (1ll << 40) / v, "%s: %lld rows of %lld labels", what, static_cast<long long>(n), static_cast<long long>(v));
-  SBOD_REQUIRE(temperature > 0.f && temperature < __builtin_inff(), "%s: temperature %g", what, temperature);
+  SBOD_REQUIRE(temperature >= 1e-30f && temperature <= 1e30f, "%s: temperature %g", what, temperature);   // (1 / T and T^2 / T)
   SBOD_REQUIRE(reduction >= SBOD_REDUCE_NONE && reduction <= SBOD_REDUCE_SUM, "%s: reduction %d", what, reduction);
   SBOD_REQUIRE(n == 0 || (x && ids && top), "%s: null tensor", what);
   return SBOD_OK;

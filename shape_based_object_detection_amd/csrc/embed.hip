@@ -372,7 +372,7 @@ dim3 row_grid(int64_t rows, dim3 block, int64_t tiles = 1) {
 
 int check_embed(const char *what, int dt, int64_t n, int64_t v, int64_t d) {
   SBOD_REQUIRE(known_dt(dt), "%s: dtype %d", what, dt);
-  SBOD_REQUIRE(n >= 0 && n < (1ll << 31) - 65536 && v >= 0 && v < (1ll << 31) - 65536 && d >= 0 && d < (1ll << 31),
+  SBOD_REQUIRE(n >= 0 && n < (1ll << 31) - 65536 && v >= 0 && v < (1ll << 31) - 65536 && d >= 0 && d < (1ll << 23),
                "%s: %lld labels, table [%lld, %lld]", what, static_cast<long long>(n), static_cast<long long>(v),
                static_cast<long long>(d));
   return SBOD_OK;

@@ -8,12 +8,16 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "sbod.h"
 
@@ -58,6 +62,34 @@ inline at::Tensor once(at::Tensor grad) {
   return (*late)({g})[0];
 }
 
+// foreign_leaves(t): whether a leaf below t has a gradient node that was made on another stream than the current one
+// (a graph from before still holds it).  Such a backward pass synchronises the two streams.
+inline PyObject *foreign_leaves_call(PyObject *const *a, Py_ssize_t n) {
+  const at::Tensor *t = n == 1 ? tensor_of(a[0]) : nullptr;
+  if (!t) {
+    PyErr_SetString(PyExc_TypeError, "foreign_leaves: expected a tensor");
+    return nullptr;
+  }
+  const c10::Stream now = c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device());
+  std::shared_ptr<torch::autograd::Node> top = t->grad_fn();
+  if (!top) top = torch::autograd::impl::try_get_grad_accumulator(*t);
+  std::vector<torch::autograd::Node *> todo;
+  std::unordered_set<torch::autograd::Node *> seen;
+  if (top) todo.push_back(top.get());
+  while (!todo.empty()) {
+    torch::autograd::Node *node = todo.back();
+    todo.pop_back();
+    if (!seen.insert(node).second) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad *>(node)) {
+      const auto made = node->stream();
+      if (made && made->device() == now.device() && *made != now) Py_RETURN_TRUE;
+    }
+    for (const auto &e : node->next_edges())
+      if (e.is_valid()) todo.push_back(e.function.get());
+  }
+  Py_RETURN_FALSE;
+}
+
 // ------------------------------------------------------------------------------------------ distillation
 struct DistillCall {
   at::Tensor ids, top, lse, w;
@@ -98,7 +130,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list go) {
-      if (go.empty() || !go[0].defined()) return {at::Tensor(), at::Tensor()};
+    if (go.empty() || !go[0].defined()) return {at::Tensor(), at::Tensor()};
     auto saved = ctx->get_saved_variables();
     auto &sd = ctx->saved_data;
     const at::Tensor &x = saved[0], &ids = saved[1], &top = saved[2], &lse = saved[3], &w = saved[4], &kept = saved[5];
@@ -127,7 +159,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
 };
 
 // label_distill(logits, ids, top, lse | None, weights | None, temperature, reduction, unit_ptr | None, stream)
-inline PyObject *label_distill(PyObject *, PyObject *const *a, Py_ssize_t n) {
+inline PyObject *label_distill_call(PyObject *const *a, Py_ssize_t n) {
   if (n != 9) {
     PyErr_SetString(PyExc_TypeError, "label_distill: expected 9 arguments");
     return nullptr;
@@ -147,21 +179,15 @@ inline PyObject *label_distill(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (!x->is_cuda() || (c.dt = label_dt(*x)) < 0 || (c.top_dt = label_dt(*top)) < 0 || !is_id(*ids) || !good_rows(*x) ||
       x->size(1) < 1 || ids->dim() != 2 || !ids->is_contiguous() || !top->is_contiguous() || ids->sizes() != top->sizes() ||
       ids->size(0) != x->size(0) || ids->size(1) < 1 || ids->size(1) > 1024 || ids->device() != x->device() ||
-      top->device() != x->device() || wants(*top) || !vec(lse) || !vec(w) || !(c.temperature > 0.f) ||
-      !std::isfinite(c.temperature))
+      top->device() != x->device() || wants(*top) || !vec(lse) || !vec(w) ||
+      !(c.temperature >= 1e-30f && c.temperature <= 1e30f))
     Py_RETURN_NONE;
   c.ids = *ids, c.top = top->detach();
   if (lse) c.lse = lse->detach();
   if (w) c.w = w->detach();
   c.want = wants(*x);
-  at::Tensor out;
-  try {
-    const c10::DeviceGuard guard(x->device());
-    out = DistillFn::apply(*x, &c);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::DeviceGuard guard(x->device());
+  at::Tensor out = DistillFn::apply(*x, &c);
   return wrap_status(c.status, std::move(out));
 }
 
@@ -204,7 +230,7 @@ struct EmbedFn : public torch::autograd::Function<EmbedFn> {
 };
 
 // label_embed(ids, weight, scale, padding id | None, stream)
-inline PyObject *label_embed(PyObject *, PyObject *const *a, Py_ssize_t n) {
+inline PyObject *label_embed_call(PyObject *const *a, Py_ssize_t n) {
   if (n != 5) {
     PyErr_SetString(PyExc_TypeError, "label_embed: expected 5 arguments");
     return nullptr;
@@ -222,21 +248,15 @@ inline PyObject *label_embed(PyObject *, PyObject *const *a, Py_ssize_t n) {
       (a[3] != Py_None && (c.pad < 0 || c.pad >= w->size(0))))
     Py_RETURN_NONE;
   c.ids = *ids;
-  at::Tensor out;
-  try {
-    const c10::DeviceGuard guard(w->device());
-    out = EmbedFn::apply(*w, &c);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::DeviceGuard guard(w->device());
+  at::Tensor out = EmbedFn::apply(*w, &c);
   return wrap_status(c.status, std::move(out));
 }
 
 // ------------------------------------------------------------------------------------------ logits
 // label_logits(logits, history | None, history_len | None, prompt_len | None, repetition, presence, frequency,
 //              bias | None, bias_ids | None, bias_values | None, allowed | None, out | None, stream)
-inline PyObject *label_logits(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+inline PyObject *label_logits_call(PyObject *const *a, Py_ssize_t n_args) {
   if (n_args != 13) {
     PyErr_SetString(PyExc_TypeError, "label_logits: expected 13 arguments");
     return nullptr;
@@ -290,36 +310,40 @@ inline PyObject *label_logits(PyObject *, PyObject *const *a, Py_ssize_t n_args)
     kind = mask->scalar_type() == at::kBool ? SBOD_MASK_BYTES : SBOD_MASK_BITS;
     ok = kind == SBOD_MASK_BYTES ? cols(mask) == v : mask->scalar_type() == at::kInt && cols(mask) >= (v + 31) / 32;
   }
-  ok = ok && (!hist || is_id(*hist)) && (!bids == !bval) && (!bids || (is_id(*bids) && bval->scalar_type() == at::kFloat)) &&
+  ok = ok && (!hist || (is_id(*hist) && cols(hist) < (1 << 29))) && cols(bids) <= 4096 && (!bids == !bval) && (!bids || (is_id(*bids) && bval->scalar_type() == at::kFloat)) &&
        (!bias || bias->scalar_type() == at::kFloat || bias->scalar_type() == x->scalar_type()) &&
        (per_row[0] || (scalar[0] > 0.f && std::isfinite(scalar[0]))) && (a[11] == Py_None || a[11] == a[0]);
   if (!ok) Py_RETURN_NONE;
   void *stream = PyLong_AsVoidPtr(a[12]);
   if (PyErr_Occurred()) return nullptr;
-  at::Tensor out;
-  int st;
-  try {
-    const c10::DeviceGuard guard(x->device());
-    const at::NoGradGuard no_grad;
-    out = a[11] == Py_None ? empty_rows(*x) : *x;
-    st = sbod_logits_process(x->data_ptr(), dt, n, v, row_stride(*x), hist ? hist->data_ptr() : nullptr,
-                             hist && hist->scalar_type() == at::kLong, cols(hist), ld(hist),
-                             hlen ? hlen->data_ptr<int32_t>() : nullptr, plen ? plen->data_ptr<int32_t>() : nullptr, per_row[0],
-                             per_row[1], per_row[2], scalar[0], scalar[1], scalar[2], bias ? bias->data_ptr() : nullptr,
-                             bias ? label_dt(*bias) : 0, ld(bias), bids ? bids->data_ptr() : nullptr,
-                             bids && bids->scalar_type() == at::kLong, bval ? bval->data_ptr<float>() : nullptr,
-                             static_cast<int>(cols(bids)), ld(bids), ld(bval), mask ? mask->data_ptr() : nullptr, kind, ld(mask),
-                             out.data_ptr(), row_stride(out), stream);
-  } catch (const std::exception &e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  const c10::DeviceGuard guard(x->device());
+  const at::NoGradGuard no_grad;
+  at::Tensor out = a[11] == Py_None ? empty_rows(*x) : *x;
+  const int st = sbod_logits_process(x->data_ptr(), dt, n, v, row_stride(*x), hist ? hist->data_ptr() : nullptr,
+                                     hist && hist->scalar_type() == at::kLong, cols(hist), ld(hist),
+                                     hlen ? hlen->data_ptr<int32_t>() : nullptr, plen ? plen->data_ptr<int32_t>() : nullptr, per_row[0],
+                                     per_row[1], per_row[2], scalar[0], scalar[1], scalar[2], bias ? bias->data_ptr() : nullptr,
+                                     bias ? label_dt(*bias) : 0, ld(bias), bids ? bids->data_ptr() : nullptr,
+                                     bids && bids->scalar_type() == at::kLong, bval ? bval->data_ptr<float>() : nullptr,
+                                     static_cast<int>(cols(bids)), ld(bids), ld(bval), mask ? mask->data_ptr() : nullptr, kind, ld(mask),
+                                     out.data_ptr(), row_stride(out), stream);
   if (st == SBOD_OK && a[11] == a[0]) {   // in place: the caller's own object, and its version counted
     x->unsafeGetTensorImpl()->bump_version();
     Py_INCREF(a[0]);
     return a[0];
   }
   return wrap_status(st, std::move(out));
+}
+
+// Nothing that ATen throws passes the interpreter.
+template <PyObject *(*kCall)(PyObject *const *, Py_ssize_t)>
+PyObject *guarded(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  try {
+    return kCall(a, n);
+  } catch (const std::exception &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
 }
 
 }  // namespace sbod_label

@@ -569,12 +569,14 @@ PyObject *criterion_focal_fast(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {
-    {"label_distill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::label_distill)),
+    {"label_distill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::guarded<sbod_label::label_distill_call>)),
      METH_FASTCALL, "operators.Loss.topk_distill_loss on device tensors (host_label.h)."},
-    {"label_embed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::label_embed)),
+    {"label_embed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::guarded<sbod_label::label_embed_call>)),
      METH_FASTCALL, "operators.Embedding.scaled_embedding on device tensors (host_label.h)."},
-    {"label_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::label_logits)),
+    {"label_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::guarded<sbod_label::label_logits_call>)),
      METH_FASTCALL, "operators.Logits.process_logits on device tensors (host_label.h)."},
+    {"foreign_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sbod_label::guarded<sbod_label::foreign_leaves_call>)),
+     METH_FASTCALL, "Whether a leaf below a tensor holds a gradient node of another stream (host_label.h)."},
     {"criterion_focal_fast",
      reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(criterion_focal_fast)),
      METH_FASTCALL, "GT packing + sbod_criterion_focal + a C++ autograd node for the loss."},

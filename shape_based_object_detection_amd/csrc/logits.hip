@@ -294,7 +294,8 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
                static_cast<long long>(v), static_cast<long long>(ld), static_cast<long long>(out_ld));
   SBOD_REQUIRE(history_cols >= 0 && history_cols <= kCount && bias_cols >= 0 && bias_cols <= kMaxBiases && history_ld >= 0 && bias_ld >= 0 &&
                    bias_ids_ld >= 0 && bias_values_ld >= 0 && mask_ld >= 0,
-               "sbod_logits_process: negative size or stride");
+               "sbod_logits_process: %lld history entries, %d listed biases (0 .. %u, 0 .. %d), or a negative stride",
+               static_cast<long long>(history_cols), bias_cols, kCount, kMaxBiases);
   SBOD_REQUIRE(mask_kind == SBOD_MASK_NONE || ((mask_kind == SBOD_MASK_BITS || mask_kind == SBOD_MASK_BYTES) && mask),
                "sbod_logits_process: mask kind %d", mask_kind);
   SBOD_REQUIRE((history_cols == 0 || history) && (bias_cols == 0 || (bias_ids && bias_values)),

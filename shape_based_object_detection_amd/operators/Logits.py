@@ -18,12 +18,12 @@ def process_logits(logits, history=None, history_len=None, prompt_len=None, repe
     * a label of the row's history: ``x / repetition`` where x > 0, else ``x * repetition``;
     * ``- frequency * count - presence * (count > 0)``, count over the answered part of the history;
     * ``+ bias`` ([V] or [N, V], float32 or the logits' type), ``+ bias_values`` (float32) at ``bias_ids``
-      ([M] or [N, M]; a label listed twice adds both);
+      ([M] or [N, M], M <= 4096; a label listed twice adds both);
     * ``-inf`` where ``allowed`` forbids the label: truth values [V] or [N, V], or int32 words [W] or [N, W]
       with label v in bit ``v % 32`` of word ``v // 32``.  A forbidden label is -inf whatever it was before;
       a row that allows nothing is all -inf.
 
-    ``history`` [N, L] (or [L]: the same for every row) int32 / int64: its first ``history_len`` [N] entries count
+    ``history`` [N, L] (or [L]: the same for every row; L < 2^29) int32 / int64: its first ``history_len`` [N] entries count
     (default: all), the first ``prompt_len`` [N] of them were given (repetition only), the others answered.
     ``repetition`` (> 0), ``presence``, ``frequency``: numbers, or float tensors [N].  An id outside [0, V) is
     absent (padding).  Not differentiable: logits that require a gradient are refused while gradients are on.

@@ -419,6 +419,33 @@ def test_captured_steps_equal_eager(dt):
             assert torch.equal(a, b)
 
 
+def test_capture_is_refused_while_an_eager_graph_holds_the_leaves():
+    """(Its captured backward pass would join the eager graph's stream; only forward calls are made here.)"""
+    x, tid, top, _ = dev(*C.distill_inputs(6, 40, 3, torch.float32, 2, True))
+    table = torch.randn(9, 40, device=DEV).requires_grad_(True)
+    leaf = x.clone().requires_grad_(True)
+    ids = torch.arange(6, device=DEV)
+    calls = {'embed': lambda: scaled_embedding(ids, table, 2.0), 'leaf': lambda: topk_distill_loss(leaf, tid, top),
+             'network': lambda: topk_distill_loss(table[:6] * 2.0, tid, top)}
+    s = torch.cuda.Stream()
+    for name, call in calls.items():
+        held = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            with pytest.raises(RuntimeError, match='release its result first'):
+                call()
+            with torch.no_grad():
+                again = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, held.detach()), name
+        del held
+        gc.collect()
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+            call()
+
+
 def test_other_streams():
     """Calls on several streams at once hold their own scratch memory."""
     sets = [dev(*C.distill_inputs(64, 30011, 16, torch.bfloat16, i, True)) for i in range(4)]

@@ -99,6 +99,7 @@ X, IDS, TOP = torch.zeros(2, 5), torch.zeros(2, 3, dtype=torch.int64), torch.zer
     ((X, IDS, TOP, None, torch.zeros(2, 1)), ValueError),
     ((X, IDS, TOP, None, None, 0.0), ValueError),
     ((X, IDS, TOP, None, None, math.inf), ValueError),
+    ((X, IDS, TOP, None, None, 1e-38), ValueError),
     ((X, IDS, TOP, None, None, 1.0, 'batchmean'), ValueError),
     ((X, IDS, TOP.clone().requires_grad_(True)), ValueError),
     ((X, IDS, TOP, None, torch.ones(2, requires_grad=True)), ValueError),
@@ -129,6 +130,8 @@ H = torch.zeros(2, 4, dtype=torch.int64)
     (dict(bias=torch.zeros(4)), ValueError),
     (dict(bias_ids=H), ValueError),
     (dict(bias_ids=H, bias_values=torch.zeros(2, 3)), ValueError),
+    (dict(bias_ids=torch.zeros(4097, dtype=torch.int64), bias_values=torch.zeros(4097)), ValueError),
+    (dict(history=torch.zeros(1, dtype=torch.int64).expand(1 << 29)), ValueError),
     (dict(bias_ids=H, bias_values=torch.zeros(2, 4, dtype=torch.float16)), TypeError),
     (dict(allowed=torch.ones(2, 4, dtype=torch.bool)), ValueError),
     (dict(allowed=torch.ones(2, 0, dtype=torch.int32)), ValueError),
@@ -160,7 +163,7 @@ def test_entry_points_refuse_before_any_launch():
     def distill(dt=0, n=2, v=5, ld=5, k=3, T=1.0, red=1, ws=1 << 20):
         return L.call('sbod_distill_fwd', 8, dt, n, v, ld, 8, 1, 8, 0, k, None, None, T, red, 8, 8, 8, 8, None, 0, 8, ws, None)
 
-    for kw in (dict(dt=3), dict(n=-1), dict(v=0), dict(ld=4), dict(k=0), dict(k=1025), dict(T=0.0), dict(T=math.inf),
+    for kw in (dict(dt=3), dict(n=-1), dict(v=0), dict(ld=4), dict(k=0), dict(k=1025), dict(T=0.0), dict(T=math.inf), dict(T=1e-38),
                dict(red=3), dict(ws=0), dict(v=1 << 31, ld=1 << 31)):
         with pytest.raises(L.SbodError, match='sbod_distill_fwd'):
             distill(**kw)
@@ -175,6 +178,7 @@ def test_entry_points_refuse_before_any_launch():
             logits(**kw)
     for name, args in (('sbod_embed_fwd', (8, 3, 5, 4, 8, 1, 2, 1.0, 8, None)), ('sbod_embed_fwd', (8, 0, 0, 4, 8, 1, 2, 1.0, 8, None)),
                        ('sbod_embed_fwd', (8, 0, 5, 4, 8, 1, -2, 1.0, 8, None)),
+                       ('sbod_embed_fwd', (8, 0, 5, 1 << 23, 8, 1, 2, 1.0, 8, None)),
                        ('sbod_embed_bwd', (8, 0, 5, 4, 8, 1, 2, -1, 1.0, 8, 8, 1, None)),
                        ('sbod_embed_bwd', (8, 0, 5, 4, 8, 1, 2, -1, 1.0, None, 8, 1 << 20, None))):
         with pytest.raises(L.SbodError, match=name):
