@@ -156,28 +156,40 @@ __device__ __forceinline__ bool teacher_norm(const DistillArgs &a, int64_t r, in
   return !(sum == 0.f);
 }
 
+// A value that all lanes hold, in a scalar register.
+__device__ __forceinline__ float uniform(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+__device__ __forceinline__ double uniform(double v) {
+  return __hiloint2double(__builtin_amdgcn_readfirstlane(__double2hiint(v)), __builtin_amdgcn_readfirstlane(__double2loint(v)));
+}
+
 // The bucket of a row: the teacher's mass outside the kept labels, 1 - mass, against the student's, q_o.
 // term: its part of the KL; coef: q_o - rest.  Both sides are near 1 where the kept labels hold little, so
 // their logarithms and their difference are then taken from what the kept labels hold (P - Q = q_o - rest);
 // `mass` comes in 64 bits, for where they hold nearly all.  others: there is a label that is not kept (else
-// what is left of the teacher's mass is rounding).
+// what is left of the teacher's mass is rounding).  kOne: all lanes of a wave have one row (its values pass
+// through scalar registers: k_distill_row's are full of the row).
 struct Bucket {
   double term;
   float coef;
 };
+template <bool kOne>
 __device__ __forceinline__ Bucket bucket_of(const DistillArgs &a, double mass, float kept, float sum, float so, float mo,
                                             float base, bool others) {
+  const auto one = [](auto v) { return kOne ? uniform(v) : v; };
+  mass = one(mass);
   double rest = 1.0 - mass;
   if (rest < 0 || !others) rest = 0;
-  const float q = kept / sum;
+  const float q = one(kept / sum);
   const bool little = q < 0.5f;
-  const double logr = mass < 0.5 ? log1pf(static_cast<float>(-mass)) : logf(static_cast<float>(rest));
+  const float logr = one(mass < 0.5 ? log1pf(static_cast<float>(-mass)) : logf(static_cast<float>(rest)));
   const double logo = so == 0.f ? kNegInf
-                      : little  ? log1pf(-q)
-                                : (static_cast<double>(mo) - base) * a.inv_td + logf(so) - logf(sum);
+                      : little  ? one(log1pf(-q))
+                                : (static_cast<double>(mo) - base) * a.inv_td + one(logf(so)) - one(logf(sum));
   Bucket b;
   b.term = rest > 0 ? rest * (logr - logo) : rest;
-  b.coef = little && mass < 1 && others ? static_cast<float>(mass - q) : static_cast<float>(expf(static_cast<float>(logo)) - rest);
+  b.coef = little && mass < 1 && others ? static_cast<float>(mass - q) : static_cast<float>(one(expf(static_cast<float>(logo))) - rest);
   return b;
 }
 
@@ -256,7 +268,7 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
     kl = wave_sum_f64(kl);
     float coef = 1.f;
     if (kBucket) {
-      const Bucket b = bucket_of(a, wave_sum_f64(mass), ksum, sum, so, mo, m, kept < a.v);
+      const Bucket b = bucket_of<true>(a, wave_sum_f64(mass), ksum, sum, so, mo, m, kept < a.v);
       kl += b.term;
       coef = b.coef;
     }
@@ -537,7 +549,7 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     double kl = has0 ? term(p0, logp0, x0) : 0.0;
     more([&](int, int, float t, float x) { kl += term(p_at(logp_at(t)), logp_at(t), x); });
     if (kBucket) {
-      const Bucket b = bucket_of(a, mass, ksum, sum, so, mo, base, others);
+      const Bucket b = bucket_of<G == kWave>(a, mass, ksum, sum, so, mo, base, others);
       if (lane == 0) kl += b.term;
       coef = so == 0.f ? 0.f : b.coef / so;
     }
@@ -614,6 +626,8 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     const int in = (v - head) / P, tail = v - head - in * P;
     return tid < head ? tid : tid >= P && tid < P + tail ? head + in * P + tid - P : -1;
   };
+  // its byte in `bits`, of the first granule, and where in that
+  const int look = P == 8 ? tid + 1 : (tid + 1) >> 1, shift = 4 * ((tid + 1) & 1);
   // (a granule's address is a scalar base and the thread's own offset, the same for all of them)
   const uint32_t mine = static_cast<uint32_t>(tid) * 16;
   const auto base_of = [&](const T *row, int head) { return reinterpret_cast<const char *>(row + head); };
@@ -621,8 +635,12 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     at += NT * 16;
     asm volatile("" : "+s"(at));
   };
-  const auto fetch = [&](int i, const char *at, int granules) {
-    if (i * NT + tid < granules) raw[i] = *reinterpret_cast<const raw16_t *>(at + mine);
+  const auto fetch = [&](int i, const char *at, int left) {
+    if (tid < left) raw[i] = *reinterpret_cast<const raw16_t *>(at + mine);
+  };
+  const auto fewer = [&](int &left) {   // (as step_on: no vector register per granule)
+    left -= NT;
+    asm volatile("" : "+s"(left));
   };
   // The registers hold the row as it was read, a granule's work at a time.  Without this the compiler widens
   // each element once and keeps twice the registers from pass to pass.
@@ -645,7 +663,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     const int head = head_of(row);
     const char *at = base_of(row, head);
 #pragma unroll
-    for (int i = 0; i < NG; ++i, step_on(at)) fetch(i, at, (v - head) / P);
+    for (int i = 0, left = (v - head) / P; i < NG; ++i, step_on(at), fewer(left)) fetch(i, at, left);
     fetch_rest(r, row, head);
   }
   for (; r < a.n; r += gridDim.x) {
@@ -674,19 +692,17 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       float x1 = e1 >= 0 ? bits_value<DT>(xraw) : kNegInf;
       if (kBucket && e1 >= 0 && bits[(e1 - head + P) >> 5] >> ((e1 - head + P) & 31) & 1) x1 = kNegInf;
       mo = x1;
+      int left = inner;
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int g = i * NT + tid;
+      for (int i = 0; i < NG; ++i, fewer(left)) {
         as_read(i);
         // (by masks: a branch would hold the row twice where it joins)
         uint32_t b = 0;
         if (kBucket) {
-          int at = P == 8 ? g + 1 : (g + 1) >> 1;
-          asm volatile("" : "+v"(at));   // (looked up here, not ahead for all granules)
-          const uint32_t byte = reinterpret_cast<const uint8_t *>(bits)[at];
-          b = P == 8 ? byte : byte >> (4 * ((g + 1) & 1)) & 15;
+          const uint32_t byte = reinterpret_cast<const uint8_t *>(bits)[look + i * (NT * P / 8)];
+          b = P == 8 ? byte : byte >> shift & 15;
         }
-        b = g >= inner ? ~0u : b;
+        b = tid >= left ? ~0u : b;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const auto bit = [&](int k) { return static_cast<uint32_t>(static_cast<int32_t>(b << (31 - k)) >> 31); };
@@ -705,11 +721,11 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       other = wave_max_f32(other);
       if ((tid & 63) == 0) red[0][wave] = mo, red[1][wave] = other;
       __syncthreads();
-      mo = group_max<NW>(red[0][tid % NW]), other = group_max<NW>(red[1][tid % NW]);
+      mo = uniform(group_max<NW>(red[0][tid % NW])), other = uniform(group_max<NW>(red[1][tid % NW]));
       if (kBucket && id >= 0) bits[place >> 5] = 0;   // (read for the last time above)
-      obase = mo == kNegInf ? 0.f : mo;
+      obase = uniform(mo == kNegInf ? 0.f : mo);
       const float m = kBucket ? fmaxf(mo, other) : mo;
-      base = m == kNegInf ? 0.f : m;
+      base = uniform(m == kNegInf ? 0.f : m);
       const float tb = kBucket || other == kNegInf ? 0.f : other;
       float tl = kBucket ? a.lse[r] : 0.f;
       const auto logp_at = [&](float q) { return static_cast<float>((static_cast<double>(q) - tb) * a.inv_td - tl); };
@@ -741,7 +757,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       if (kBucket) s2 = group_sum<kWave>(s2);
       if ((tid & 63) == 0) sums[0][wave] = so, sums[1][wave] = s1, masses[wave] = s2;
       __syncthreads();
-      so = group_sum<NW>(sums[0][tid % NW]), s1 = group_sum<NW>(sums[1][tid % NW]);
+      so = uniform(group_sum<NW>(sums[0][tid % NW])), s1 = uniform(group_sum<NW>(sums[1][tid % NW]));
       if (kBucket) s2 = group_sum<NW>(masses[tid % NW]);
       const float sum = kBucket ? s1 + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s)) : so;
       // a row of -inf alone has no distribution, a teacher without mass nothing to say: left out, as of weight 0
@@ -751,14 +767,14 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
         tl = log_hw(s1);
         pk = id >= 0 ? p_at(logp_at(t)) : 0.f;
       }
-      inv = 1.f / sum;
+      inv = uniform(1.f / sum);
       coef = inv;
       // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
       double kl = pk == 0.f ? 0.0 : pk * (logp_at(t) - ((static_cast<double>(xk) - base) * a.inv_td - logs));
       if (kBucket) {
-        const Bucket b = bucket_of(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
+        const Bucket b = bucket_of<true>(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
         if (tid == 0) kl += b.term;
-        coef = so == 0.f ? 0.f : b.coef / so;
+        coef = uniform(so == 0.f ? 0.f : b.coef / so);
       }
       if (again) {
         pk = 0.f;
@@ -776,12 +792,13 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     }
     float g = a.t * w * norm * up;
     if (a.up && a.up_stride) g *= a.up[r];
-    const float gc = g * coef;
+    const float gc = uniform(g * coef);
     if (a.dx && e1 >= 0) drow[e1] = static_cast<T>(live && !(kBucket && so == 0.f) ? gc * exp2_hw((bits_value<DT>(xraw) - obase) * a.s) : 0.f);
     const char *from = base_of(next, nhead), *to = base_of(drow, head);
+    int left = inner, nleft = ninner;
 #pragma unroll
-    for (int i = 0; i < NG; ++i, step_on(from), step_on(to)) {
-      if (a.dx && i * NT + tid < inner) {
+    for (int i = 0; i < NG; ++i, step_on(from), step_on(to), fewer(left), fewer(nleft)) {
+      if (a.dx && tid < left) {
         float f[P];
         as_read(i);
         raw_values<DT>(raw[i], f);
@@ -798,7 +815,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
           for (int j = 0; j < P; ++j) at[j] = static_cast<T>(f[j]);
         }
       }
-      fetch(i, from, ninner);
+      fetch(i, from, nleft);
     }
     __syncthreads();
     // the kept labels, over what the row's pass wrote there
@@ -878,10 +895,10 @@ int launch_small(const DistillArgs &a, hipStream_t s) {
 struct RowShape {
   int nt, ng, groups;
 };
-constexpr RowShape kRowShapes[] = {{256, 4, 1280}, {256, 8, 1024}, {256, 16, 1024}, {512, 16, 512}, {1024, 16, 256}};
+constexpr RowShape kRowShapes[] = {{256, 4, 1280}, {256, 8, 1024}, {256, 16, 1024}, {512, 16, 512}, {1024, 15, 256}, {1024, 16, 256}};
 int row_shape(int64_t v, int k, int dt, bool bucket) {
   const int64_t granules = v / static_cast<int64_t>(16 / elt_bytes(dt));
-  for (int i = 0; i < (bucket ? 4 : 5); ++i)
+  for (int i = 0; i < (bucket ? 5 : 6); ++i)
     if (kRowShapes[i].nt >= k && static_cast<int64_t>(kRowShapes[i].nt) * kRowShapes[i].ng >= granules) return i;
   return -1;
 }
@@ -902,7 +919,8 @@ int launch_row(const DistillArgs &a, hipStream_t s) {
   else if (shape == 1) SBOD_ROW(1);
   else if (shape == 2) SBOD_ROW(2);
   else if (shape == 3) SBOD_ROW(3);
-  else if constexpr (!kBucket) SBOD_ROW(4);
+  else if (shape == 4) SBOD_ROW(4);
+  else if constexpr (!kBucket) SBOD_ROW(5);
 #undef SBOD_ROW
   SBOD_LAUNCHED("k_distill_row");
   return SBOD_OK;

@@ -35,7 +35,8 @@ def run_distill(x, ids, top, lse, w=None, T=1.0, reduction='mean', upstream=None
 @pytest.mark.parametrize('n,v,k', [(1, 1, 1), (1, 2, 1), (3, 7, 7), (65, 21, 5), (257, 33, 8), (5, 64, 64), (9, 91, 1),
                                    (4, 255, 16), (6, 513, 100), (3, 1203, 16), (2, 1024, 1024), (3, 2048, 33),
                                    (2, 2049, 20), (3, 8191, 64), (2, 8193, 64), (2, 16385, 1000), (1, 40000, 3),
-                                   (2, 50001, 100), (1, 131072, 64), (1, 200003, 50)])
+                                   (2, 50001, 100), (1, 131072, 64), (1, 200003, 50), (300, 40003, 30), (258, 61433, 7),
+                                   (2, 100003, 60), (261, 70001, 1024)])
 def test_distill_sizes(dt, tail, n, v, k):
     x, ids, top, lse = dev(*C.distill_inputs(n, v, k, dt, 7 * n + v + k, tail, wide=v % 2 == 0))
     loss, grad = run_distill(x, ids, top, lse, T=1.5)
