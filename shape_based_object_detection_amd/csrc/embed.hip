@@ -37,7 +37,8 @@ __host__ __device__ inline int flag_shift(int64_t per) {
 // where each label's begin (an absent id has no place).  Every workgroup reads all ids (they stay in its
 // XCD's L2), counts its own labels and those below its range, and flags the stretches that hold one of
 // its own: only those are read again, to place.  A wave owns a run of positions and a row of counters, so
-// its placing needs no other wave: the order is that of the positions.
+// its placing needs no other wave: the order is that of the positions.  Bound by the latency of its passes: 54 us
+// for 65,536 ids of 131,072 labels, 10 for 6,400 of 21.
 template <typename ID>
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID *__restrict__ ids, int64_t n, int64_t v, int range,
                                                              int32_t *__restrict__ begin, int32_t *__restrict__ sorted) {
@@ -173,7 +174,8 @@ __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID *__restric
   }
 }
 
-// out[i] = scale table[id_i].  A block is rows x column groups of kV elements.
+// out[i] = scale table[id_i].  A block is rows x column groups of kV elements.  Bound by memory: 143 us for 65,536
+// rows of 4,096 bfloat16 elements (537 MB written and the rows read: 5.2 TB/s), 3 us for 32 of them.
 template <int DT, int kV>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const void *table, const void *ids, int ids64, int64_t n,
                                                             int64_t v, int64_t groups, float scale, void *out) {
@@ -240,7 +242,8 @@ __device__ __forceinline__ void add_rows(float (&acc)[kV], const T *grad, const 
 }
 
 // Sums of the positions [c rows, (c + 1) rows) for the labels that came more than `rows` times: such a
-// run covers the chunk's first position (pieces[c][0]) or, begun inside, its last one (pieces[c][1]).
+// run covers the chunk's first position (pieces[c][0]) or, begun inside, its last one (pieces[c][1]).  Bound by
+// its reads: 76 us where 65,536 positions follow their labels' frequencies (1 / rank), 4,096 columns.
 template <int DT, int kV>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_pieces(const void *grad, const void *ids, int ids64,
                                                               const int32_t *begin, const int32_t *sorted, int64_t v,
@@ -277,8 +280,8 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_pieces(const void *grad, 
 
 // d table[v] from the sorted positions.  The same blocks over the table's rows, kEmbRows of them per thread:
 // most labels came once or not at all, so a row is a chain of three loads (its places, their first row's
-// number, that row), and the rows' chains run side by side: 395 us with 4, 453 with 1 for 65,536 positions
-// into a table of 1 GB.
+// number, that row), and the rows' chains run side by side: 305 us for 65,536 positions into
+// a table of 1 GB (before its stores went past the caches 395 with 4 rows, 453 with 1).
 template <int DT, int kV, int kEmbRows>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, const int32_t *begin,
                                                             const int32_t *sorted, int64_t v, int64_t padding, int rows,
@@ -336,7 +339,7 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, co
       V o;
 #pragma unroll
       for (int j = 0; j < kV; ++j) o[j] = static_cast<T>(acc[j] * scale);
-      // (written once and not read here: past the caches, 505 against 535 us for a table of 1 GB)
+      // (written once and not read here: past the caches: the backward pass of a 1 GB table 505 against 535 us)
       __builtin_nontemporal_store(o, reinterpret_cast<V *>(static_cast<T *>(dtable) + r * d) + g);
     }
   }
