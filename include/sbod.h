@@ -489,7 +489,7 @@ int sbod_map_f32(const float *det_boxes, const int64_t *det_labels, const float 
  * *upstream is 1 (grad then holds what fwd wrote). */
 enum { SBOD_REDUCE_NONE = 0, SBOD_REDUCE_MEAN = 1, SBOD_REDUCE_SUM = 2 };
 int sbod_distill_stat_floats(void);
-size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int has_lse, int dtype);
+size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int dtype);
 int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids, int ids64,
                      const void *top, int top_dtype, int k, const float *lse, const float *weights,
                      float temperature, int reduction, float *rows, float *loss, float *norm, float *stats,

@@ -1298,7 +1298,7 @@ class _TopKDistill(torch.autograd.Function):
         dev = x.device
         dt, red = L.LABEL_DT[x.dtype], L.REDUCE[reduction]
         nst = L.lib().sbod_distill_stat_floats()
-        nb = L.lib().sbod_distill_workspace_bytes(n, v, top.shape[1], int(lse is not None), dt)
+        nb = L.lib().sbod_distill_workspace_bytes(n, v, top.shape[1], dt)
         kept = torch.empty(nst * n + 1, dtype=torch.float32, device=dev)   # statistics | the reduction's norm
         loss = torch.empty((), dtype=torch.float32, device=dev) if red else None
         rows = None if red else torch.empty(n, dtype=torch.float32, device=dev)

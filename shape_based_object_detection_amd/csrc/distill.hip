@@ -617,7 +617,9 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   __shared__ uint32_t bits[kBucket ? NT * NG * P / 32 + 1 : 1];
   __shared__ int ids_s[NT];
   __shared__ float top_s[NT], red[2][NW], sums[2][NW];
-  __shared__ double red64[16], masses[NW];
+  // (1,024 threads have no register to spare beside 16 granules: each one's loss waits in LDS, and its t is read again)
+  constexpr bool kTight = NT == 1024;
+  __shared__ double red64[16], masses[NW], losses[kTight ? NT : 1];
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int tid = threadIdx.x, wave = tid >> 6, v = static_cast<int>(a.v), kk = a.k;
   if (kBucket)
@@ -625,6 +627,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
   const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
   double loss = 0;
+  if (kTight) losses[threadIdx.x] = 0;
   const bool entry = tid < kk;
   raw16_t raw[NG];
   uint32_t xraw = 0;
@@ -780,19 +783,20 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       inv = uniform(1.f / sum);
       coef = inv;
       // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
-      double kl = pk == 0.f ? 0.0 : pk * (logp_at(t) - ((static_cast<double>(xk) - base) * a.inv_td - logs));
-      if (kBucket) {
-        const Bucket b = bucket_of<true>(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
-        if (tid == 0) kl += b.term;
-        coef = uniform(so == 0.f ? 0.f : b.coef / so);
-      }
+      double kl = pk == 0.f ? 0.0 : pk * (logp_at(kTight ? top_s[tid] : t) - ((static_cast<double>(xk) - base) * a.inv_td - logs));
       if (again) {
         pk = 0.f;
         for (int j = 0; j < kk; ++j)
           if (ids_s[j] == id) pk += p_at(logp_at(top_s[j]));
       }
+      if (kBucket) {
+        const Bucket b = bucket_of<true>(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
+        if (tid == 0) kl += b.term;
+        coef = uniform(so == 0.f ? 0.f : b.coef / so);
+      }
       kl = live ? kl * a.tt * w : 0.0;
-      loss += kl;
+      if (kTight) losses[tid] += kl;
+      else loss += kl;
       if (a.rows) {
         kl = block_sum(kl, red64);
         if (tid == 0) a.rows[r] = static_cast<float>(kl);
@@ -833,7 +837,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     if (ahead) fetch_rest(rn, next, nhead);
   }
   if (a.parts) {
-    loss = block_sum(loss, red64);
+    loss = block_sum(kTight ? losses[tid] : loss, red64);
     if (tid == 0) a.parts[blockIdx.x] = loss;
   }
 }
@@ -900,37 +904,35 @@ int launch_small(const DistillArgs &a, hipStream_t s) {
 }
 
 // Threads and granules of k_distill_row for a row, smallest first, and the workgroups that the device holds at
-// once.  With a bucket the longest rows' lookups do not fit the registers beside them (-1: k_distill_part and
-// the kernels behind it).
+// once.  -1: none, k_distill_part and the kernels behind it.
 struct RowShape {
   int nt, ng, groups;
 };
-constexpr RowShape kRowShapes[] = {{256, 4, 1280}, {256, 8, 1024}, {256, 16, 1024}, {512, 16, 512}, {1024, 15, 256}, {1024, 16, 256}};
-int row_shape(int64_t v, int k, int dt, bool bucket) {
+constexpr RowShape kRowShapes[] = {{256, 4, 1280}, {256, 8, 1024}, {256, 16, 1024}, {512, 16, 512}, {1024, 16, 256}};
+int row_shape(int64_t v, int k, int dt) {
   const int64_t granules = v / static_cast<int64_t>(16 / elt_bytes(dt));
-  for (int i = 0; i < (bucket ? 5 : 6); ++i)
+  for (int i = 0; i < 5; ++i)
     if (kRowShapes[i].nt >= k && static_cast<int64_t>(kRowShapes[i].nt) * kRowShapes[i].ng >= granules) return i;
   return -1;
 }
 
 // Which kernels take a call.
 enum Path { kSmall, kRow, kChunks };
-Path path_of(int64_t v, int k, int dt, bool bucket) {
-  return v <= kSmallMax ? kSmall : row_shape(v, k, dt, bucket) >= 0 ? kRow : kChunks;
+Path path_of(int64_t v, int k, int dt) {
+  return v <= kSmallMax ? kSmall : row_shape(v, k, dt) >= 0 ? kRow : kChunks;
 }
 int64_t row_blocks(int64_t n, int shape) { return n < kRowShapes[shape].groups ? n : kRowShapes[shape].groups; }
 
 template <int DT, bool kBucket>
 int launch_row(const DistillArgs &a, hipStream_t s) {
-  const int shape = row_shape(a.v, a.k, DT, kBucket);
+  const int shape = row_shape(a.v, a.k, DT);
   const dim3 grid(static_cast<unsigned>(row_blocks(a.n, shape))), block(kRowShapes[shape].nt);
 #define SBOD_ROW(I) hipLaunchKernelGGL((k_distill_row<DT, kBucket, kRowShapes[I].nt, kRowShapes[I].ng>), grid, block, 0, s, a)
   if (shape == 0) SBOD_ROW(0);
   else if (shape == 1) SBOD_ROW(1);
   else if (shape == 2) SBOD_ROW(2);
   else if (shape == 3) SBOD_ROW(3);
-  else if (shape == 4) SBOD_ROW(4);
-  else if constexpr (!kBucket) SBOD_ROW(5);
+  else SBOD_ROW(4);
 #undef SBOD_ROW
   SBOD_LAUNCHED("k_distill_row");
   return SBOD_OK;
@@ -939,7 +941,7 @@ int launch_row(const DistillArgs &a, hipStream_t s) {
 // The forward's, or with a.up the gradient's, launches of one type.
 template <int DT, bool kBucket>
 int launch_typed(const DistillArgs &a, hipStream_t s) {
-  const Path p = path_of(a.v, a.k, DT, kBucket);
+  const Path p = path_of(a.v, a.k, DT);
   if (p == kSmall) return launch_small<DT, kBucket>(a, s);
   if (p == kRow) return launch_row<DT, kBucket>(a, s);
   if (!a.up) {
@@ -956,12 +958,12 @@ int launch_any(const DistillArgs &a, int dt, hipStream_t s) {
 
 // The forward's workspace: partial weight sums | loss parts | chunk statistics.
 size_t parts_offset() { return kWeightParts * sizeof(double); }
-int64_t parts_count(int64_t n, int64_t v, int k, int dt, bool bucket) {
-  const Path p = path_of(v, k, dt, bucket);
-  return p == kSmall ? small_blocks(n, small_lanes(v, k)) : p == kRow ? row_blocks(n, row_shape(v, k, dt, bucket)) : n;
+int64_t parts_count(int64_t n, int64_t v, int k, int dt) {
+  const Path p = path_of(v, k, dt);
+  return p == kSmall ? small_blocks(n, small_lanes(v, k)) : p == kRow ? row_blocks(n, row_shape(v, k, dt)) : n;
 }
-size_t chunks_offset(int64_t n, int64_t v, int k, int dt, bool bucket) {
-  return align_up(parts_offset() + parts_count(n, v, k, dt, bucket) * sizeof(double));
+size_t chunks_offset(int64_t n, int64_t v, int k, int dt) {
+  return align_up(parts_offset() + parts_count(n, v, k, dt) * sizeof(double));
 }
 
 int check_common(const char *what, const void *x, int dt, int64_t n, int64_t v, int64_t ldx, const void *ids,
@@ -993,10 +995,10 @@ using namespace sbod::label;
 
 extern "C" int sbod_distill_stat_floats(void) { return kStats; }
 
-extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int has_lse, int dtype) {
+extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int dtype) {
   if (n < 0 || v <= 0 || k <= 0 || k > kMaxTop || !known_dt(dtype)) return 0;
-  const size_t chunks = path_of(v, k, dtype, has_lse) == kChunks ? static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2) : 0;
-  return chunks_offset(n, v, k, dtype, has_lse) + chunks;
+  const size_t chunks = path_of(v, k, dtype) == kChunks ? static_cast<size_t>(n) * distill_chunks(v, dtype) * sizeof(float2) : 0;
+  return chunks_offset(n, v, k, dtype) + chunks;
 }
 
 extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -1010,8 +1012,8 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || (loss && norm), "sbod_distill_fwd: a reduction needs loss and norm");
   SBOD_REQUIRE(!grad || (grad_ld >= v && reduction != SBOD_REDUCE_NONE), "sbod_distill_fwd: gradient with row stride %lld, reduction %d",
                static_cast<long long>(grad_ld), reduction);
-  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, k, lse != nullptr, dtype) || !workspace) {
-    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, k, lse != nullptr, dtype));
+  if (workspace_bytes < sbod_distill_workspace_bytes(n, v, k, dtype) || !workspace) {
+    set_error("sbod_distill_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, sbod_distill_workspace_bytes(n, v, k, dtype));
     return SBOD_E_WORKSPACE;
   }
   hipStream_t s = as_stream(stream);
@@ -1019,10 +1021,10 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   a.x = logits, a.n = n, a.v = v, a.ldx = ld, a.ids = ids, a.ids64 = ids64, a.top = top, a.top_dt = top_dtype;
   a.k = k, a.lse = lse, a.w = weights, a.stats = stats, a.reduction = reduction;
   a.rows = reduction == SBOD_REDUCE_NONE ? rows : nullptr;
-  a.part = ws_at<float2>(workspace, chunks_offset(n, v, k, dtype, lse)), a.nchunk = distill_chunks(v, dtype);
+  a.part = ws_at<float2>(workspace, chunks_offset(n, v, k, dtype)), a.nchunk = distill_chunks(v, dtype);
   a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
-  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v, k, dtype, lse);
+  if (reduction != SBOD_REDUCE_NONE) a.parts = ws_at<double>(workspace, parts_offset()), a.nparts = parts_count(n, v, k, dtype);
   if (reduction == SBOD_REDUCE_MEAN && weights) {
     // (64 partial sums: each workgroup of the loss joins them)
     a.wparts = static_cast<const double *>(workspace);
@@ -1040,7 +1042,7 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
   a.loss = loss, a.norm = norm;
   hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, s, a);
   SBOD_LAUNCHED("k_distill_sum");
-  return grad && n > 0 && path_of(v, k, dtype, lse) == kChunks ? launch_grad(a, dtype, s) : SBOD_OK;
+  return grad && n > 0 && path_of(v, k, dtype) == kChunks ? launch_grad(a, dtype, s) : SBOD_OK;
 }
 
 extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
@@ -1062,5 +1064,5 @@ extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_
   a.stats = const_cast<float *>(stats), a.up = upstream, a.up_stride = reduction == SBOD_REDUCE_NONE ? 1 : 0;
   a.nchunk = distill_chunks(v, dtype), a.dx = grad, a.lddx = grad_ld;
   set_temperature(a, temperature);
-  return path_of(v, k, dtype, lse) != kChunks ? launch_any(a, dtype, as_stream(stream)) : launch_grad(a, dtype, as_stream(stream));
+  return path_of(v, k, dtype) != kChunks ? launch_any(a, dtype, as_stream(stream)) : launch_grad(a, dtype, as_stream(stream));
 }

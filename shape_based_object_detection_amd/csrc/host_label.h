@@ -104,7 +104,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, DistillCall *c) {
     const int64_t n = x.size(0), v = x.size(1), nst = sbod_distill_stat_floats();
     const int k = static_cast<int>(c->top.size(1));
-    const size_t nb = sbod_distill_workspace_bytes(n, v, k, c->lse.defined(), c->dt);
+    const size_t nb = sbod_distill_workspace_bytes(n, v, k, c->dt);
     const auto f32 = x.options().dtype(at::kFloat);
     at::Tensor kept = at::empty({nst * n + 1}, f32), ws = at::empty({static_cast<int64_t>(nb)}, x.options().dtype(at::kByte));
     const bool red = c->reduction != SBOD_REDUCE_NONE;

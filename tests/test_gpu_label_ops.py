@@ -36,7 +36,8 @@ def run_distill(x, ids, top, lse, w=None, T=1.0, reduction='mean', upstream=None
                                    (4, 255, 16), (6, 513, 100), (3, 1203, 16), (2, 1024, 1024), (3, 2048, 33),
                                    (2, 2049, 20), (3, 8191, 64), (2, 8193, 64), (2, 16385, 1000), (1, 40000, 3),
                                    (2, 50001, 100), (1, 131072, 64), (1, 200003, 50), (300, 40003, 30), (258, 61433, 7),
-                                   (2, 100003, 60), (261, 70001, 1024)])
+                                   (2, 100003, 60), (261, 70001, 1024), (259, 131070, 9),
+                                   (2, 65536, 65)])
 def test_distill_sizes(dt, tail, n, v, k):
     x, ids, top, lse = dev(*C.distill_inputs(n, v, k, dt, 7 * n + v + k, tail, wide=v % 2 == 0))
     loss, grad = run_distill(x, ids, top, lse, T=1.5)
@@ -45,7 +46,7 @@ def test_distill_sizes(dt, tail, n, v, k):
 
 @DT
 @TAIL
-@pytest.mark.parametrize('v', [21, 1203, 33000])
+@pytest.mark.parametrize('v', [21, 1203, 33000, 140001])
 @pytest.mark.parametrize('reduction', ['mean', 'sum', 'none'])
 def test_distill_odd_rows(dt, tail, v, reduction):
     """Weights, repeated and absent entries, masked and dead rows, NaN where nothing may read it."""
@@ -80,7 +81,7 @@ def test_distill_odd_rows(dt, tail, v, reduction):
 
 
 @DT
-@pytest.mark.parametrize('v', [13, 700, 9001])
+@pytest.mark.parametrize('v', [13, 700, 9001, 140001])
 def test_distill_values_that_are_not_finite(dt, v):
     """A live row's NaN or +inf comes out as NaN; a label the student forbids but the teacher keeps as an infinite loss."""
     x, ids, top, _ = dev(*C.distill_inputs(4, v, 3, dt, 5))
@@ -97,7 +98,7 @@ def test_distill_values_that_are_not_finite(dt, v):
 
 @DT
 @TAIL
-@pytest.mark.parametrize('v', [21, 1203, 20001])
+@pytest.mark.parametrize('v', [21, 1203, 20001, 133001])
 @pytest.mark.parametrize('extra,offset', [(0, 1), (3, 0), (5, 3), (64, 8)])
 def test_distill_strides(dt, tail, v, extra, offset):
     """Rows of a padded table that start anywhere; nothing outside them is read or written."""
@@ -114,7 +115,7 @@ def test_distill_strides(dt, tail, v, extra, offset):
 
 
 @DT
-@pytest.mark.parametrize('v', [21, 5003])
+@pytest.mark.parametrize('v', [21, 5003, 140001])
 def test_distill_backward_forms(dt, v):
     """Upstream 1, unit_grad, another factor, a retained graph used twice, no gradient: the same numbers."""
     x, ids, top, lse = dev(*C.distill_inputs(33, v, 5, dt, 11, True))
@@ -140,7 +141,7 @@ def test_distill_backward_forms(dt, v):
 
 
 @DT
-@pytest.mark.parametrize('v', [700, 30011, 90001])
+@pytest.mark.parametrize('v', [700, 30011, 90001, 140001])
 def test_distill_bucket_that_holds_nearly_all(dt, v):
     """Kept labels with little mass on both sides: rest and q_o are 1 but for it, and the loss is far below the rounding
     of 1.  It is off by what its terms are, each a share P (teacher) or Q (student) of the mass."""
