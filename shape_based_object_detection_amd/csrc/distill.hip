@@ -395,7 +395,7 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
 // labels: with a bucket they leave the row's sum, and their gradients come by a table in LDS.
 // Slots that every vocabulary of a (G, E) fills are read and written without a test.
 // Bound by instructions and its waves' waits, not by memory: 33 us for 327,936 anchors of 21 float32 labels (8 lanes
-// each; 76 MB, 2.3 TB/s), 57 to 63 us for 32,768 proposals of 1,203 bfloat16 labels (64 lanes; 163 MB).
+// each; 76 MB, 2.3 TB/s), 57 to 65 us for 32,768 proposals of 1,203 bfloat16 labels (64 lanes; 163 MB).
 template <int DT, int G, int E, bool kBucket, bool kMore>
 __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -605,9 +605,9 @@ constexpr int kSmallBlocks = 1280;
 // has kept entry k (K <= NT).  The elements before the row's first 16-byte boundary and behind its last
 // granule are one value each of the first 2 P threads.
 // With a bucket the kept labels leave the registers by a bit each in LDS, looked up a granule at a time.
-// Bound by memory: 476 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.5 TB/s of the 5.07 that a copy
-// reaches; 708 with a pass each for statistics and gradient); 254 us with the call for 2,049 rows of 50,001
-// float32 labels and a bucket, in nine rounds of 256 workgroups (327 by the kernels above).
+// Bound by memory: 476 to 502 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.4 TB/s of the 5.07 that a copy
+// reaches; 708 with a pass each for statistics and gradient); 255 us for 2,049 rows of 50,001
+// float32 labels and a bucket, in nine rounds of 256 workgroups (324 by the kernels above).
 template <int DT, bool kBucket, int NT, int NG>
 __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   using T = typename Elt<DT>::T;
