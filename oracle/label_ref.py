@@ -28,10 +28,12 @@ def distill_row(x, ids, top, lse, T):
             if pk != 0:
                 kl += pk * (lp - logq[i])
             g[i] -= pk
-        if lse is not None:
+        if lse is not None:   # (the masses sum to 1 with the bucket, unless it is cut off at 0 or has no label)
             other = np.ones(V, bool)
             other[[i for i, _ in keep]] = False
             rest = max(0.0, 1.0 - p.sum()) if other.any() else 0.0
+            total = p.sum() + rest
+            g += (total - 1.0) * np.exp(logq)
             if other.any():
                 zo = logq[other]
                 mo = zo.max()
@@ -39,7 +41,7 @@ def distill_row(x, ids, top, lse, T):
                 if rest > 0:
                     kl += rest * (np.log(rest) - logo)
                 share = np.zeros(zo.shape) if mo == -np.inf else np.exp(zo - mo) / np.exp(zo - mo).sum()
-                g[other] = share * (np.exp(logo) - rest)
+                g[other] = share * (total * np.exp(logo) - rest)
         return T * T * kl, T * g
 
 

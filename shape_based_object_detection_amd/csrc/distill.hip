@@ -8,7 +8,9 @@
 //   it did not keep, rest = 1 - sum p, is one bucket against the student's mass outside the kept
 //   labels, q_o: KL += rest (log rest - log q_o).
 //   row loss = w T^2 KL;  d/dx_v = w T (q_v - p_v) for a kept label (p summed over its repetitions),
-//   w T q_v for another one, or with a bucket w T (q_o - rest) q_v / q_o.
+//   w T q_v for another one;  with a bucket w T (total q_v - p_v) and w T (total q_o - rest) q_v / q_o,
+//   where total = sum p + rest: 1, unless sum p is above 1 (kept logits and lse rounded apart; rest is then
+//   0) or every label is kept (there is no bucket).
 //
 // The other labels' sum has a maximum of its own: q_o would underflow, and 1 - sum of the kept q
 // cancel, where the student is sure of a kept label.  The kept labels are gathered by themselves.
@@ -44,8 +46,8 @@ struct DistillArgs {
   double inv_td, tt;      // 1 / T, T^2
 };
 
-// What a row leaves for its gradient: q_v = 2^((x - m) s - l2s); another label than the kept ones
-// gets coef 2^((x - mo) s - l2so); p_k = exp((t_k - tb) / T - tl).
+// What a row leaves for its gradient: q_v (with a bucket total q_v) = 2^((x - m) s - l2s); another label
+// than the kept ones gets coef 2^((x - mo) s - l2so); p_k = exp((t_k - tb) / T - tl).
 enum { kStM, kStL2s, kStMo, kStL2so, kStCoef, kStTb, kStTl, kStLive, kStats };
 
 __device__ __forceinline__ bool row_has_weight(const DistillArgs &a, int64_t r) { return !a.w || a.w[r] != 0.f; }
@@ -167,14 +169,14 @@ __device__ __forceinline__ double uniform(double v) {
 }
 
 // The bucket of a row: the teacher's mass outside the kept labels, 1 - mass, against the student's, q_o.
-// term: its part of the KL; coef: q_o - rest.  Both sides are near 1 where the kept labels hold little, so
+// term: its part of the KL; coef: total q_o - rest.  Both sides are near 1 where the kept labels hold little, so
 // their logarithms and their difference are then taken from what the kept labels hold (P - Q = q_o - rest);
 // `mass` comes in 64 bits, for where they hold nearly all.  others: there is a label that is not kept (else
-// what is left of the teacher's mass is rounding).  kOne: all lanes of a wave have one row (its values pass
+// what is left of the teacher's mass has no label).  total: both, 1 unless the bucket was cut off.  kOne: all lanes of a wave have one row (its values pass
 // through scalar registers: k_distill_row's are full of the row).
 struct Bucket {
   double term;
-  float coef;
+  float coef, total;
 };
 template <bool kOne>
 __device__ __forceinline__ Bucket bucket_of(const DistillArgs &a, double mass, float kept, float sum, float so, float mo,
@@ -191,7 +193,9 @@ __device__ __forceinline__ Bucket bucket_of(const DistillArgs &a, double mass, f
                                 : (static_cast<double>(mo) - base) * a.inv_td + one(logf(so)) - one(logf(sum));
   Bucket b;
   b.term = rest > 0 ? rest * (logr - logo) : rest;
-  b.coef = little && mass < 1 && others ? static_cast<float>(mass - q) : static_cast<float>(one(expf(static_cast<float>(logo))) - rest);
+  b.total = mass > 1 || !others ? static_cast<float>(mass) : 1.f;
+  b.coef = little && mass < 1 && others ? static_cast<float>(mass - q)
+                                        : static_cast<float>(b.total * one(expf(static_cast<float>(logo))) - rest);
   return b;
 }
 
@@ -259,6 +263,7 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
     const float logs = logf(sum);
     // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
     double kl = 0, mass = 0;
+    float total = 1.f;
     for (int k = lane; k < a.k; k += kWave) {
       const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
       if (id < 0) continue;
@@ -273,11 +278,11 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
     if (kBucket) {
       const Bucket b = bucket_of<true>(a, wave_sum_f64(mass), ksum, sum, so, mo, m, kept < a.v);
       kl += b.term;
-      coef = b.coef;
+      coef = b.coef, total = b.total;
     }
     if (lane == 0) {
       st[kStM] = m;
-      st[kStL2s] = log2f(sum);
+      st[kStL2s] = log2f(sum / total);
       // (no other label with mass: 2^((x - 0) s - 0) is 0 for each of them)
       st[kStMo] = so == 0.f ? 0.f : mo;
       st[kStL2so] = so == 0.f ? 0.f : log2f(so);
@@ -547,8 +552,8 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     }
     // a row of -inf alone has no distribution: it is left out, as one of weight 0
     live = live && !(m == kNegInf && sum == 0.f);
-    const float logs = log_hw(sum), inv = 1.f / sum;
-    float coef = inv;   // what a label not kept takes of its exponential
+    const float logs = log_hw(sum);
+    float inv = 1.f / sum, coef = inv;   // what a label not kept takes of its exponential
     // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
     const auto term = [&](float p, float logp, float x) {   // 0 log 0 = 0
       return p == 0 ? 0.0 : p * (logp - ((static_cast<double>(x) - base) * a.inv_td - logs));
@@ -558,6 +563,7 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     if (kBucket) {
       const Bucket b = bucket_of<G == kWave>(a, mass, ksum, sum, so, mo, base, others);
       if (lane == 0) kl += b.term;
+      inv *= b.total;
       coef = so == 0.f ? 0.f : b.coef / so;
     }
     kl = live ? kl * a.tt * w : 0.0;
@@ -792,6 +798,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       if (kBucket) {
         const Bucket b = bucket_of<true>(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
         if (tid == 0) kl += b.term;
+        inv = uniform(inv * b.total);
         coef = uniform(so == 0.f ? 0.f : b.coef / so);
       }
       kl = live ? kl * a.tt * w : 0.0;

@@ -476,15 +476,16 @@ class _TopKDistill(torch.autograd.Function):
         kl = torch.where(p == 0, torch.zeros_like(p), p * (logp - logq.gather(1, ids))).sum(1)
         mass = torch.zeros_like(x).scatter_add_(1, ids, p)
         grad = logq.exp() - mass
-        if lse is not None:
+        if lse is not None:   # the masses and the bucket, `total`, are 1 unless the bucket was cut off at 0
             listed = torch.zeros(n, v).scatter_add_(1, ids, there.to(torch.float32)) > 0
             others = logq.masked_fill(listed, -math.inf)
             logo = torch.logsumexp(others, 1)
             rest = (1.0 - p.sum(1)).clamp(min=0.0)
             rest = rest.masked_fill(listed.all(1), 0.0)
+            total = (p.sum(1) + rest)[:, None]
             kl = kl + torch.where(rest > 0, rest * (torch.log(rest) - logo), rest)
             share = torch.softmax(others, 1).masked_fill((logo == -math.inf)[:, None], 0.0)
-            grad = torch.where(listed, grad, share * (logo.exp() - rest)[:, None])
+            grad = torch.where(listed, total * logq.exp() - mass, share * (total * logo.exp()[:, None] - rest[:, None]))
         elif not live.all():
             grad = grad.masked_fill(~live[:, None], 0.0)
         ctx.live = live

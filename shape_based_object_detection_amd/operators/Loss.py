@@ -120,7 +120,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, wei
     ``teacher_ids`` [..., K] (int32 / int64; an id outside [0, V) is an absent entry, one listed twice adds its
     masses) and ``teacher_logits`` [..., K], 1 <= K <= 1024: the teacher is their softmax at T.  With
     ``teacher_lse`` [...], its log-sum-exp of logits / T over the whole vocabulary, the kept entries keep their own
-    probabilities and what is left is one bucket against the student's mass on all other labels.
+    probabilities and what is left is one bucket against the student's mass on all other labels (nothing is left where
+    they exceed 1, as logits kept in fewer bits than the lse make them).
 
     ``weights`` [...]: each row's share.  'mean' divides by their sum (without weights: by the rows; 0 where that
     is 0), 'sum' adds, 'none' returns the weighted row losses [...].  Loss in float32, gradient in the logits'
