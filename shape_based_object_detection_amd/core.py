@@ -7,6 +7,7 @@ import contextlib
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -1208,8 +1209,12 @@ def _one_device(what, tensors):
 
 
 def _constant(what, name, t):
-    if t is not None and t.requires_grad and torch.is_grad_enabled():
+    if t is None:
+        return
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError('%s: %s requires a gradient, which is not computed: detach() it' % (what, name))
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError('%s: %s has a forward-mode tangent, which is not computed: unpack_dual() it' % (what, name))
 
 
 def _integral(what, name, t):

@@ -33,6 +33,8 @@ inline int label_dt(const at::Tensor &t) {
 }
 inline bool is_id(const at::Tensor &t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
 inline bool wants(const at::Tensor &t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+// core._constant refuses it: a derivative of either mode would be dropped.
+inline bool varies(const at::Tensor &t) { return wants(t) || t._fw_grad(0).defined(); }
 // [n, v] whose rows are contiguous and apart, as core._rows_of takes them without a copy.
 inline bool good_rows(const at::Tensor &t) {
   return t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
@@ -174,12 +176,12 @@ inline PyObject *label_distill_call(PyObject *const *a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   const auto vec = [&](const at::Tensor *t) {
     return !t || (t->dim() == 1 && t->size(0) == x->size(0) && t->scalar_type() == at::kFloat && t->is_contiguous() &&
-                  t->device() == x->device() && !wants(*t));
+                  t->device() == x->device() && !varies(*t));
   };
   if (!x->is_cuda() || (c.dt = label_dt(*x)) < 0 || (c.top_dt = label_dt(*top)) < 0 || !is_id(*ids) || !good_rows(*x) ||
       x->size(1) < 1 || ids->dim() != 2 || !ids->is_contiguous() || !top->is_contiguous() || ids->sizes() != top->sizes() ||
       ids->size(0) != x->size(0) || ids->size(1) < 1 || ids->size(1) > 1024 || ids->device() != x->device() ||
-      top->device() != x->device() || wants(*top) || !vec(lse) || !vec(w) ||
+      top->device() != x->device() || varies(*top) || !vec(lse) || !vec(w) ||
       !(c.temperature >= 1e-30f && c.temperature <= 1e30f))
     Py_RETURN_NONE;
   c.ids = *ids, c.top = top->detach();
@@ -262,7 +264,7 @@ inline PyObject *label_logits_call(PyObject *const *a, Py_ssize_t n_args) {
     return nullptr;
   }
   const at::Tensor *x = tensor_of(a[0]);
-  if (!x || !x->is_cuda() || !good_rows(*x) || x->size(1) < 1 || wants(*x)) Py_RETURN_NONE;
+  if (!x || !x->is_cuda() || !good_rows(*x) || x->size(1) < 1 || varies(*x)) Py_RETURN_NONE;
   const int dt = label_dt(*x);
   if (dt < 0) Py_RETURN_NONE;
   const int64_t n = x->size(0), v = x->size(1);
@@ -272,7 +274,7 @@ inline PyObject *label_logits_call(PyObject *const *a, Py_ssize_t n_args) {
   const auto opt = [&](PyObject *o) -> const at::Tensor * {
     if (o == Py_None) return none;
     const at::Tensor *t = tensor_of(o);
-    if (!t || t->device() != x->device() || wants(*t)) ok = false;
+    if (!t || t->device() != x->device() || varies(*t)) ok = false;
     // (in place, an argument in the logits' own storage: core.py's path looks at where)
     if (ok && a[11] == a[0] && t->is_alias_of(*x)) ok = false;
     return ok ? t : none;
@@ -300,7 +302,7 @@ inline PyObject *label_logits_call(PyObject *const *a, Py_ssize_t n_args) {
       scalar[i] = static_cast<float>(PyFloat_AS_DOUBLE(a[4 + i]));
     } else {
       const at::Tensor *t = tensor_of(a[4 + i]);
-      ok = t && t->device() == x->device() && !wants(*t) && t->dim() == 1 && t->size(0) == n && t->scalar_type() == at::kFloat &&
+      ok = t && t->device() == x->device() && !varies(*t) && t->dim() == 1 && t->size(0) == n && t->scalar_type() == at::kFloat &&
            t->is_contiguous();
       if (ok) per_row[i] = t->data_ptr<float>();
     }

@@ -26,7 +26,8 @@ def process_logits(logits, history=None, history_len=None, prompt_len=None, repe
     ``history`` [N, L] (or [L]: the same for every row; L < 2^29) int32 / int64: its first ``history_len`` [N] entries count
     (default: all), the first ``prompt_len`` [N] of them were given (repetition only), the others answered.
     ``repetition`` (> 0), ``presence``, ``frequency``: numbers, or float tensors [N].  An id outside [0, V) is
-    absent (padding).  Not differentiable: logits that require a gradient are refused while gradients are on.
+    absent (padding).  Not differentiable: tensors that require a gradient are refused while gradients are on, and
+    ones with a forward-mode tangent.
     """
     r = core.label_call('label_logits', logits, logits, history, history_len, prompt_len, repetition, presence, frequency,
                         bias, bias_ids, bias_values, allowed, out)

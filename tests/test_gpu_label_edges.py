@@ -3,9 +3,11 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import label_cases as C
 import label_wide as W
+import test_label_edges as E
 from shape_based_object_detection_amd.operators.Loss import topk_distill_loss
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +43,14 @@ def test_distill_bucket_gradient_is_the_derivative_of_its_loss(dt, top_dt, n, v,
     left = grad.double().sum(1).abs()
     rel = C.STEP * (105 + 4 * 30 + 4 * 26 + k + 4 * math.log(v + 1.0))
     assert torch.all(left <= C.half_step(dt) * 1.001 * grad.double().abs().sum(1) + v * C.smallest(dt) + 3.0 / n * T * rel * 12)
+
+
+# ------------------------------------------------------------------------------------------------ forward mode
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_is_refused(grad):
+    for name, t, call, error in E.tangent_calls(DEV):
+        with torch.set_grad_enabled(grad), fwAD.dual_level():
+            with pytest.raises(error):
+                call(fwAD.make_dual(t, torch.ones_like(t)))
+                pytest.fail(name)
+            call(t)
