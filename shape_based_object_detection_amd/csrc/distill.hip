@@ -628,8 +628,10 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   __shared__ double red64[16], masses[NW], losses[kTight ? NT : 1];
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int tid = threadIdx.x, wave = tid >> 6, v = static_cast<int>(a.v), kk = a.k;
-  if (kBucket)
+  if (kBucket) {
     for (int i = tid; i < NT * NG * P / 32 + 1; i += NT) bits[i] = 0;
+    __syncthreads();   // (another wave's threads set bits of these words)
+  }
   const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
   const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
   double loss = 0;

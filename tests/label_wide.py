@@ -47,6 +47,8 @@ def distill64(x, ids, top, lse, w, T, reduction, up):
 def check(loss, grad, x, ids, top, lse, w, T, reduction, up=1.0):
     """As label_cases.check_distill derives it; a factor of the kept mass, where that is above 1, on what it multiplies."""
     dt, (n, v) = x.dtype, x.shape
+    if w is not None:   # (a row of weight 0 is not read)
+        x = x.detach().masked_fill((w == 0)[:, None], 0.0)
     up = up.double() if torch.is_tensor(up) else torch.tensor(float(up), dtype=torch.float64, device=x.device)
     up = up.expand(n)
     want, gwant, rows, g1 = distill64(x, ids, top, lse, w, T, reduction, up)

@@ -54,3 +54,42 @@ def test_forward_mode_is_refused(grad):
                 call(fwAD.make_dual(t, torch.ones_like(t)))
                 pytest.fail(name)
             call(t)
+
+
+# ------------------------------------------------------------------------------------------------ many rows per workgroup
+def mixed_rows(n, v, k, dt, tail, seed):
+    """Rows of every kind beside one another, so that a workgroup's next row differs from its last: of weight 0 (some of
+    NaN), of -inf alone, with entries listed twice or absent, partly masked, plain."""
+    x, ids, top, lse = W.over_full(n, v, k, dt, dt, 1.5, seed) if tail else C.distill_inputs(n, v, k, dt, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    w = torch.rand(n, generator=g) + 0.1
+    kind = torch.randint(0, 8, (n,), generator=g)
+    w[kind == 0] = 0.0
+    x[(kind == 0).nonzero()[::2, 0]] = math.nan
+    x[kind == 1] = -math.inf
+    ids[kind == 2, 1] = ids[kind == 2, 0]
+    ids[kind == 3, 1:] = v
+    ids[kind == 4, 2] = -1
+    masked = (kind == 5).nonzero()[:, 0]
+    at = ids[masked].clamp(0, v - 1)   # (the student allows the kept labels)
+    keep = x[masked].gather(1, at)
+    x[masked, ::3] = -math.inf
+    x[masked] = x[masked].scatter(1, at, keep)
+    return x, ids, top, lse, w
+
+
+@TAIL
+@pytest.mark.parametrize('dt,n,v,k', [
+    (torch.float32, 50001, 21, 5), (torch.bfloat16, 45001, 33, 9), (torch.float16, 21001, 100, 12),
+    (torch.float32, 6001, 700, 16), (torch.bfloat16, 5501, 1203, 100), (torch.float16, 5203, 2048, 16),
+    (torch.float32, 2701, 2100, 256), (torch.bfloat16, 2601, 4101, 31), (torch.float16, 1301, 9001, 20),
+    (torch.float32, 1101, 6001, 200), (torch.float32, 1101, 9001, 7), (torch.bfloat16, 1030, 30003, 64),
+    (torch.float32, 1041, 17001, 500), (torch.bfloat16, 530, 50257, 64), (torch.float16, 521, 33000, 9),
+    (torch.float32, 600, 40003, 64), (torch.bfloat16, 520, 70001, 1000)])
+def test_distill_many_rows_per_workgroup(dt, tail, n, v, k):
+    x, ids, top, lse, w = dev(*mixed_rows(n, v, k, dt, tail, v + n))
+    one = torch.tensor(1.0, device=DEV)
+    for reduction, up in (('none', torch.rand(n, device=DEV) + 0.5), ('mean', one), ('sum', one * 0.25)):
+        loss, grad = run_distill(x, ids, top, lse, w, 1.5, reduction, up)
+        W.check(loss, grad, x, ids, top, lse, w, 1.5, reduction, up)
+        assert torch.all(grad[w == 0] == 0)
