@@ -479,8 +479,8 @@ int sbod_map_f32(const float *det_boxes, const int64_t *det_labels, const float 
  * at temperature T (1e-30 to 1e30):  p = softmax(top / T) over a row's entries, or with lse [N] (the teacher's
  * log sum exp(logits / T) over its whole vocabulary) p = exp(top / T - lse) and one bucket for the
  * mass outside the kept labels (none where theirs is above 1);  row = weights_row T^2 KL(p || softmax(logits / T)).  An entry listed
- * twice adds its masses.  A row of weight 0, without an entry, or whose logits are all -inf gives
- * loss 0 and a zero gradient, whatever else it holds.
+ * twice adds its masses.  A row of weight 0, without an entry (without lse: one that has mass), or
+ * whose logits are all -inf gives loss 0 and a zero gradient, whatever else it holds.
  *   rows [N] (reduction NONE): the row losses; loss, norm [1] (MEAN, SUM): the reduced loss and the factor
  *   on each row's gradient (1 / sum of weights, 1 / N or 1; MEAN over weights that sum to 0 gives 0);
  *   stats [sbod_distill_stat_floats(), per row]: kept for the gradient.

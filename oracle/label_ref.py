@@ -10,7 +10,7 @@ def distill_row(x, ids, top, lse, T):
     zero = np.zeros(V)
     if np.all(x == -np.inf):
         return 0.0, zero
-    if lse is None and not any(t > -np.inf or np.isnan(t) for _, t in keep):
+    if not any(lse is not None or t > -np.inf or np.isnan(t) for _, t in keep):
         return 0.0, zero
     with np.errstate(all='ignore'):
         z = x / T

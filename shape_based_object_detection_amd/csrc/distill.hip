@@ -253,8 +253,8 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
       sum = ksum + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s));
       wave_lds_fence();
     }
-    // a row of -inf alone has no distribution: it is left out, as one of weight 0
-    if (m == kNegInf && sum == 0.f) live = false;
+    // a row of -inf alone has no distribution, one without an entry nothing to learn: left out, as of weight 0
+    if ((m == kNegInf && sum == 0.f) || (kBucket && kept == 0)) live = false;
     if (!live) {
       if (lane < kStats) st[lane] = 0.f;
       if (lane == 0) put_row(a, r, 0.0);
@@ -512,9 +512,11 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
       // (slots of the lane that hold a label: j G + lane < v)
       const int held = v > lane ? (v - lane + G - 1) / G : 0;
       others = group_any<G>(held > 0 && (~mine & (0xffffffffu >> (32 - held))) != 0);
+      bool some = has0;
       if (has0) mk = x0;
-      more([&](int, int, float, float x) { mk = fmaxf(mk, x); });
+      more([&](int, int, float, float x) { mk = fmaxf(mk, x), some = true; });
       mk = group_max<G>(mk);
+      live = group_any<G>(some);   // (an entry is there in live rows only)
     }
 #pragma unroll
     for (int j = 0; j < E; ++j) {
@@ -626,10 +628,12 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   // (1,024 threads have no register to spare beside 16 granules: each one's loss waits in LDS, and its t is read again)
   constexpr bool kTight = NT == 1024;
   __shared__ double red64[16], masses[NW], losses[kTight ? NT : 1];
+  __shared__ int entered;   // with a bucket: the last row that has an entry (v > kSmallMax: n is below 2^31)
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int tid = threadIdx.x, wave = tid >> 6, v = static_cast<int>(a.v), kk = a.k;
   if (kBucket) {
     for (int i = tid; i < NT * NG * P / 32 + 1; i += NT) bits[i] = 0;
+    if (tid == 0) entered = -1;
     __syncthreads();   // (another wave's threads set bits of these words)
   }
   const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
@@ -708,7 +712,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       if (id >= 0) xk_raw = reinterpret_cast<const bits_t<DT> *>(row)[id];
       const int place = id - head + P;
       if (entry) ids_s[tid] = id, top_s[tid] = t;
-      if (kBucket && id >= 0) atomicOr(&bits[place >> 5], 1u << (place & 31));
+      if (kBucket && id >= 0) atomicOr(&bits[place >> 5], 1u << (place & 31)), entered = static_cast<int>(r);
       __syncthreads();
       float x1 = e1 >= 0 ? bits_value<DT>(xraw) : kNegInf;
       if (kBucket && e1 >= 0 && bits[(e1 - head + P) >> 5] >> ((e1 - head + P) & 31) & 1) x1 = kNegInf;
@@ -781,8 +785,9 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       so = uniform(group_sum<NW>(sums[0][tid % NW])), s1 = uniform(group_sum<NW>(sums[1][tid % NW]));
       if (kBucket) s2 = group_sum<NW>(masses[tid % NW]);
       const float sum = kBucket ? s1 + (mo == kNegInf ? so : so * exp2_hw((mo - base) * a.s)) : so;
-      // a row of -inf alone has no distribution, a teacher without mass nothing to say: left out, as of weight 0
-      live = !(m == kNegInf && sum == 0.f) && (kBucket || !(s1 == 0.f));
+      // a row of -inf alone has no distribution, a teacher without mass, or with a bucket without an entry, nothing to
+      // say: left out, as of weight 0
+      live = !(m == kNegInf && sum == 0.f) && (kBucket ? entered == static_cast<int>(r) : !(s1 == 0.f));
       const float logs = log_hw(sum);
       if (!kBucket) {
         tl = log_hw(s1);

@@ -467,9 +467,8 @@ class _TopKDistill(torch.autograd.Function):
         ids = ids.long().masked_fill(~there, 0)
         p = torch.softmax(t.masked_fill(~there, -math.inf), 1) if lse is None else torch.exp(t - lse.double()[:, None])
         p = p.masked_fill(~there, 0.0)
-        live = ~(logits == -math.inf).all(1)
-        if lse is None:   # without an entry that has mass there is nothing to learn
-            live &= ~(~there | (top == -math.inf)).all(1)
+        # without an entry (a bucket aside: one that has mass) there is nothing to learn
+        live = ~(logits == -math.inf).all(1) & (there if lse is not None else there & (top != -math.inf)).any(1)
         x, p = x.masked_fill(~live[:, None], 0.0), p.masked_fill(~live[:, None], 0.0)
         logq = torch.log_softmax(x, 1)
         logp = torch.log(p)
@@ -486,8 +485,6 @@ class _TopKDistill(torch.autograd.Function):
             kl = kl + torch.where(rest > 0, rest * (torch.log(rest) - logo), rest)
             share = torch.softmax(others, 1).masked_fill((logo == -math.inf)[:, None], 0.0)
             grad = torch.where(listed, total * logq.exp() - mass, share * (total * logo.exp()[:, None] - rest[:, None]))
-        elif not live.all():
-            grad = grad.masked_fill(~live[:, None], 0.0)
         ctx.live = live
         ctx.save_for_backward(grad.masked_fill_(~live[:, None], 0.0) * temperature)
         ctx.dtype = logits.dtype

@@ -125,8 +125,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, wei
 
     ``weights`` [...]: each row's share.  'mean' divides by their sum (without weights: by the rows; 0 where that
     is 0), 'sum' adds, 'none' returns the weighted row losses [...].  Loss in float32, gradient in the logits'
-    type.  A row of weight 0, without an entry that has mass, or whose logits are all -inf gives loss 0 and a zero
-    gradient.  The teacher's tensors and the weights are constants: one that requires a gradient (or has a forward-mode
+    type.  A row of weight 0, without an entry (without teacher_lse: one that has mass), or whose logits are all -inf
+    gives loss 0 and a zero gradient, whatever else it holds.  The teacher's tensors and the weights are constants: one that requires a gradient (or has a forward-mode
     tangent) is refused."""
     if reduction in REDUCE and torch.is_tensor(logits):
         r = core.label_call('label_distill', logits, logits, teacher_ids, teacher_logits, teacher_lse, weights,

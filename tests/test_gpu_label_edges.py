@@ -93,3 +93,20 @@ def test_distill_many_rows_per_workgroup(dt, tail, n, v, k):
         loss, grad = run_distill(x, ids, top, lse, w, 1.5, reduction, up)
         W.check(loss, grad, x, ids, top, lse, w, 1.5, reduction, up)
         assert torch.all(grad[w == 0] == 0)
+# ------------------------------------------------------------------------------------------------ rows without an entry
+@DT
+@pytest.mark.parametrize('v,k', [(13, 3), (200, 70), (1203, 3), (2049, 5), (9001, 3), (40001, 300), (140001, 3)])
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+def test_distill_row_without_an_entry(dt, v, k, reduction):
+    x, ids, top, lse = dev(*E.rows_without_entry(v, k, dt))
+    up = torch.ones(5 if reduction == 'none' else (), device=DEV)
+    loss, grad = run_distill(x, ids, top, lse, None, 1.0, reduction, up)
+    assert torch.all(grad[[0, 1, 4]] == 0) and grad.isfinite().all() and grad[3].abs().amax() > 0
+    # (row 2's largest gradient is one label's share, about 1 / v: half precision rounds shares below 2^-25 to 0)
+    assert dt == torch.float16 or grad[2].abs().amax() > 0
+    if reduction == 'none':
+        assert torch.all(loss[[0, 1, 4]] == 0) and loss[2] > 0
+    w = torch.tensor([0.0, 0, 1, 1, 1], device=DEV)   # (weight 0: as without an entry, but for the mean)
+    one, gone = run_distill(x, ids, top, lse, w, 1.0, reduction, up * (0.6 if reduction == 'mean' else 1.0))
+    W.check(one, gone, x, ids, top, lse, w, 1.0, reduction, up * (0.6 if reduction == 'mean' else 1.0))
+    assert torch.allclose(gone.float(), grad.float(), rtol=4 * C.half_step(dt) + 1e-6, atol=2 * C.smallest(dt))

@@ -83,3 +83,29 @@ def test_forward_mode_is_refused(grad):
     x = torch.randn(2, 5)
     with pytest.raises(ValueError, match='tangent'):
         torch.func.jvp(process_logits, (x,), (x,))
+
+
+# ------------------------------------------------------------------------------------------------ rows without an entry
+def rows_without_entry(v, k, dt):
+    """Five rows of a bucket: the first two without an entry, one of them in a row of NaN, the other beside an lse of NaN;
+    then one whose entry has no mass, an ordinary one, and one without an entry, all finite."""
+    x, ids, top, lse = C.distill_inputs(5, v, k, dt, 3, True)
+    ids[:2], ids[4] = -1, v + 1
+    x[0], lse[1] = math.nan, math.nan
+    top[2], ids[2, 1:] = -math.inf, -1
+    return x, ids, top, lse
+
+
+@pytest.mark.parametrize('reduction', ['none', 'sum', 'mean'])
+def test_distill_row_without_an_entry(reduction):
+    """Loss 0 and a zero gradient, whatever else the row holds, with a bucket too."""
+    x, ids, top, lse = rows_without_entry(13, 3, torch.float32)
+    x.requires_grad_(True)
+    loss = topk_distill_loss(x, ids, top, lse, reduction=reduction)
+    grad, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    assert torch.all(grad[[0, 1, 4]] == 0) and grad.isfinite().all() and torch.all(grad[[2, 3]].abs().amax(1) > 0)
+    want, gwant, _ = R.distill(x.detach().numpy(), ids.numpy(), top.numpy(), lse.numpy(), None, 1.0, reduction)
+    # float64 but for the returned float32
+    assert np.allclose(loss.detach().numpy(), want, rtol=2 * C.STEP) and np.allclose(grad.numpy(), gwant, rtol=1e-6, atol=1e-7)
+    if reduction == 'none':
+        assert torch.all(loss[[0, 1, 4]] == 0) and loss[2] > 0
