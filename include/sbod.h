@@ -502,8 +502,8 @@ int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_t v, int64_
 /* Penalties, biases and masks on logits before a label is chosen.  history [N, history_cols < 2^29] (row
  * stride history_ld, 0: one row for all): a row's first history_len entries count (NULL: all), of
  * them the first prompt_len were given, the others answered.  In this order:
- *   x / r where x > 0, else x r, for a label in the history;  - frequency count - presence [count > 0],
- *   count over the answered entries;  + bias (float32 or of dtype; row stride bias_ld, 0: one row);  + the listed biases
+ *   x / r where x > 0, else x r, for a label in the history;  - frequency count - presence for one that was
+ *   answered, count times;  + bias (float32 or of dtype; row stride bias_ld, 0: one row);  + the listed biases
  *   (bias_ids, bias_values [N, bias_cols <= 4096]; a label listed twice adds both, in order);
  *   -inf where the mask is 0 (SBOD_MASK_BITS: int32 words, label v in bit v % 32 of word v / 32;
  *   SBOD_MASK_BYTES: one byte per label; row stride mask_ld in words / bytes, 0: one row).

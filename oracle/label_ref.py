@@ -84,8 +84,10 @@ def process_logits(x, history=None, history_len=None, prompt_len=None, repetitio
                 c = int((h[max(given, 0):n] == v).sum()) if given < n else 0
                 rep = float(row(repetition, r))
                 x[r, v] = x[r, v] / rep if x[r, v] > 0 else x[r, v] * rep
-                mag[r, v] = np.abs(x[r, v]) + abs(row(frequency, r)) * c + abs(row(presence, r))
-                x[r, v] -= row(frequency, r) * c + (row(presence, r) if c else 0.0)
+                mag[r, v] = np.abs(x[r, v])
+                if c:   # (what was not answered keeps its value under an infinite penalty)
+                    mag[r, v] += abs(row(frequency, r)) * c + abs(row(presence, r))
+                    x[r, v] -= row(frequency, r) * c + row(presence, r)
         if bias is not None:
             b = np.asarray(bias, np.float64)
             x[r] += b if b.ndim == 1 else b[r]

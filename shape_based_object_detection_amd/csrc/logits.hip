@@ -2,7 +2,7 @@
 //
 // For a row x [V] with a history of labels, its first `prompt` entries given and the rest answered:
 //   x_v -> x_v / r (x_v > 0) or x_v r, where v is in the history;
-//   x_v -> x_v - frequency count_v - presence [count_v > 0], count over the answered entries;
+//   x_v -> x_v - frequency count_v - presence, where v was answered, count_v times;
 //   x_v -> x_v + bias_v (+ every listed bias of v, in the order listed);
 //   x_v -> -inf where the mask forbids v.
 // In 32 bits, one rounding at the end.
@@ -41,8 +41,7 @@ __device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int v, f
   if (word & (kSeen | kCount)) {
     x = x > 0.f ? x / rep : x * rep;
     const uint32_t answered = word & kCount;
-    x = x - freq * static_cast<float>(answered);
-    if (answered) x -= pres;
+    if (answered) x = x - freq * static_cast<float>(answered) - pres;   // (an infinite penalty times 0 is NaN)
   }
   if (kBias >= 0) x += ld_any(a.bias, r * a.ldb + v, kBias);
   if (word & kTwice) {   // in the order listed

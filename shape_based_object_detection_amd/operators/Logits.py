@@ -16,7 +16,7 @@ def process_logits(logits, history=None, history_len=None, prompt_len=None, repe
     In this order, in 32 bits with one rounding at the end:
 
     * a label of the row's history: ``x / repetition`` where x > 0, else ``x * repetition``;
-    * ``- frequency * count - presence * (count > 0)``, count over the answered part of the history;
+    * a label of the answered part, count times: ``- frequency * count - presence`` (infinite ones forbid it);
     * ``+ bias`` ([V] or [N, V], float32 or the logits' type), ``+ bias_values`` (float32) at ``bias_ids``
       ([M] or [N, M], M <= 4096; a label listed twice adds both);
     * ``-inf`` where ``allowed`` forbids the label: truth values [V] or [N, V], or int32 words [W] or [N, W]

@@ -109,3 +109,29 @@ def test_distill_row_without_an_entry(reduction):
     assert np.allclose(loss.detach().numpy(), want, rtol=2 * C.STEP) and np.allclose(grad.numpy(), gwant, rtol=1e-6, atol=1e-7)
     if reduction == 'none':
         assert torch.all(loss[[0, 1, 4]] == 0) and loss[2] > 0
+
+
+# ------------------------------------------------------------------------------------------------ penalties without end
+def endless(dt):
+    """Labels given but not answered, answered once and twice, and neither, under penalties without end."""
+    x = torch.tensor([[1.0, -2.0, 3.0, 0.5, 0.0, -1.0], [4.0, 1.0, -1.0, 2.0, -3.0, 0.25]]).to(dt)
+    hist, prompt = torch.tensor([[0, 1, 4, 2, 2], [5, 3, 3, 0, -1]]), torch.tensor([3, 1])
+    want = x.clone()
+    want[0, [0, 1, 4]] = torch.tensor([0.5, -4.0, 0.0]).to(dt)   # given: repetition alone
+    want[1, 5] = 0.125
+    want[0, 2], want[1, 3], want[1, 0] = -math.inf, -math.inf, -math.inf
+    return x, hist, prompt, want
+
+
+ENDLESS = [dict(frequency=math.inf), dict(presence=math.inf), dict(frequency=math.inf, presence=math.inf)]
+
+
+@pytest.mark.parametrize('kw', ENDLESS, ids=['frequency', 'presence', 'both'])
+@pytest.mark.parametrize('dt', list(C.DTYPES.values()), ids=list(C.DTYPES))
+def test_logits_penalties_without_end(dt, kw):
+    """An infinite penalty forbids what was answered and nothing else."""
+    x, hist, prompt, want = endless(dt)
+    assert torch.equal(process_logits(x, hist, prompt_len=prompt, repetition=2.0, **kw), want)
+    oracle, _ = R.process_logits(x.double().numpy(), hist.numpy(), None, prompt.numpy(), 2.0,
+                                 kw.get('presence', 0.0), kw.get('frequency', 0.0))
+    assert np.array_equal(oracle, want.double().numpy())
