@@ -1249,13 +1249,17 @@ def _empty_rows(t):
 def label_call(name, t, *args):
     """A label-vocabulary call in C++ (_sbodhost, csrc/host_label.h): its result, or None when it needs this module's
     path (CPU tensors, conversions, errors, no extension, or a caller that records the sbod_* calls)."""
-    ext = L.host_ext
-    if ext is None or L._recorder or not t.is_cuda:
+    if not t.is_cuda:
         return None
-    if t.requires_grad and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing() and ext.foreign_leaves(t):
+    L.lib()   # (a process's first call may be a captured one: the extension is there from here on)
+    ext = L.host_ext
+    if (t.requires_grad and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()
+            and (ext is None or ext.foreign_leaves(t))):
         # captured, the backward pass would take the other stream into the graph, and the capture's end stops the process
         raise RuntimeError('%s: a graph from before the capture still holds gradient nodes of these leaves, made on another '
-                           'stream: release its result first' % name)
+                           'stream%s: release its result first' % (name, '' if ext else ' (or may: no _sbodhost to tell)'))
+    if ext is None or L._recorder:
+        return None
     r = getattr(ext, name)(*args, L._raw_stream(t.get_device()))
     if type(r) is int:
         raise L.SbodError('%s failed (%d): %s' % (name, r, L.lib().sbod_last_error().decode(errors='replace')))
