@@ -242,11 +242,12 @@ inline PyObject *label_embed_call(PyObject *const *a, Py_ssize_t n) {
   EmbedCall c;
   const double scale = PyFloat_AS_DOUBLE(a[2]);
   c.scale = static_cast<float>(scale);
-  c.pad = a[3] == Py_None ? -1 : PyLong_AsLongLong(a[3]);
+  int beyond = 0;   // (an id beyond 64 bits: core.py's error)
+  c.pad = a[3] == Py_None ? -1 : PyLong_AsLongLongAndOverflow(a[3], &beyond);
   c.stream = PyLong_AsVoidPtr(a[4]);
   if (PyErr_Occurred()) return nullptr;
   if (!w->is_cuda() || (c.dt = label_dt(*w)) < 0 || !is_id(*ids) || ids->device() != w->device() || w->dim() != 2 ||
-      !w->is_contiguous() || !ids->is_contiguous() || !std::isfinite(scale) || w->size(0) < 1 ||
+      !w->is_contiguous() || !ids->is_contiguous() || !std::isfinite(scale) || beyond || w->size(0) < 1 ||
       (a[3] != Py_None && (c.pad < 0 || c.pad >= w->size(0))))
     Py_RETURN_NONE;
   c.ids = *ids;
@@ -289,7 +290,7 @@ inline PyObject *label_logits_call(PyObject *const *a, Py_ssize_t n_args) {
     ok = ok && (cols < 0 || t->size(-1) == cols);
   };
   const auto ld = [&](const at::Tensor *t) { return t && t->dim() == 2 ? t->stride(0) : 0; };
-  const auto cols = [&](const at::Tensor *t) { return t ? t->size(-1) : 0; };
+  const auto cols = [&](const at::Tensor *t) { return t && t->dim() > 0 ? t->size(-1) : 0; };
   rows(hist, -1), rows(bias, v), rows(bids, -1), rows(bval, bids ? cols(bids) : -1), rows(mask, -1);
   const auto lens = [&](const at::Tensor *t) {
     ok = ok && (!t || (hist && t->dim() == 1 && t->size(0) == n && t->scalar_type() == at::kInt && t->is_contiguous()));

@@ -153,3 +153,11 @@ def test_capture_is_refused_where_the_extension_is_not_loaded(state, monkeypatch
             monkeypatch.setattr(L, '_lib', None)
     del held
     gc.collect()
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_refusals_name_their_argument():
+    for call, name in E.refused(DEV):
+        with pytest.raises(ValueError, match='(process_logits|topk_distill_loss|scaled_embedding): .*' + name):
+            call()
+            pytest.fail(name)

@@ -135,3 +135,33 @@ def test_logits_penalties_without_end(dt, kw):
     oracle, _ = R.process_logits(x.double().numpy(), hist.numpy(), None, prompt.numpy(), 2.0,
                                  kw.get('presence', 0.0), kw.get('frequency', 0.0))
     assert np.array_equal(oracle, want.double().numpy())
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def refused(device):
+    """(call, what its error names) for arguments without a dimension, and a padding id beyond 64 bits."""
+    x, one = torch.randn(2, 5, device=device), torch.tensor(1.0, device=device)
+    ids, whole = torch.zeros(2, 3, dtype=torch.int64, device=device), torch.tensor(1, device=device)
+    top = torch.zeros(2, 3, device=device)
+    yield lambda: process_logits(x, history=whole), 'history'
+    yield lambda: process_logits(x, ids, history_len=whole.int()), 'history_len'
+    yield lambda: process_logits(x, bias=one), 'bias'
+    yield lambda: process_logits(x, bias_ids=whole, bias_values=one), 'bias_ids'
+    yield lambda: process_logits(x, bias_ids=ids, bias_values=one), 'bias_values'
+    yield lambda: process_logits(x, allowed=one > 0), 'allowed'
+    yield lambda: process_logits(x, allowed=whole.int()), 'allowed'
+    yield lambda: process_logits(x, ids, presence=one), 'presence'
+    yield lambda: process_logits(one), 'logits'
+    yield lambda: topk_distill_loss(one, whole, one), 'logits'
+    yield lambda: topk_distill_loss(x, whole, one), 'teacher_ids'
+    yield lambda: topk_distill_loss(x, ids, top, one), 'teacher_lse'
+    yield lambda: topk_distill_loss(x, ids, top, None, one), 'weights'
+    yield lambda: scaled_embedding(ids, one), 'weight'
+    yield lambda: scaled_embedding(ids, x, 1.0, 1 << 70), 'padding_idx'
+
+
+def test_refusals_name_their_argument():
+    for call, name in refused('cpu'):
+        with pytest.raises(ValueError, match='(process_logits|topk_distill_loss|scaled_embedding): .*' + name):
+            call()
+            pytest.fail(name)
