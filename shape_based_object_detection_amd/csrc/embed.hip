@@ -7,6 +7,7 @@
 // that own a range of labels each, then each row of the table is summed by the threads that own its
 // columns, in 32 bits, and written once (zeros where no label came): no atomics on sums, no clearing pass.
 // A label that came often is summed in pieces first (k_embed_pieces), so that no thread walks a long run.
+// Few labels at few positions take one launch instead (k_embed_few).
 #include <type_traits>
 
 #include "label_dev.h"
@@ -345,6 +346,98 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_grad(const void *grad, co
   }
 }
 
+// d table of few labels from few positions, in one launch and without a sort.  A workgroup has a label and a tile
+// of columns: its waves look through 512 positions each for the label's and list them in order, its threads, as
+// (columns, slots), add every slots'th row of the list, and the slots are joined: in a wave by lane swaps, the waves'
+// sums in LDS.  Bound by the latency of that chain: 7 us for 6,400 positions of 21 labels, 256 float32 columns (the
+// sort and what is behind it 18 in three launches), 21 where all 8,192 have one label (49).
+constexpr int kFewWave = 512;              // positions of a wave
+constexpr int kFewMost = 16 * kFewWave;    // of a workgroup of 1,024 threads
+constexpr int kFewCols = 64;               // columns of a tile
+template <int DT, int kV>
+__global__ __launch_bounds__(1024) void k_embed_few(const void *grad, const void *ids, int ids64, int n, int64_t v,
+                                                    int64_t padding, int64_t groups, int lanes, float scale, void *dtable) {
+  using T = typename Elt<DT>::T;
+  using V = vec_t<T, kV>;
+  constexpr int kSteps = kFewWave / kWave;
+  __shared__ uint16_t list[kFewMost];
+  __shared__ int counts[16];
+  __shared__ float part[16][kFewCols];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, waves = blockDim.x >> 6, label = blockIdx.x;
+  const int first = wv * kFewWave + lane;
+  RawId raw[kSteps];
+#pragma unroll
+  for (int u = 0; u < kSteps; ++u) raw[u] = ld_raw_id(ids, min(first + u * kWave, n - 1), ids64);
+  unsigned long long hit[kSteps];
+  int mine = 0;
+#pragma unroll
+  for (int u = 0; u < kSteps; ++u) {
+    hit[u] = __ballot(first + u * kWave < n && label != padding && id_of(raw[u], ids64, v) == label);
+    mine += __popcll(hit[u]);
+  }
+  if (lane == 0) counts[wv] = mine;
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int w = 0; w < waves; ++w) {
+    if (w < wv) at += counts[w];
+    total += counts[w];
+  }
+#pragma unroll
+  for (int u = 0; u < kSteps; ++u) {
+    if (hit[u] >> lane & 1) list[at + __popcll(hit[u] & ((1ull << lane) - 1))] = static_cast<uint16_t>(first + u * kWave);
+    at += __popcll(hit[u]);
+  }
+  __syncthreads();
+  const int col = threadIdx.x & (lanes - 1), slots = blockDim.x / lanes;
+  const int64_t d = groups * kV, g = blockIdx.y * static_cast<int64_t>(lanes) + col;
+  float acc[kV];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) acc[j] = 0.f;
+  if (g < groups) {
+    constexpr int kU = 4;   // rows in flight
+    for (int i = threadIdx.x / lanes; i < total; i += kU * slots) {
+      V s[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (i + u * slots < total) s[u] = reinterpret_cast<const V *>(static_cast<const T *>(grad) + list[i + u * slots] * d)[g];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (i + u * slots < total) {
+#pragma unroll
+          for (int j = 0; j < kV; ++j) acc[j] += static_cast<float>(s[u][j]);
+        }
+    }
+  }
+  for (int m = lanes; m < kWave; m <<= 1) {
+#pragma unroll
+    for (int j = 0; j < kV; ++j) acc[j] += __shfl_xor(acc[j], m, kWave);
+  }
+  if (lane < lanes) {
+#pragma unroll
+    for (int j = 0; j < kV; ++j) part[wv][lane * kV + j] = acc[j];
+  }
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < lanes && g < groups) {
+    for (int w = 1; w < waves; ++w) {
+#pragma unroll
+      for (int j = 0; j < kV; ++j) acc[j] += part[w][lane * kV + j];
+    }
+    V o;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) o[j] = static_cast<T>(acc[j] * scale);
+    reinterpret_cast<V *>(static_cast<T *>(dtable) + label * d)[g] = o;
+  }
+}
+
+// Columns of a tile of k_embed_few; 0: the sort and the kernels behind it.  Half tiles, for more rows at a time, where
+// they fit the device at once; whole ones up to two (of fewer positions, with fewer waves, four) workgroups of 1,024
+// threads per place: there it takes 0.4 to 0.8 of the others' time, at twice as many 0.5 to 1.3 of it.
+int few_columns(int64_t n, int64_t v, int64_t d) {
+  if (n < 1 || n > kFewMost) return 0;
+  if (v * ((2 * d + kFewCols - 1) / kFewCols) <= 512) return kFewCols / 2;
+  return v * ((d + kFewCols - 1) / kFewCols) <= (n <= kFewMost / 2 ? 2048 : 1024) ? kFewCols : 0;
+}
+
 template <int DT, int kV>
 constexpr auto k_embed_grad_wide = &k_embed_grad<DT, kV, 4>;
 template <int DT, int kV>
@@ -422,6 +515,7 @@ extern "C" int sbod_embed_fwd(const void *table, int dtype, int64_t v, int64_t d
 
 extern "C" size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v, int64_t d) {
   if (n < 0 || v <= 0 || d < 0) return 0;
+  if (few_columns(n, v, d)) return align_up(1);   // (not used: a call always brings one)
   const int64_t rows = piece_rows(n), chunks = n > rows ? (n + rows - 1) / rows : 0;
   return align_up((v + 1) * sizeof(int32_t)) + align_up((n > 0 ? n : 1) * sizeof(int32_t)) +
          static_cast<size_t>(chunks) * 2 * d * sizeof(float);
@@ -439,6 +533,15 @@ extern "C" int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d,
     return SBOD_E_WORKSPACE;
   }
   hipStream_t s = as_stream(stream);
+  const int w = column_group(d, dtype, grad, grad_table);
+  if (const int c = few_columns(n, v, d)) {
+    const dim3 few(static_cast<unsigned>(v), static_cast<unsigned>((d + c - 1) / c));
+    const dim3 threads(n <= 4 * kFewWave ? 256 : n <= 8 * kFewWave ? 512 : 1024);
+    SBOD_EMBED_LAUNCH(k_embed_few, dtype, w, few, threads, grad, ids, ids64, static_cast<int>(n), v, padding, d / w, c / w, scale,
+                      grad_table);
+    SBOD_LAUNCHED("k_embed_few");
+    return SBOD_OK;
+  }
   int32_t *begin = static_cast<int32_t *>(workspace);
   int32_t *sorted = ws_at<int32_t>(workspace, align_up((v + 1) * sizeof(int32_t)));
   const int range = static_cast<int>(sort_range(v));
@@ -449,7 +552,6 @@ extern "C" int sbod_embed_bwd(const void *grad, int dtype, int64_t v, int64_t d,
   else
     hipLaunchKernelGGL(k_embed_sort<int32_t>, sgrid, sblock, lds, s, static_cast<const int32_t *>(ids), n, v, range, begin, sorted);
   SBOD_LAUNCHED("k_embed_sort");
-  const int w = column_group(d, dtype, grad, grad_table);
   const dim3 block = row_block(d / w);
   const int64_t tiles = (d / w + block.x - 1) / block.x;   // of a row's columns, a workgroup each
   const int rows = piece_rows(n);

@@ -186,3 +186,40 @@ def test_logits_in_place_gives_the_same_bits(dt, n, v, length, m, kind):
     view.copy_(x)
     process_logits(view, *args, allowed=allowed, out=view)
     assert torch.equal(view, got) and torch.all(off[:3] == 7)
+
+
+# ------------------------------------------------------------------------------------------------ gradients of few labels
+@DT
+@pytest.mark.parametrize('n,v,d', [(1, 1, 1), (63, 2, 31), (65, 512, 32), (300, 513, 32), (512, 21, 33), (513, 91, 100), (2047, 9, 7),
+                                   (2048, 3, 1000), (2049, 2048, 64), (4096, 2049, 64), (4097, 1024, 48), (4096, 40, 3201),
+                                   (8191, 1025, 64), (8192, 21, 256), (8193, 21, 256), (8192, 1, 2049)])
+@pytest.mark.parametrize('kind', ['spread', 'one', 'unaligned'])
+def test_embedding_gradient_of_few_labels(dt, n, v, d, kind):
+    """On both sides of each bound where another kernel, tile or workgroup takes over; one label at all positions; rows off
+    every boundary, 32-bit ids."""
+    g = torch.Generator().manual_seed(n + v + d)
+    ids = torch.randint(-1, v + 1, (n,), generator=g) if kind != 'one' else torch.full((n,), v - 1)
+    ids = ids.int() if kind == 'unaligned' else ids
+    pad = v // 2 if kind == 'spread' and v > 1 else None
+    go = torch.randn(n, d, generator=g).to(dt)
+    table = torch.zeros(v, d, dtype=dt, device=DEV).requires_grad_(True)
+    god = go.to(DEV)
+    if kind == 'unaligned':
+        store = torch.zeros(n * d + 1, dtype=dt, device=DEV)
+        god = store[1:].view(n, d).copy_(god)
+    idd = ids.to(DEV)
+    grads = [torch.autograd.grad(scaled_embedding(idd, table, 1.7, pad), table, god)[0] for _ in range(2)]
+    C.check_embedding_grad(grads[0], ids, go, v, 1.7, -1 if pad is None else pad)
+    assert torch.equal(grads[0], grads[1])
+
+
+def test_embedding_gradient_of_few_labels_holds_nan_where_it_came():
+    ids = torch.tensor([2, 0, 2, -1, 1], device=DEV)
+    go = torch.ones(5, 40, device=DEV)
+    go[0, 3], go[4, 7], go[3] = math.nan, math.inf, math.nan
+    table = torch.zeros(4, 40, device=DEV).requires_grad_(True)
+    grad, = torch.autograd.grad(scaled_embedding(ids, table), table, go)
+    want = torch.zeros(4, 40, device=DEV)
+    want[0], want[1], want[2] = 1.0, 1.0, 2.0
+    want[2, 3], want[1, 7] = math.nan, math.inf
+    assert torch.equal(grad.isnan(), want.isnan()) and torch.equal(grad.nan_to_num(), want.nan_to_num())
