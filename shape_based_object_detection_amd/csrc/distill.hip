@@ -505,6 +505,45 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     const uint32_t mine = mask[lane];
     wave_lds_fence();
     mask[lane] = 0;
+    // A label listed twice counts at its first entry (bit c of `firsts`: this lane's entry c G + lane), and that
+    // one has the sum of its masses, in the list's order, by the label's place in the row.
+    uint32_t firsts = ~0u;
+    if (twice) {
+      uint32_t *place = reinterpret_cast<uint32_t *>(own);
+      if (has0) place[id0] = ~0u;
+      more([&](int, int id, float, float) { place[id] = ~0u; });
+      wave_lds_fence();
+      if (has0) atomicMin(&place[id0], static_cast<uint32_t>(lane));
+      more([&](int k, int id, float, float) { atomicMin(&place[id], static_cast<uint32_t>(k)); });
+      wave_lds_fence();
+      if (has0 && place[id0] != static_cast<uint32_t>(lane)) firsts &= ~1u;
+      more([&](int k, int id, float, float) {
+        if (place[id] != static_cast<uint32_t>(k)) firsts &= ~(1u << (k / G));
+      });
+      wave_lds_fence();
+      if (a.dx) {
+        if (has0 && firsts & 1) own[id0] = p0;
+        more([&](int k, int id, float t, float) {
+          if (firsts >> (k / G) & 1) own[id] = p_at(logp_at(t));
+        });
+        wave_lds_fence();
+        for (int c = 0; c * G < kk; ++c) {   // the others one by one
+          const int k = c * G + lane;
+          int id = c == 0 && has0 ? id0 : -1;
+          float p = p0;
+          if (kMore && c > 0 && k < kk && live) {
+            id = ld_id(a.ids, r * kk + k, a.ids64, a.v);
+            p = p_at(logp_at(ld_any(a.top, r * kk + k, a.top_dt)));
+          }
+          for (unsigned long long late = group_ballot<G>(id >= 0 && !(firsts >> c & 1)); late; late &= late - 1) {
+            const int from = __ffsll(late) - 1, label = __shfl(id, from, G);
+            const float more_mass = __shfl(p, from, G);
+            if (lane == 0) own[label] += more_mass;
+          }
+        }
+        wave_lds_fence();
+      }
+    }
     // the student: the row's labels, with a bucket those not kept
     float mo = kNegInf, mk = kNegInf;
     bool others = false;
@@ -536,16 +575,10 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     float sum = so, ksum = 0.f;
     double mass = 0;
     if (kBucket) {
-      // (a label listed twice counts once, at its first entry: the sums' order is the list's)
-      const auto first = [&](int k, int id) {
-        for (int i = 0; i < k; ++i)
-          if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id) return false;
-        return true;
-      };
-      float sk = has0 && (!twice || first(lane, id0)) ? e0 : 0.f;
+      float sk = has0 && firsts & 1 ? e0 : 0.f;
       mass = p0;
-      more([&](int k, int id, float t, float x) {
-        if (!twice || first(k, id)) sk += exp2_hw((x - base) * a.s);
+      more([&](int k, int, float t, float x) {
+        if (firsts >> (k / G) & 1) sk += exp2_hw((x - base) * a.s);
         mass += p_at(logp_at(t));
       });
       ksum = sk = group_sum<G>(sk);
@@ -577,17 +610,9 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
     if (!a.dx) continue;
     float g = a.t * w * norm * up;
     if (a.up && a.up_stride) g *= a.up[r];
-    const auto mass_of = [&](int id, float p) {
-      if (!twice) return p;
-      p = 0.f;
-      for (int i = 0; i < kk; ++i)
-        if (ld_id(a.ids, r * kk + i, a.ids64, a.v) == id)
-          p += p_at(logp_at(ld_any(a.top, r * kk + i, a.top_dt)));
-      return p;
-    };
-    if (has0) own[id0] = g * (e0 * inv - mass_of(id0, p0));
-    more([&](int, int id, float t, float x) {
-      own[id] = g * (exp2_hw((x - base) * a.s) * inv - mass_of(id, p_at(logp_at(t))));
+    if (has0 && firsts & 1) own[id0] = g * (e0 * inv - (twice ? own[id0] : p0));
+    more([&](int k, int id, float t, float x) {
+      if (firsts >> (k / G) & 1) own[id] = g * (exp2_hw((x - base) * a.s) * inv - (twice ? own[id] : p_at(logp_at(t))));
     });
     wave_lds_fence();
     const float gc = g * coef;

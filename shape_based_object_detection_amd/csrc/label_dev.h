@@ -191,11 +191,15 @@ __device__ __forceinline__ double group_sum(double v) {
   for (int m = G / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
   return v;
 }
+// Bit i: lane i of the group.
+template <int G>
+__device__ __forceinline__ unsigned long long group_ballot(bool b) {
+  const unsigned long long m = __ballot(b);
+  return G < kWave ? m >> ((threadIdx.x & 63) / G * G) & ((1ull << (G & 63)) - 1) : m;
+}
 template <int G>
 __device__ __forceinline__ bool group_any(bool b) {
-  unsigned long long m = __ballot(b);
-  if (G < kWave) m = m >> ((threadIdx.x & 63) / G * G) & ((1ull << (G & 63)) - 1);
-  return m != 0;
+  return group_ballot<G>(b) != 0;
 }
 __device__ __forceinline__ float wave_max_f32(float v) { return group_max<kWave>(v); }
 

@@ -223,3 +223,23 @@ def test_embedding_gradient_of_few_labels_holds_nan_where_it_came():
     want[0], want[1], want[2] = 1.0, 1.0, 2.0
     want[2, 3], want[1, 7] = math.nan, math.inf
     assert torch.equal(grad.isnan(), want.isnan()) and torch.equal(grad.nan_to_num(), want.nan_to_num())
+
+
+# ------------------------------------------------------------------------------------------------ repeated entries
+@DT
+@TAIL
+@pytest.mark.parametrize('n,v,k', [(40, 5, 8), (70, 33, 32), (50, 100, 31), (30, 128, 64), (20, 700, 600), (30, 1203, 231),
+                                   (12, 2048, 1024), (10, 2049, 256), (6, 40001, 700), (4, 140001, 90)])
+def test_distill_entries_listed_many_times(dt, tail, n, v, k):
+    """Each label several times, and rows of one label alone: masses are added, the student's label counts once."""
+    x, ids, top, lse = W.over_full(n, v, k, dt, dt, 1.5, k) if tail else C.distill_inputs(n, v, k, dt, k)
+    g = torch.Generator().manual_seed(v)
+    ids = torch.randint(0, max(v // 2 if v < 100 else k // 3, 1), (n, k), generator=g) * (1 if v < 100 else v // k)
+    ids[1] = v - 1
+    ids[2, ::2] = -1
+    x, ids, top, lse = dev(x, ids, top, lse)
+    for reduction, up in (('none', torch.rand(n, device=DEV) + 0.5), ('sum', torch.tensor(1.0, device=DEV))):
+        loss, grad = run_distill(x, ids, top, lse, None, 1.5, reduction, up)
+        W.check(loss, grad, x, ids, top, lse, None, 1.5, reduction, up)
+        again = run_distill(x, ids, top, lse, None, 1.5, reduction, up)
+        assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
