@@ -518,8 +518,9 @@ int sbod_logits_process(const void *logits, int dtype, int64_t n, int64_t v, int
                         const void *mask, int mask_kind, int64_t mask_ld, void *out, int64_t out_ld, void *stream);
 
 /* out [N, D < 2^23] = scale table[ids] (an absent id: zeros), and d table [V, D] = scale sum of grad's rows of
- * each label, added in 32 bits in ascending position, zeros where none came; `padding` (-1: none) is a
- * label that gets no gradient.  table, out, grad, grad_table are contiguous. */
+ * each label, zeros where none came; `padding` (-1: none) is a label that gets no gradient.  A label's rows are added
+ * in 32 bits in an order that the call's ids and sizes fix: the same call gives the same bits, but a label's may differ
+ * in a call whose other ids differ.  table, out, grad, grad_table are contiguous. */
 int sbod_embed_fwd(const void *table, int dtype, int64_t v, int64_t d, const void *ids, int ids64, int64_t n,
                    float scale, void *out, void *stream);
 size_t sbod_embed_bwd_workspace_bytes(int64_t n, int64_t v, int64_t d);

@@ -14,8 +14,9 @@ def scaled_embedding(ids, weight, scale=1.0, padding_idx=None):
     bfloat16 or float16.
 
     The product is taken in 32 bits and rounded once.  An id outside [0, V) reads zeros.  The table's gradient is
-    dense, each label's rows added in 32 bits in the order of their positions (the same bits every time), zeros
-    where a label did not occur and for ``padding_idx``, whose row is looked up like any other."""
+    dense, each label's rows added in 32 bits in an order that the call's ids and sizes fix (the same bits every time for
+    the same ids; other ids beside a label's may change its last bits), zeros where a label did not occur and for
+    ``padding_idx``, whose row is looked up like any other."""
     r = core.label_call('label_embed', weight, ids, weight, float(scale), padding_idx)
     if r is not None:
         return r
