@@ -71,7 +71,7 @@ __device__ __forceinline__ void mark_kept(const DistillArgs &a, int64_t r, int64
 
 // {max, sum of 2^((x - max) s)} of each chunk of a row; with a bucket, of its labels not kept.  For rows
 // that no workgroup's registers hold: 16 KB per item, so that few long rows fill the device too.  Bound by its
-// one read: 94 us for 2,049 rows of 50,001 float32 labels (410 MB, 4.4 TB/s).
+// one read: 249 us for 2,048 rows of 131,072 float32 labels and a bucket (1.07 GB, 4.3 TB/s).
 template <int DT, bool kBucket>
 __global__ __launch_bounds__(kDistThreads) void k_distill_part(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -205,7 +205,7 @@ __device__ __forceinline__ double teacher_logp(const DistillArgs &a, int64_t i, 
 }
 
 // One wave per row: the chunks joined, the teacher's side, the row's loss and statistics.  Bound by its chain of
-// loads (ids, then the logits they name): 22 us for 2,049 rows with 100 kept labels.
+// loads (ids, then the logits they name): 15 us for 2,048 rows with 64 kept labels and a bucket.
 template <int DT, bool kBucket>
 __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -336,8 +336,8 @@ __global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
 // dx of one chunk of a row from the row's statistics.  The kept labels are written a second time,
 // behind a barrier, by a thread each.  The rows are taken from the last to the first: the ones that
 // k_distill_part read last are still in the Infinity Cache (256 MB), and the gradient is stored past it.
-// Bound by its read and write: 202 us for 2,049 rows of 50,001 float32 labels (819 MB, 4.1 TB/s), 222 from the
-// first row to the last.
+// Bound by its read and write: 439 us for 2,048 rows of 131,072 float32 labels (2.15 GB, 4.9 TB/s); from the
+// first row to the last the three kernels take 710 us instead of 690 (256 rows, all in the cache: 95 both ways).
 template <int DT>
 __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -399,8 +399,9 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
 // they are needed; their code costs the others registers), its logit gathered from the row.  A bit mask per lane says which of its slots are kept
 // labels: with a bucket they leave the row's sum, and their gradients come by a table in LDS.
 // Slots that every vocabulary of a (G, E) fills are read and written without a test.
-// Bound by instructions and its waves' waits, not by memory: 33 us for 327,936 anchors of 21 float32 labels (8 lanes
-// each; 76 MB, 2.3 TB/s), 57 to 65 us for 32,768 proposals of 1,203 bfloat16 labels (64 lanes; 163 MB).
+// Bound by instructions and its waves' waits, not by memory: 27 us for 327,936 anchors of 21 float32 labels (8 lanes
+// each; 76 MB, 2.8 TB/s; vector instructions keep the SIMDs busy 52 % of the time), 64 to 67 us for 32,768 proposals
+// of 1,203 bfloat16 labels (64 lanes; 163 MB, busy 34 %).
 template <int DT, int G, int E, bool kBucket, bool kMore>
 __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -630,6 +631,8 @@ __global__ __launch_bounds__(256) void k_distill_small(DistillArgs a) {
 }
 
 constexpr int kSmallMax = 2048;   // labels k_distill_small holds
+// Workgroups at most: what the device holds at once at five waves per SIMD.  (From 1,025 labels on, and with a bucket from
+// 513, the registers allow two to four: a second, uneven round.)
 constexpr int kSmallBlocks = 1280;
 
 // A vocabulary that a workgroup's registers hold: NT threads with NG 16-byte granules each keep the row from
@@ -638,9 +641,11 @@ constexpr int kSmallBlocks = 1280;
 // has kept entry k (K <= NT).  The elements before the row's first 16-byte boundary and behind its last
 // granule are one value each of the first 2 P threads.
 // With a bucket the kept labels leave the registers by a bit each in LDS, looked up a granule at a time.
-// Bound by memory: 476 to 502 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.4 TB/s of the 5.07 that a copy
-// reaches; 708 with a pass each for statistics and gradient); 255 us for 2,049 rows of 50,001
-// float32 labels and a bucket, in nine rounds of 256 workgroups (324 by the kernels above).
+// Bound by memory: 484 to 512 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.3 TB/s of the 5.07 that a copy
+// reaches; 708 with a pass each for statistics and gradient), 566 with a bucket.  With a bucket the reductions of the one
+// row that a CU holds are not under another row's traffic: 255 us for 2,049 rows of 50,001 float32 labels, in nine rounds
+// of 256 workgroups (324 by the kernels above), and 321 us for 4,096 rows of 50,257 bfloat16 labels, whose 512 threads
+// have one workgroup per CU (162 us of memory; 217 for the pass without a bucket).
 template <int DT, bool kBucket, int NT, int NG>
 __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -942,8 +947,9 @@ int launch_small(const DistillArgs &a, hipStream_t s) {
   return SBOD_OK;
 }
 
-// Threads and granules of k_distill_row for a row, smallest first, and the workgroups that the device holds at
-// once.  -1: none, k_distill_part and the kernels behind it.
+// Threads and granules of k_distill_row for a row, smallest first, and the workgroups launched at most: what the
+// device holds at once without a bucket (with one, the registers of 16 granules allow 768 and 256 workgroups of the 256
+// and 512 threads).  -1: none, k_distill_part and the kernels behind it.
 struct RowShape {
   int nt, ng, groups;
 };

@@ -1,12 +1,14 @@
 // Rows of a label table, scaled, and the table's gradient by sorted labels.
 //
-//   out[i] = scale table[id_i];   d table[v] = scale sum over {i : id_i = v} of grad[i], in ascending i.
+//   out[i] = scale table[id_i];   d table[v] = scale sum over {i : id_i = v} of grad[i].
 // An id outside [0, V) reads a row of zeros and gets no gradient; the padding id gets none.
 //
-// The gradient's order is fixed: the positions of each label are sorted first, one launch of workgroups
+// The gradient's order is fixed by the call's ids and sizes: the positions of each label are sorted first, one launch of workgroups
 // that own a range of labels each, then each row of the table is summed by the threads that own its
 // columns, in 32 bits, and written once (zeros where no label came): no atomics on sums, no clearing pass.
-// A label that came often is summed in pieces first (k_embed_pieces), so that no thread walks a long run.
+// A label that came often is summed in pieces first (k_embed_pieces), so that no thread walks a long run: in
+// ascending position within a piece, the pieces in that order; where they are cut depends on how many labels
+// below it the call has.
 // Few labels at few positions take one launch instead (k_embed_few).
 #include <type_traits>
 
@@ -39,7 +41,7 @@ __host__ __device__ inline int flag_shift(int64_t per) {
 // XCD's L2), counts its own labels and those below its range, and flags the stretches that hold one of
 // its own: only those are read again, to place.  A wave owns a run of positions and a row of counters, so
 // its placing needs no other wave: the order is that of the positions.  Bound by the latency of its passes: 54 us
-// for 65,536 ids of 131,072 labels, 10 for 6,400 of 21.
+// for 65,536 ids of 131,072 labels, 11 for 8,192 of 32,000.
 template <typename ID>
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID *__restrict__ ids, int64_t n, int64_t v, int range,
                                                              int32_t *__restrict__ begin, int32_t *__restrict__ sorted) {
@@ -442,8 +444,8 @@ template <int DT, int kV>
 constexpr auto k_embed_grad_wide = &k_embed_grad<DT, kV, 4>;
 template <int DT, int kV>
 constexpr auto k_embed_grad_narrow = &k_embed_grad<DT, kV, 1>;
-// Four rows per thread where that leaves every CU 512 threads; 6,400 positions into 21 rows of 256 take 36 us
-// so and 29 with one.
+// Four rows per thread where that leaves every CU 512 threads: the pass into 32,000 rows of 512 bfloat16 columns (8,192
+// positions) takes 19 us so and 22 with one, into 21 rows of 256 float32 columns (16,384 positions) 37 and 26.
 bool wide_rows(int64_t v, int64_t groups) { return v * groups >= 4 * 256 * 512; }
 
 // The widest column group that every row of both tensors starts on a multiple of.

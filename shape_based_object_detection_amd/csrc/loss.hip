@@ -890,9 +890,10 @@ __device__ __forceinline__ void multibox_rows(const LossArgs &a, T *__restrict__
       }
       const float zt = row[c];
       float s = 0.f;
-      // focal: the exponentials stay in registers for the gradient (computed once), packed
-      // fp32 for the elementwise steps — this pass is VALU-issue-bound (a v_exp costs 8 cycles
-      // of a wave's issue, a plain or packed op 4), every wave of the round computing at once
+      // focal: the exponentials are kept for the gradient (computed once).  Pairs of slots set the
+      // sums' order; the build has no packed fp32 instructions, so each is two plain ones — this
+      // pass is VALU-issue-bound (a v_exp costs 8 cycles of a wave's issue, a plain op 4), every
+      // wave of the round computing at once
       typedef float f2 __attribute__((ext_vector_type(2)));
       if constexpr (CLS == SBOD_CLS_FOCAL) {
         // the exponentials replace the logits in the LDS row (the gradient pass reads them back:

@@ -646,7 +646,8 @@ __global__ __launch_bounds__(kDTile) void k_det_prepare(DetArgs a, T *__restrict
       m = r[0];
 #pragma unroll
       for (int k = 1; k < KN; ++k) m = fmaxf(m, r[k]);   // NaN rows give NaN probabilities either way
-      // (x - m) * log2(e) two slots per packed op, hardware exp2, pairwise packed sums
+      // (x - m) * log2(e), hardware exp2, sums: two slots at a time (pairs, though the build has no packed fp32
+      // instructions: the sums' order, and so the results, are those of the pairs)
       const f2 nm2 = {-m, -m}, l2 = {1.4426950408889634f, 1.4426950408889634f};
 #pragma unroll
       for (int k = 0; k + 1 < KN; k += 2) {
