@@ -57,6 +57,23 @@ __device__ __forceinline__ void put_row(const DistillArgs &a, int64_t r, double 
   else a.rows[r] = static_cast<float>(loss);
 }
 
+// Where label `id` is in a table of `size` (a power of two, twice the entries at least) that holds -1 or the number
+// of an entry, whose label is ids[entry]: the label's own place, or with kInsert one that now holds `k`.  An open hash:
+// from the label's first place on.  (A row's entries find the repeated ones by it, each in a few steps whatever K.)
+template <bool kInsert>
+__device__ __forceinline__ int find_label(int *table, int size, const int *ids, int id, int k) {
+  int h = static_cast<int>(static_cast<uint32_t>(id) * 2654435761u >> (__clz(size) + 1));
+  for (;; h = (h + 1) & (size - 1)) {
+    const int at = kInsert ? atomicCAS(&table[h], -1, k) : table[h];
+    if ((kInsert && at < 0) || ids[at] == id) return h;
+  }
+}
+__host__ __device__ inline int table_size(int k) {
+  int size = 64;
+  while (size < 2 * k) size *= 2;
+  return size;
+}
+
 // Bits of the kept labels among the elements [e0, e0 + 32 nwords): all threads of the block.
 __device__ __forceinline__ void mark_kept(const DistillArgs &a, int64_t r, int64_t e0, uint32_t *bits, int nwords) {
   for (int i = threadIdx.x; i < nwords; i += blockDim.x) bits[i] = 0;
@@ -210,6 +227,7 @@ template <int DT, bool kBucket>
 __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   using T = typename Elt<DT>::T;
   __shared__ int ids_s[kBucket ? 4 : 1][kBucket ? kMaxTop : 1];
+  extern __shared__ int tables[];   // with a bucket, table_size(K) words for each wave
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   for (int64_t r = blockIdx.x * 4ll + wv; r < a.n; r += gridDim.x * 4ll) {
     float *st = a.stats + r * kStats;
@@ -236,14 +254,18 @@ __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
       }
       m = wave_max_f32(m);
       const float base = m == kNegInf ? 0.f : m;
+      // a label listed twice counts at its first entry
+      const int size = table_size(a.k);
+      int *table = tables + wv * size;
+      for (int i = lane; i < size; i += kWave) table[i] = -1;
+      wave_lds_fence();
+      for (int k = lane; k < a.k; k += kWave)
+        if (ids_s[wv][k] >= 0) atomicMin(&table[find_label<true>(table, size, ids_s[wv], ids_s[wv][k], k)], k);
       wave_lds_fence();
       float sk = 0.f;
       for (int k = lane; k < a.k; k += kWave) {
         const int id = ids_s[wv][k];
-        bool first = id >= 0;   // (no early end: the reads are in flight together)
-#pragma unroll 8
-        for (int j = 0; j < k; ++j) first = first && ids_s[wv][j] != id;
-        if (first) {
+        if (id >= 0 && table[find_label<false>(table, size, ids_s[wv], id, k)] == k) {
           sk += exp2_hw((static_cast<float>(row[id]) - base) * a.s);
           ++kept;
         }
@@ -334,19 +356,25 @@ __global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
 }
 
 // dx of one chunk of a row from the row's statistics.  The kept labels are written a second time,
-// behind a barrier, by a thread each.  The rows are taken from the last to the first: the ones that
-// k_distill_part read last are still in the Infinity Cache (256 MB), and the gradient is stored past it.
+// behind a barrier, by a thread each, the masses of one listed twice added in the list's order.  The rows are
+// taken from the last to the first: the ones that k_distill_part read last are still in the Infinity Cache
+// (256 MB), and the gradient is stored past it.
 // Bound by its read and write: 439 us for 2,048 rows of 131,072 float32 labels (2.15 GB, 4.9 TB/s); from the
 // first row to the last the three kernels take 710 us instead of 690 (256 rows, all in the cache: 95 both ways).
 template <int DT>
 __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   using T = typename Elt<DT>::T;
   constexpr int P = Elt<DT>::P, kPer = kDistGran / kDistThreads;
-  __shared__ int ids_s[kMaxTop];
+  __shared__ int ids_s[kMaxTop], table[2 * kMaxTop];   // the chunk's entries (-1: another chunk's)
   __shared__ float p_s[kMaxTop];
+  __shared__ int some, repeated;   // the last turn whose chunk had an entry, one listed before
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int64_t items = a.n * a.nchunk;
-  for (int64_t at = blockIdx.x; at < items; at += gridDim.x) {
+  const int size = table_size(a.k);
+  if (threadIdx.x == 0) some = repeated = -1;
+  __syncthreads();
+  int turn = 0;
+  for (int64_t at = blockIdx.x; at < items; at += gridDim.x, ++turn) {
     const int64_t it = items - 1 - at, r = it / a.nchunk;
     const T *row = static_cast<const T *>(a.x) + r * a.ldx;
     T *drow = static_cast<T *>(a.dx) + r * a.lddx;
@@ -369,9 +397,11 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
     const float tb = st[kStTb], tl = st[kStTl];
     for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
       const int id = ld_id(a.ids, r * a.k + k, a.ids64, a.v);
-      ids_s[k] = id;
-      p_s[k] = id >= 0 ? expf(static_cast<float>(teacher_logp(a, r * a.k + k, tb, tl))) : 0.f;
+      const bool mine = id >= 0 && id >= e0 && id < e1;
+      ids_s[k] = mine ? id : -1;
+      if (mine) p_s[k] = expf(static_cast<float>(teacher_logp(a, r * a.k + k, tb, tl))), some = turn;
     }
+    for (int i = threadIdx.x; i < size; i += kDistThreads) table[i] = -1;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int64_t e = e0 + static_cast<int64_t>(i * kDistThreads + threadIdx.x) * P;
@@ -381,13 +411,33 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
       st_granule<DT, true>(drow, e, a.v, aligned, f);
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
-      const int id = ids_s[k];
-      if (id < 0 || id < e0 || id >= e1) continue;
-      float p = 0.f;
-      for (int j = 0; j < a.k; ++j) p += ids_s[j] == id ? p_s[j] : 0.f;
-      const float q = exp2_hw((static_cast<float>(row[id]) - st[kStM]) * a.s - st[kStL2s]);
-      drow[id] = static_cast<T>(g * (q - p));
+    if (some == turn) {
+      for (int k = threadIdx.x; k < a.k; k += kDistThreads)
+        if (ids_s[k] >= 0) atomicMin(&table[find_label<true>(table, size, ids_s, ids_s[k], k)], k);
+      __syncthreads();
+      const auto first_of = [&](int k) { return table[find_label<false>(table, size, ids_s, ids_s[k], k)]; };
+      for (int k = threadIdx.x; k < a.k; k += kDistThreads)
+        if (ids_s[k] >= 0 && first_of(k) != k) repeated = turn;
+      __syncthreads();
+      if (repeated == turn) {
+        for (int k0 = 0; k0 < a.k; k0 += kWave) {   // a wave's entries after another's
+          const int k = k0 + (threadIdx.x & 63);
+          if (k0 % kDistThreads / kWave == threadIdx.x / kWave) {
+            const int first = k < a.k && ids_s[k] >= 0 ? first_of(k) : k;
+            for (unsigned long long late = __ballot(first != k); late; late &= late - 1) {
+              if ((threadIdx.x & 63) == __ffsll(late) - 1) p_s[first] += p_s[k];
+              wave_lds_fence();
+            }
+          }
+          __syncthreads();
+        }
+      }
+      for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
+        const int id = ids_s[k];
+        if (id < 0 || (repeated == turn && first_of(k) != k)) continue;
+        const float q = exp2_hw((static_cast<float>(row[id]) - st[kStM]) * a.s - st[kStL2s]);
+        drow[id] = static_cast<T>(g * (q - p_s[k]));
+      }
     }
     __syncthreads();
   }
@@ -647,25 +697,27 @@ constexpr int kSmallBlocks = 1280;
 // of 256 workgroups (324 by the kernels above), and 321 us for 4,096 rows of 50,257 bfloat16 labels, whose 512 threads
 // have one workgroup per CU (162 us of memory; 217 for the pass without a bucket).
 template <int DT, bool kBucket, int NT, int NG>
-__global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
+__global__ __launch_bounds__(NT, NG == 16 ? 4 : 1) void k_distill_row(DistillArgs a) {
   using T = typename Elt<DT>::T;
   constexpr int P = Elt<DT>::P, NW = NT / kWave;
   constexpr uint32_t kInfBits = DT == SBOD_DT_F32 ? 0xff800000u : DT == SBOD_DT_BF16 ? 0xff80u : 0xfc00u;
   // bit e - head + P: element e is kept (head: the elements before the first granule)
   __shared__ uint32_t bits[kBucket ? NT * NG * P / 32 + 1 : 1];
-  __shared__ int ids_s[NT];
+  __shared__ int ids_s[NT], table[2 * NT];   // (find_label: the row's entries)
   __shared__ float top_s[NT], red[2][NW], sums[2][NW];
-  // (1,024 threads have no register to spare beside 16 granules: each one's loss waits in LDS, and its t is read again)
-  constexpr bool kTight = NT == 1024;
+  // (128 registers, four waves per SIMD, have none to spare beside 16 granules: each thread's loss waits in LDS, and its
+  // t is read again)
+  constexpr bool kTight = NG == 16;
   __shared__ double red64[16], masses[NW], losses[kTight ? NT : 1];
-  __shared__ int entered;   // with a bucket: the last row that has an entry (v > kSmallMax: n is below 2^31)
+  __shared__ int entered, repeated;   // the last row that has an entry (with a bucket), one listed before
+                                      // (v > kSmallMax: n is below 2^31)
   if (a.skip_one && *a.up == 1.f) return;   // the forward wrote this very gradient
   const int tid = threadIdx.x, wave = tid >> 6, v = static_cast<int>(a.v), kk = a.k;
-  if (kBucket) {
+  if (kBucket)
     for (int i = tid; i < NT * NG * P / 32 + 1; i += NT) bits[i] = 0;
-    if (tid == 0) entered = -1;
-    __syncthreads();   // (another wave's threads set bits of these words)
-  }
+  table[tid] = table[tid + NT] = -1;
+  if (tid == 0) entered = repeated = -1;
+  __syncthreads();   // (other waves' threads write these words)
   const float norm = a.norm ? *a.norm : static_cast<float>(norm_of(a));
   const float up = a.up && a.up_stride == 0 ? *a.up : 1.f;
   double loss = 0;
@@ -681,8 +733,6 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     const int in = (v - head) / P, tail = v - head - in * P;
     return tid < head ? tid : tid >= P && tid < P + tail ? head + in * P + tid - P : -1;
   };
-  // its byte in `bits`, of the first granule, and where in that
-  const int look = P == 8 ? tid + 1 : (tid + 1) >> 1, shift = 4 * ((tid + 1) & 1);
   // (a granule's address is a scalar base and the thread's own offset, the same for all of them)
   const uint32_t mine = static_cast<uint32_t>(tid) * 16;
   const auto base_of = [&](const T *row, int head) { return reinterpret_cast<const char *>(row + head); };
@@ -746,6 +796,11 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       __syncthreads();
       float x1 = e1 >= 0 ? bits_value<DT>(xraw) : kNegInf;
       if (kBucket && e1 >= 0 && bits[(e1 - head + P) >> 5] >> ((e1 - head + P) & 31) & 1) x1 = kNegInf;
+      // its byte in `bits`, of the first granule, and where in that (made here, not kept from row to row)
+      int look = tid + 1;
+      asm volatile("" : "+v"(look));
+      const int shift = 4 * (look & 1);
+      if (P == 4) look >>= 1;
       mo = x1;
       int left = inner;
 #pragma unroll
@@ -770,6 +825,12 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
 #pragma unroll
         for (int j = 0; j < P; ++j) mo = fmaxf(mo, f[j]);
       }
+      // listed before?  then the label counts at its first entry, and its masses are added in the list's order
+      int h = 0;
+      if (id >= 0) {
+        h = find_label<true>(table, 2 * NT, ids_s, id, tid);
+        atomicMin(&table[h], tid);
+      }
       const float xk = bits_value<DT>(xk_raw);
       float other = id < 0 ? kNegInf : kBucket ? xk : t;   // the kept logits, or the teacher's
       mo = wave_max_f32(mo);
@@ -785,11 +846,10 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       float tl = kBucket ? a.lse[r] : 0.f;
       const auto logp_at = [&](float q) { return static_cast<float>((static_cast<double>(q) - tb) * a.inv_td - tl); };
       const auto p_at = [&](float logp) { return kBucket ? expf(logp) : exp_hw(logp); };
-      // listed before?  then the label counts at its first entry, and its masses are added in the list's order
-      bool first = id >= 0, again = false;
-      if (id >= 0)
-        for (int j = 0; j < kk; ++j)
-          if (j != tid && ids_s[j] == id) again = true, first = first && j > tid;
+      const int entry1 = id >= 0 ? table[h] : tid;   // the label's first entry
+      const bool first = id >= 0 && entry1 == tid;
+      if (entry1 != tid) repeated = static_cast<int>(r);
+      ids_s[tid] = entry1;   // (the labels were read for the last time before the maxima)
       ek = id >= 0 ? exp2_hw((xk - base) * a.s) : 0.f;
       float s1;         // the teacher's normaliser; with a bucket the kept labels' sum,
       double s2 = 0;    // and their mass, in 64 bits (bucket_of)
@@ -827,10 +887,19 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
       coef = inv;
       // (the few kept terms in 64 bits: a label masked by the type's lowest value is a finite loss)
       double kl = pk == 0.f ? 0.0 : pk * (logp_at(kTight ? top_s[tid] : t) - ((static_cast<double>(xk) - base) * a.inv_td - logs));
-      if (again) {
-        pk = 0.f;
-        for (int j = 0; j < kk; ++j)
-          if (ids_s[j] == id) pk += p_at(logp_at(top_s[j]));
+      table[tid] = table[tid + NT] = -1;   // (read for the last time before the sums)
+      if (repeated == static_cast<int>(r)) {
+        top_s[tid] = pk;   // (this thread's own logit is read)
+        __syncthreads();
+        for (int w = 0; w < NW; ++w) {   // a wave's entries after another's
+          if (wave == w)
+            for (unsigned long long late = __ballot(ids_s[tid] != tid); late; late &= late - 1) {
+              if ((tid & 63) == __ffsll(late) - 1) top_s[ids_s[tid]] += pk;
+              wave_lds_fence();
+            }
+          __syncthreads();
+        }
+        pk = top_s[tid];
       }
       if (kBucket) {
         const Bucket b = bucket_of<true>(a, s2, s1, sum, so, mo, base, true);   // (K < V here)
@@ -877,7 +946,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs a) {
     }
     __syncthreads();
     // the kept labels, over what the row's pass wrote there
-    if (a.dx && live && id >= 0) drow[id] = static_cast<T>(g * (ek * inv - pk));
+    if (a.dx && live && id >= 0 && ids_s[tid] == tid) drow[id] = static_cast<T>(g * (ek * inv - pk));
     if (ahead) fetch_rest(rn, next, nhead);
   }
   if (a.parts) {
@@ -910,7 +979,8 @@ template <int DT, bool kBucket>
 int launch_rows(const DistillArgs &a, hipStream_t s) {
   hipLaunchKernelGGL((k_distill_part<DT, kBucket>), dim3(grid_for(a.n * a.nchunk)), dim3(kDistThreads), 0, s, a);
   SBOD_LAUNCHED("k_distill_part");
-  hipLaunchKernelGGL((k_distill_join<DT, kBucket>), dim3(grid_for((a.n + 3) / 4)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((k_distill_join<DT, kBucket>), dim3(grid_for((a.n + 3) / 4)), dim3(256),
+                     kBucket ? 4 * table_size(a.k) * sizeof(int) : 0, s, a);
   SBOD_LAUNCHED("k_distill_join");
   return SBOD_OK;
 }
@@ -947,9 +1017,8 @@ int launch_small(const DistillArgs &a, hipStream_t s) {
   return SBOD_OK;
 }
 
-// Threads and granules of k_distill_row for a row, smallest first, and the workgroups launched at most: what the
-// device holds at once without a bucket (with one, the registers of 16 granules allow 768 and 256 workgroups of the 256
-// and 512 threads).  -1: none, k_distill_part and the kernels behind it.
+// Threads and granules of k_distill_row for a row, smallest first, and the workgroups that the device holds at
+// once.  -1: none, k_distill_part and the kernels behind it.
 struct RowShape {
   int nt, ng, groups;
 };

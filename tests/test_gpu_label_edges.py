@@ -243,3 +243,29 @@ def test_distill_entries_listed_many_times(dt, tail, n, v, k):
         W.check(loss, grad, x, ids, top, lse, None, 1.5, reduction, up)
         again = run_distill(x, ids, top, lse, None, 1.5, reduction, up)
         assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+
+
+@DT
+@TAIL
+@pytest.mark.parametrize('n,v,k', [(5, 2048, 1024), (6, 2049, 1024), (5, 9001, 257), (300, 20001, 513), (5, 61001, 1024), (4, 140001, 1024),
+                                   (3, 140001, 65)])
+@pytest.mark.parametrize('where', ['spread', 'together', 'repeated'])
+def test_distill_most_entries(dt, tail, n, v, k, where):
+    """As many entries as there can be: all over the vocabulary, next to one another (one chunk of a long row has them all), and
+    those with repetitions, the same labels once in ascending and once in descending order."""
+    x, ids, top, lse = W.over_full(n, v, k, dt, dt, 1.5, k) if tail else C.distill_inputs(n, v, k, dt, k)
+    if where != 'spread':
+        ids = (torch.arange(k) + 1000).expand(n, k).contiguous()
+        ids[1::2] = ids[1::2].flip(1)
+    if where == 'repeated':
+        ids[:, k // 2:] -= k // 3
+        ids[2] = 17
+    x, ids, top, lse = dev(x, ids, top, lse)
+    up = torch.rand(n, device=DEV) + 0.5
+    loss, grad = run_distill(x, ids, top, lse, None, 1.5, 'none', up)
+    W.check(loss, grad, x, ids, top, lse, None, 1.5, 'none', up)
+    again = run_distill(x, ids, top, lse, None, 1.5, 'none', up)
+    assert torch.equal(loss, again[0]) and torch.equal(grad, again[1])
+    one = torch.tensor(1.0, device=DEV)
+    loss, grad = run_distill(x, ids, top, lse, None, 1.5, 'mean', one)
+    W.check(loss, grad, x, ids, top, lse, None, 1.5, 'mean', one)
