@@ -88,7 +88,7 @@ __device__ __forceinline__ void mark_kept(const DistillArgs &a, int64_t r, int64
 
 // {max, sum of 2^((x - max) s)} of each chunk of a row; with a bucket, of its labels not kept.  For rows
 // that no workgroup's registers hold: 16 KB per item, so that few long rows fill the device too.  Bound by its
-// one read: 249 us for 2,048 rows of 131,072 float32 labels and a bucket (1.07 GB, 4.3 TB/s).
+// one read: 248 us for 2,048 rows of 131,072 float32 labels and a bucket (1.07 GB, 4.3 TB/s).
 template <int DT, bool kBucket>
 __global__ __launch_bounds__(kDistThreads) void k_distill_part(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -222,7 +222,7 @@ __device__ __forceinline__ double teacher_logp(const DistillArgs &a, int64_t i, 
 }
 
 // One wave per row: the chunks joined, the teacher's side, the row's loss and statistics.  Bound by its chain of
-// loads (ids, then the logits they name): 15 us for 2,048 rows with 64 kept labels and a bucket.
+// loads (ids, then the logits they name): 13 us for 2,048 rows with 64 kept labels and a bucket.
 template <int DT, bool kBucket>
 __global__ __launch_bounds__(256) void k_distill_join(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -359,8 +359,8 @@ __global__ __launch_bounds__(1024) void k_distill_sum(DistillArgs a) {
 // behind a barrier, by a thread each, the masses of one listed twice added in the list's order.  The rows are
 // taken from the last to the first: the ones that k_distill_part read last are still in the Infinity Cache
 // (256 MB), and the gradient is stored past it.
-// Bound by its read and write: 439 us for 2,048 rows of 131,072 float32 labels (2.15 GB, 4.9 TB/s); from the
-// first row to the last the three kernels take 710 us instead of 690 (256 rows, all in the cache: 95 both ways).
+// Bound by its read and write: 404 us for 2,048 rows of 131,072 float32 labels (2.15 GB, 5.3 TB/s); from the
+// first row to the last 20 more (256 rows, all in the cache: the same both ways).
 template <int DT>
 __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistillArgs a) {
   using T = typename Elt<DT>::T;
@@ -691,11 +691,10 @@ constexpr int kSmallBlocks = 1280;
 // has kept entry k (K <= NT).  The elements before the row's first 16-byte boundary and behind its last
 // granule are one value each of the first 2 P threads.
 // With a bucket the kept labels leave the registers by a bit each in LDS, looked up a granule at a time.
-// Bound by memory: 484 to 512 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.3 TB/s of the 5.07 that a copy
-// reaches; 708 with a pass each for statistics and gradient), 566 with a bucket.  With a bucket the reductions of the one
-// row that a CU holds are not under another row's traffic: 255 us for 2,049 rows of 50,001 float32 labels, in nine rounds
-// of 256 workgroups (324 by the kernels above), and 321 us for 4,096 rows of 50,257 bfloat16 labels, whose 512 threads
-// have one workgroup per CU (162 us of memory; 217 for the pass without a bucket).
+// Bound by memory: 490 to 512 us for 4,096 rows of 131,072 bfloat16 labels (2.15 GB, 4.3 TB/s of the 5.07 that a copy
+// reaches; 708 with a pass each for statistics and gradient), 552 with a bucket.  211 us for 2,049 rows of 50,001
+// float32 labels and a bucket (162 us of memory), in nine rounds of 256 workgroups, the last of one row; 204 us for 4,096
+// rows of 50,257 bfloat16 labels, 221 with a bucket (162 of memory).
 template <int DT, bool kBucket, int NT, int NG>
 __global__ __launch_bounds__(NT, NG == 16 ? 4 : 1) void k_distill_row(DistillArgs a) {
   using T = typename Elt<DT>::T;
