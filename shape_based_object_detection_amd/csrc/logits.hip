@@ -34,7 +34,7 @@ struct LogitsArgs {
   float rep_s, pres_s, freq_s;
 };
 
-// A touched label's value but for its mask: x with the history's word of it, its bias and its listed bias.
+// A touched label's value but for its mask: x with the history's word of it, its bias and its listed biases' sum.
 template <int kBias>
 __device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int v, float x, uint32_t word, float listed,
                                         float rep, float pres, float freq) {
@@ -44,15 +44,7 @@ __device__ __forceinline__ float adjust(const LogitsArgs &a, int64_t r, int v, f
     if (answered) x = x - freq * static_cast<float>(answered) - pres;   // (an infinite penalty times 0 is NaN)
   }
   if (kBias >= 0) x += ld_any(a.bias, r * a.ldb + v, kBias);
-  if (word & kTwice) {   // in the order listed
-    float s = 0.f;
-    for (int i = 0; i < a.m; ++i)
-      if (ld_id(a.bias_ids, r * a.ldi + i, a.ids64, a.v) == v) s += a.bias_val[r * a.ldv + i];
-    x += s;
-  } else if (word & kBiased) {
-    x += listed;
-  }
-  return x;
+  return word & kBiased ? x + listed : x;
 }
 
 // P biases of type BT of the labels [e, e + P), all inside the row: in flight until bias_values.
@@ -102,29 +94,88 @@ __device__ __forceinline__ uint32_t mask_of(const LogitsArgs &a, int64_t r, int6
   return ~0u;
 }
 
+// A value made where it is used: what is computed from it is not kept in registers from item to item.
+__device__ __forceinline__ int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Elements of the list of listed labels: with room for a float for every two of m.
+__host__ __device__ inline int list_size(int tile, int m) { return m > tile ? (m + 31) / 32 * 32 : tile; }
+
+// The listed biases of a tile's labels that are listed twice (bits in `repeated`), each label's added to its place in
+// `sums` (floats) in the order listed.  All threads: a wave has the places of its number modulo the waves, and reads the
+// whole list, 64 entries at a time: one row of 32,000 labels and 4,096 listed biases takes 12 us, 26 where one label is
+// listed twice, 100 where they are all of one.
+__device__ __forceinline__ void sum_repeated(const LogitsArgs &a, int64_t r, int64_t e0, uint32_t *sums, const uint32_t *repeated) {
+  const int me = here(threadIdx.x), lane = me & 63, wave = __builtin_amdgcn_readfirstlane(me >> 6), waves = blockDim.x >> 6;
+  const auto one = [](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
+  const auto id_at = [&](int i) { return ld_raw_id(a.bias_ids, r * a.ldi + min(i, a.m - 1), a.ids64); };
+  const auto value_at = [&](int i) { return a.bias_val[r * a.ldv + min(i, a.m - 1)]; };
+  RawId next = id_at(lane);
+  float next_value = value_at(lane);
+  for (int i = lane; i - lane < a.m; i += kWave) {
+    const int id = i < a.m ? id_of(next, a.ids64, a.v) : -1;
+    const float value = next_value;
+    next = id_at(i + kWave), next_value = value_at(i + kWave);
+    const int64_t off = id - e0;
+    const int at = id >= 0 && off >= 0 && off < a.tile ? static_cast<int>(off) : 0;
+    const bool mine = id >= 0 && off == at && (at & (waves - 1)) == wave && (repeated[at >> 5] >> (at & 31) & 1);
+    unsigned long long todo = __ballot(mine), same = todo;   // same: the lanes that have this one's label
+    if (todo == 0) continue;
+    for (int b = 0; 1 << b < a.tile; ++b) {
+      const unsigned long long set = __ballot(at >> b & 1);
+      same &= at >> b & 1 ? set : ~set;
+    }
+    const bool alone = mine && (same & (same - 1)) == 0;
+    if (alone) sums[at] = __float_as_uint(__uint_as_float(sums[at]) + value);
+    for (todo &= ~__ballot(alone); todo;) {   // a label's lanes one after another
+      const int from = __ffsll(todo) - 1, to = one(at, from);
+      unsigned long long group = static_cast<uint32_t>(one(static_cast<int>(same >> 32), from));
+      group = group << 32 | static_cast<uint32_t>(one(static_cast<int>(same), from));
+      todo &= ~group;
+      float sum = __uint_as_float(sums[to]);
+      if (group == ~0ull) {   // (lists filled up with one label: each lane's number is in the instruction)
+#pragma unroll
+        for (int l = 0; l < kWave; ++l) sum += __int_as_float(one(__float_as_int(value), l));
+      } else {
+        for (; group; group &= group - 1) sum += __int_as_float(one(__float_as_int(value), __ffsll(group) - 1));
+      }
+      if (lane == from) sums[to] = __float_as_uint(sum);
+    }
+    wave_lds_fence();
+  }
+}
+
 // An item is a row's tile of up to kLogTile labels.  Its logits are on their way while the history is read:
 // the answers' counts go to a table of the tile in LDS (integer atomics), the first touch of a label puts it
 // on a list, and the first of its listed biases' threads owns it.  Each touched label is then computed by one
 // thread, its value taking its word's place in the table, and the tile passes through registers once, the
-// touched labels (a bit each) from the table.  What bounds it is the chain of those steps at the workgroups
-// that a CU's LDS holds (three): loads are asked for before the step that they wait behind.  55 us for 256 rows of
-// 131,072 bfloat16 labels with up to 4,096 entries, 300 listed biases and a bit mask (142 MB: 2.6 TB/s); without
-// history and biases 29.  One row of 32,000 float32 labels: 6.5 us.  Every tile reads its row's whole history, one row of
+// touched labels (a bit each) from the table.  Labels with two listed biases or more are written again behind
+// that, when the registers are free (sum_repeated).  What bounds it is the chain of those steps at the workgroups
+// that a CU's LDS holds (three): loads are asked for before the step that they wait behind.  53 us for 256 rows of
+// 131,072 bfloat16 labels with up to 4,096 entries, 300 listed biases and a bit mask (142 MB: 2.7 TB/s); without
+// history and biases 29.  One row of 32,000 float32 labels: 6 us.  Every tile reads its row's whole history, one row of
 // 131,072 labels takes 7 us with 4,096 entries, 80 with 131,072 and 470 with 1,048,576.
 template <int DT, int kMask, int kBias>
 __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
   using T = typename Elt<DT>::T;
   constexpr int BT = kBias < 0 ? SBOD_DT_F32 : kBias;
   constexpr int P = Elt<DT>::P, kPer = kLogTile / P / kLogThreads;
-  extern __shared__ __attribute__((aligned(16))) uint32_t table[];   // [a.tile] words, then values; [a.tile] listed labels; twice [a.tile] bits
-  __shared__ int listed;
+  // [a.tile] words, then values; [a.tile] listed labels; twice [a.tile] bits; [a.m / 2] words and labels of the labels
+  // with two listed biases.  Their logits take the list's place (list_size)
+  extern __shared__ __attribute__((aligned(16))) uint32_t table[];
+  __shared__ int listed, repeats;
   uint16_t *list = reinterpret_cast<uint16_t *>(table + a.tile);
-  uint8_t *touched = reinterpret_cast<uint8_t *>(list + a.tile);
+  uint8_t *touched = reinterpret_cast<uint8_t *>(list + list_size(a.tile, a.m));
   uint32_t *owned = reinterpret_cast<uint32_t *>(touched + a.tile / 8);   // labels with a listed bias
-  const int nt = blockDim.x, lane = threadIdx.x;
+  uint32_t *words = owned + a.tile / 32;
+  uint16_t *places = reinterpret_cast<uint16_t *>(words + a.m / 2);
+  const int nt = blockDim.x;
   const int64_t items = a.n * a.ntile;
   const bool build = a.len > 0 || a.m > 0;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int lane = here(threadIdx.x);
     // (a row's tiles one after another, on different XCDs: on one XCD they wait for the same lines of the row's
     // history, 76 against 61 us for 256 rows of 131,072 labels with up to 4,096 entries)
     const int64_t r = it / a.ntile, t = it - r * a.ntile;
@@ -166,7 +217,7 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
                   freq = a.freq ? a.freq[r] : a.freq_s;
       for (int i = lane; i < a.tile / 4; i += nt) reinterpret_cast<raw16_t *>(table)[i] = raw16_t{0, 0, 0, 0};
       for (int i = lane; i < a.tile / 16; i += nt) reinterpret_cast<uint32_t *>(touched)[i] = 0;   // (owned with it)
-      if (lane == 0) listed = 0;
+      if (lane == 0) listed = repeats = 0;
       if (a.hist_len) len = min(len, static_cast<int64_t>(max(lim, 0)));
       const auto place = [&](int label) {   // in the tile, or -1
         const int64_t at = label - e0;
@@ -200,7 +251,7 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
         const int at = biased(i);
         if (at < 0) continue;
         if (atomicOr(&table[at], kBiased) & kBiased) {
-          atomicOr(&table[at], kTwice);
+          if (!(atomicOr(&table[at], kTwice) & kTwice)) places[atomicAdd(&repeats, 1)] = static_cast<uint16_t>(at);
         } else {
           own |= 1u << c;
           mark(at);
@@ -209,7 +260,9 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
       }
       __syncthreads();
       const auto settle = [&](int at, float x, float bias) {
-        x = adjust<kBias>(a, r, static_cast<int>(e0 + at), x, table[at], bias, rep, pres, freq);
+        const uint32_t word = table[at];
+        if (word & kTwice) return;   // (below)
+        x = adjust<kBias>(a, r, static_cast<int>(e0 + at), x, word, bias, rep, pres, freq);
         table[at] = __float_as_uint(x);
       };
       for (int i = lane; i < listed; i += nt) {
@@ -220,6 +273,10 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
       for (int i = lane + nt, c = 1; i < a.m; i += nt, ++c)
         if (own >> c & 1) settle(biased(i), static_cast<float>(row[e0 + biased(i)]), a.bias_val[r * a.ldv + i]);
       __syncthreads();
+      if (repeats > 0) {   // (a.m / 2 at most; `out` may be the logits)
+        for (int i = lane; i < repeats; i += nt) reinterpret_cast<float *>(list)[i] = static_cast<float>(row[e0 + places[i]]);
+        __syncthreads();
+      }
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -259,7 +316,31 @@ __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
         }
       }
     }
-    if (build) __syncthreads();
+    if (build) {
+      __syncthreads();
+      if (repeats > 0) {
+        for (int i = lane; i < a.tile / 32; i += nt) owned[i] = 0;
+        __syncthreads();
+        for (int i = lane; i < repeats; i += nt) {
+          const int at = places[i];
+          words[i] = table[at], table[at] = 0;   // (0.f)
+          atomicOr(&owned[at >> 5], 1u << (at & 31));
+        }
+        __syncthreads();
+        sum_repeated(a, r, e0, table, owned);
+        __syncthreads();
+        const float rep = a.rep ? a.rep[r] : a.rep_s, pres = a.pres ? a.pres[r] : a.pres_s, freq = a.freq ? a.freq[r] : a.freq_s;
+        for (int i = lane; i < repeats; i += nt) {
+          const int at = places[i];
+          const int64_t v = e0 + at;
+          float x = adjust<kBias>(a, r, static_cast<int>(v), reinterpret_cast<float *>(list)[i], words[i],
+                                  __uint_as_float(table[at]), rep, pres, freq);
+          if (forbidden<kMask>(a, r, v)) x = -__builtin_inff();
+          orow[v] = static_cast<T>(x);
+        }
+        __syncthreads();
+      }
+    }
   }
 }
 
@@ -322,7 +403,9 @@ extern "C" int sbod_logits_process(const void *logits, int dtype, int64_t n, int
   const dim3 block(a.tile <= 1024 ? 128 : a.tile <= kLogTile / 2 ? 256 : kLogThreads);
   const int64_t items = n * a.ntile;
   const dim3 grid(static_cast<unsigned>(items < 65536 ? items : 65536));
-  const size_t lds = a.len > 0 || a.m > 0 ? a.tile * (sizeof(uint32_t) + sizeof(uint16_t)) + a.tile / 4 : 0;
+  const size_t lds = a.len > 0 || a.m > 0 ? a.tile * sizeof(uint32_t) + list_size(a.tile, a.m) * sizeof(uint16_t) + a.tile / 4 +
+                                                a.m / 2 * (sizeof(uint32_t) + sizeof(uint16_t))
+                                          : 0;   // (62 KB at most)
   hipStream_t s = as_stream(stream);
   if (dtype == SBOD_DT_F32) launch_logits<SBOD_DT_F32>(a, grid, block, lds, s);
   else if (dtype == SBOD_DT_BF16) launch_logits<SBOD_DT_BF16>(a, grid, block, lds, s);

@@ -2,6 +2,7 @@
 import gc
 import math
 
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -10,6 +11,7 @@ import label_cases as C
 import label_wide as W
 import test_gpu_label_ops as G
 import test_label_edges as E
+from oracle import label_ref as R
 from shape_based_object_detection_amd import _lib as L
 from shape_based_object_detection_amd.operators.Embedding import scaled_embedding
 from shape_based_object_detection_amd.operators.Logits import process_logits
@@ -269,3 +271,54 @@ def test_distill_most_entries(dt, tail, n, v, k, where):
     one = torch.tensor(1.0, device=DEV)
     loss, grad = run_distill(x, ids, top, lse, None, 1.5, 'mean', one)
     W.check(loss, grad, x, ids, top, lse, None, 1.5, 'mean', one)
+
+
+# ------------------------------------------------------------------------------------------------ repeated listed biases
+def in_order(x, ids, values, bias=None):
+    """float32: x + bias, + the sum of each label's listed biases, added one by one in the order listed."""
+    n, v = x.shape
+    s, listed, row = np.zeros((n, v), np.float32), np.zeros((n, v), bool), np.arange(n)
+    ids, values = np.broadcast_to(ids.numpy(), (n, ids.shape[-1])), np.broadcast_to(values.numpy(), (n, values.shape[-1]))
+    for i in range(ids.shape[1]):
+        ok = (ids[:, i] >= 0) & (ids[:, i] < v)
+        s[row[ok], ids[ok, i]] += values[ok, i]
+        listed[row[ok], ids[ok, i]] = True
+    x = x.float().numpy() + (0 if bias is None else bias.float().numpy())
+    return torch.from_numpy(np.where(listed, x + s, x).astype(np.float32))
+
+
+@DT
+@pytest.mark.parametrize('n,v,m', [(3, 1, 7), (5, 21, 300), (4, 1000, 4096), (2, 8193, 600), (3, 9000, 4095), (2, 32000, 4096),
+                                   (70, 131072, 300)])
+@pytest.mark.parametrize('kind', ['random', 'few', 'one', 'shared'])
+def test_logits_listed_biases_many_times(dt, n, v, m, kind):
+    """Labels listed many times, their biases added in the order listed, to the last bit; beside masks, a dense bias and in place."""
+    g = torch.Generator().manual_seed(n + v + m)
+    x = (torch.randn(n, v, generator=g) * 3).to(dt)
+    ids = torch.randint(-1, v + 1, (m,) if kind == 'shared' else (n, m), generator=g)
+    if kind in ('few', 'shared'):
+        ids = ids % max(m // 8, 1)
+    if kind == 'one':
+        ids[:] = v // 2
+    values = torch.randn(ids.shape, generator=g) * torch.rand(ids.shape, generator=g).exp()
+    dense = torch.randn(v, generator=g)
+    ok = torch.rand(n, v, generator=g) < 0.6
+    xd, idd, vd = dev(x, ids.int() if kind == 'few' else ids, values)
+    want = in_order(x, ids, values)
+    assert torch.equal(process_logits(xd, bias_ids=idd, bias_values=vd).cpu(), want.to(dt))
+    want = in_order(x, ids, values, dense).masked_fill(~ok, -math.inf).to(dt)
+    for allowed in (ok, G.words_of(ok)):
+        there = xd.clone()
+        got = process_logits(there, bias=dense.to(DEV), bias_ids=idd, bias_values=vd, allowed=allowed.to(DEV), out=there)
+        assert torch.equal(got.cpu(), want)
+    hist = torch.randint(0, v, (n, 50), generator=g)
+    hist[:, ::2] = ids[..., :25].clamp(0, v - 1) if m >= 25 else 0
+    prompt = torch.randint(0, 50, (n,), generator=g)
+    oracle, mag = R.process_logits(x.double().numpy(), hist.numpy(), None, prompt.numpy(), 1.5, 0.5, 0.25, None,
+                                   ids.expand(n, m).numpy(), values.expand(n, m).numpy(), ok.numpy()) if n < 10 else (None, None)
+    got = process_logits(xd, hist.to(DEV), prompt_len=prompt.to(DEV), repetition=1.5, presence=0.5, frequency=0.25,
+                         bias_ids=idd, bias_values=vd, allowed=ok.to(DEV))
+    if oracle is not None:
+        C.check_logits(got, oracle, mag, dt, 3 + m)
+    assert torch.equal(got, process_logits(xd.clone(), hist.to(DEV), prompt_len=prompt.to(DEV), repetition=1.5, presence=0.5,
+                                           frequency=0.25, bias_ids=idd, bias_values=vd, allowed=ok.to(DEV)))
