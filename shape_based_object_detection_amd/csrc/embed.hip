@@ -41,7 +41,7 @@ __host__ __device__ inline int flag_shift(int64_t per) {
 // XCD's L2), counts its own labels and those below its range, and flags the stretches that hold one of
 // its own: only those are read again, to place.  A wave owns a run of positions and a row of counters, so
 // its placing needs no other wave: the order is that of the positions.  Bound by the latency of its passes: 54 us
-// for 65,536 ids of 131,072 labels, 11 for 8,192 of 32,000.
+// for 65,536 ids of 131,072 labels, 11 for 8,192 of 32,000; its reads grow as ids times labels above 131,072 labels.
 template <typename ID>
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const ID *__restrict__ ids, int64_t n, int64_t v, int range,
                                                              int32_t *__restrict__ begin, int32_t *__restrict__ sorted) {

@@ -156,7 +156,7 @@ __device__ __forceinline__ void sum_repeated(const LogitsArgs &a, int64_t r, int
 // that a CU's LDS holds (three): loads are asked for before the step that they wait behind.  53 us for 256 rows of
 // 131,072 bfloat16 labels with up to 4,096 entries, 300 listed biases and a bit mask (142 MB: 2.7 TB/s); without
 // history and biases 29.  One row of 32,000 float32 labels: 6 us.  Every tile reads its row's whole history, one row of
-// 131,072 labels takes 7 us with 4,096 entries, 80 with 131,072 and 470 with 1,048,576.
+// 131,072 labels takes 7 us with 4,096 entries, 77 with 131,072 and 445 with 1,048,576.
 template <int DT, int kMask, int kBias>
 __global__ __launch_bounds__(kLogThreads) void k_logits(LogitsArgs a) {
   using T = typename Elt<DT>::T;
