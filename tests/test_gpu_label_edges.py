@@ -322,3 +322,57 @@ def test_logits_listed_biases_many_times(dt, n, v, m, kind):
         C.check_logits(got, oracle, mag, dt, 3 + m)
     assert torch.equal(got, process_logits(xd.clone(), hist.to(DEV), prompt_len=prompt.to(DEV), repetition=1.5, presence=0.5,
                                            frequency=0.25, bias_ids=idd, bias_values=vd, allowed=ok.to(DEV)))
+
+
+# ------------------------------------------------------------------------------------------------ captured
+@DT
+def test_captured_steps_with_repeated_labels_equal_eager(dt):
+    """One graph over the forms that a row's repetitions and a table's size choose, replayed on new inputs with eager work and
+    synchronisations between the replays."""
+    shapes = ((30, 90, 12), (9, 700, 100), (7, 9001, 60), (3, 140001, 40))
+    sets = [[torch.zeros(n, v, dtype=dt, device=DEV), torch.zeros(n, k, dtype=torch.int64, device=DEV),
+             torch.zeros(n, k, dtype=dt, device=DEV), torch.zeros(n, device=DEV)] for n, v, k in shapes]
+    ids, go = torch.zeros(300, dtype=torch.int64, device=DEV), torch.zeros(300, 64, dtype=dt, device=DEV)
+    x, bi, bv = torch.zeros(3, 9001, dtype=dt, device=DEV), torch.zeros(3, 600, dtype=torch.int64, device=DEV), torch.zeros(3, 600, device=DEV)
+    table, up = torch.randn(21, 64, device=DEV).to(dt), torch.tensor(3.0, device=DEV)
+
+    def step():
+        got = []
+        for s in sets:
+            for lse in (None, s[3]):
+                loss, grad = run_distill(*s[:3], lse, None, 1.5, 'mean', up)
+                got += [loss.detach(), grad]
+        w = table.detach().requires_grad_(True)
+        got += torch.autograd.grad(scaled_embedding(ids, w, 2.0), w, go)
+        return got + [process_logits(x, bi[:, :50], bias_ids=bi, bias_values=bv, presence=0.5)]
+
+    def fill(seed):
+        for s, (n, v, k) in zip(sets, shapes):
+            a = W.over_full(n, v, k, dt, dt, 1.5, seed + k)
+            a[1][:, seed % k] = a[1][:, (seed + 1) % k]
+            for t, b in zip(s, a):
+                t.copy_(b)
+        g = torch.Generator().manual_seed(seed)
+        ids.copy_(torch.randint(-1, 21, (300,), generator=g))
+        go.copy_(torch.randn(300, 64, generator=g))
+        x.copy_(torch.randn(3, 9001, generator=g))
+        bi.copy_(torch.randint(0, 200 * seed + 1, (3, 600), generator=g))
+        bv.copy_(torch.randn(3, 600, generator=g))
+
+    fill(1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step()
+    for seed in (2, 3, 0, 4):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
