@@ -483,13 +483,15 @@ int sbod_map_f32(const float *det_boxes, const int64_t *det_labels, const float 
  * whose logits are all -inf gives loss 0 and a zero gradient, whatever else it holds.
  *   rows [N] (reduction NONE): the row losses; loss, norm [1] (MEAN, SUM): the reduced loss and the factor
  *   on each row's gradient (1 / sum of weights, 1 / N or 1; MEAN over weights that sum to 0 gives 0);
- *   stats [sbod_distill_stat_floats(), per row]: kept for the gradient.
+ *   stats: kept for the gradient, sbod_distill_stats_bytes (0 where it needs none: rows that registers hold; at most
+ *   sbod_distill_stat_floats() per row).
  * fwd with grad != NULL (a reduction) also writes the gradient at upstream 1; bwd computes it for
  * upstream [1] (a reduction) or [N] (NONE), and with skip_if_one != 0 leaves grad as it is where
  * *upstream is 1 (grad then holds what fwd wrote). */
 enum { SBOD_REDUCE_NONE = 0, SBOD_REDUCE_MEAN = 1, SBOD_REDUCE_SUM = 2 };
 int sbod_distill_stat_floats(void);
 size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int dtype);
+size_t sbod_distill_stats_bytes(int64_t n, int64_t v, int k, int dtype);
 int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids, int ids64,
                      const void *top, int top_dtype, int k, const float *lse, const float *weights,
                      float temperature, int reduction, float *rows, float *loss, float *norm, float *stats,

@@ -87,6 +87,7 @@ SIGNATURES = {
                                P, SZ, P]),
     'sbod_distill_stat_floats': (I32, []),
     'sbod_distill_workspace_bytes': (SZ, [I64, I64, I32, I32]),
+    'sbod_distill_stats_bytes': (SZ, [I64, I64, I32, I32]),
     'sbod_distill_fwd': (I32, [P, I32, I64, I64, I64, P, I32, P, I32, I32, P, P, F32, I32, P, P, P, P, P, I64, P,
                                SZ, P]),
     'sbod_distill_bwd': (I32, [P, I32, I64, I64, I64, P, I32, P, I32, I32, P, P, F32, I32, P, P, P, I32, P, I64, P]),

@@ -1306,9 +1306,9 @@ class _TopKDistill(torch.autograd.Function):
         n, v = x.shape
         dev = x.device
         dt, red = L.LABEL_DT[x.dtype], L.REDUCE[reduction]
-        nst = L.lib().sbod_distill_stat_floats()
+        nst = L.lib().sbod_distill_stats_bytes(n, v, top.shape[1], dt) // 4
         nb = L.lib().sbod_distill_workspace_bytes(n, v, top.shape[1], dt)
-        kept = torch.empty(nst * n + 1, dtype=torch.float32, device=dev)   # statistics | the reduction's norm
+        kept = torch.empty(nst + 1, dtype=torch.float32, device=dev)   # statistics | the reduction's norm
         loss = torch.empty((), dtype=torch.float32, device=dev) if red else None
         rows = None if red else torch.empty(n, dtype=torch.float32, device=dev)
         grad = _empty_rows(x) if want and red and x.dtype != torch.float16 else None
@@ -1316,7 +1316,7 @@ class _TopKDistill(torch.autograd.Function):
         args = (dt, n, v, _row_stride(x), L.ptr(ids), int(ids.dtype == torch.int64), L.ptr(top), L.LABEL_DT[top.dtype],
                 top.shape[1], L.ptr(lse), L.ptr(w), temperature, red)
         with _on_device(x):
-            L.call('sbod_distill_fwd', L.ptr(x), *args, L.ptr(rows), L.ptr(loss), kept.data_ptr() + 4 * nst * n,
+            L.call('sbod_distill_fwd', L.ptr(x), *args, L.ptr(rows), L.ptr(loss), kept.data_ptr() + 4 * nst,
                    L.ptr(kept), L.ptr(grad), 0 if grad is None else _row_stride(grad), L.ptr(ws), nb, L.stream_of(x))
         if want:
             ctx.save_for_backward(x, ids, top, lse, w, kept)

@@ -1114,6 +1114,11 @@ extern "C" size_t sbod_distill_workspace_bytes(int64_t n, int64_t v, int k, int 
   return chunks_offset(n, v, k, dtype) + chunks;
 }
 
+extern "C" size_t sbod_distill_stats_bytes(int64_t n, int64_t v, int k, int dtype) {
+  if (n < 0 || v <= 0 || k <= 0 || k > kMaxTop || !known_dt(dtype) || path_of(v, k, dtype) != kChunks) return 0;
+  return static_cast<size_t>(n) * kStats * sizeof(float);
+}
+
 extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_t v, int64_t ld, const void *ids,
                                 int ids64, const void *top, int top_dtype, int k, const float *lse,
                                 const float *weights, float temperature, int reduction, float *rows, float *loss,
@@ -1121,7 +1126,8 @@ extern "C" int sbod_distill_fwd(const void *logits, int dtype, int64_t n, int64_
                                 void *stream) {
   const int bad = check_common("sbod_distill_fwd", logits, dtype, n, v, ld, ids, top, top_dtype, k, temperature, reduction);
   if (bad != SBOD_OK) return bad;
-  SBOD_REQUIRE(n == 0 || ((rows || reduction != SBOD_REDUCE_NONE) && stats), "sbod_distill_fwd: null output");
+  SBOD_REQUIRE(n == 0 || ((rows || reduction != SBOD_REDUCE_NONE) && (stats || sbod_distill_stats_bytes(n, v, k, dtype) == 0)),
+               "sbod_distill_fwd: null output");
   SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || (loss && norm), "sbod_distill_fwd: a reduction needs loss and norm");
   SBOD_REQUIRE(!grad || (grad_ld >= v && reduction != SBOD_REDUCE_NONE), "sbod_distill_fwd: gradient with row stride %lld, reduction %d",
                static_cast<long long>(grad_ld), reduction);
@@ -1166,7 +1172,8 @@ extern "C" int sbod_distill_bwd(const void *logits, int dtype, int64_t n, int64_
   const int bad = check_common("sbod_distill_bwd", logits, dtype, n, v, ld, ids, top, top_dtype, k, temperature, reduction);
   if (bad != SBOD_OK) return bad;
   if (n == 0) return SBOD_OK;
-  SBOD_REQUIRE(stats && grad && upstream && grad_ld >= v, "sbod_distill_bwd: null tensor or row stride %lld",
+  SBOD_REQUIRE((stats || sbod_distill_stats_bytes(n, v, k, dtype) == 0) && grad && upstream && grad_ld >= v,
+               "sbod_distill_bwd: null tensor or row stride %lld",
                static_cast<long long>(grad_ld));
   SBOD_REQUIRE(reduction == SBOD_REDUCE_NONE || norm, "sbod_distill_bwd: a reduction needs the forward's norm");
   SBOD_REQUIRE(!skip_if_one || reduction != SBOD_REDUCE_NONE, "sbod_distill_bwd: skip_if_one needs a reduction");

@@ -104,11 +104,12 @@ struct DistillCall {
 
 struct DistillFn : public torch::autograd::Function<DistillFn> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, DistillCall *c) {
-    const int64_t n = x.size(0), v = x.size(1), nst = sbod_distill_stat_floats();
+    const int64_t n = x.size(0), v = x.size(1);
     const int k = static_cast<int>(c->top.size(1));
+    const int64_t nst = sbod_distill_stats_bytes(n, v, k, c->dt) / sizeof(float);
     const size_t nb = sbod_distill_workspace_bytes(n, v, k, c->dt);
     const auto f32 = x.options().dtype(at::kFloat);
-    at::Tensor kept = at::empty({nst * n + 1}, f32), ws = at::empty({static_cast<int64_t>(nb)}, x.options().dtype(at::kByte));
+    at::Tensor kept = at::empty({nst + 1}, f32), ws = at::empty({static_cast<int64_t>(nb)}, x.options().dtype(at::kByte));
     const bool red = c->reduction != SBOD_REDUCE_NONE;
     at::Tensor out = red ? at::empty({}, f32) : at::empty({n}, f32), grad;
     // (float16 gradients at upstream 1 would underflow before a loss scale reaches them)
@@ -118,7 +119,7 @@ struct DistillFn : public torch::autograd::Function<DistillFn> {
                                  c->ids.scalar_type() == at::kLong, c->top.data_ptr(), c->top_dt, k,
                                  static_cast<float *>(ptr_of(c->lse)), static_cast<float *>(ptr_of(c->w)), c->temperature,
                                  c->reduction, red ? nullptr : out.data_ptr<float>(), red ? out.data_ptr<float>() : nullptr,
-                                 stats + nst * n, stats, ptr_of(grad), grad.defined() ? row_stride(grad) : 0, ws.data_ptr(), nb,
+                                 stats + nst, stats, ptr_of(grad), grad.defined() ? row_stride(grad) : 0, ws.data_ptr(), nb,
                                  c->stream);
     if (c->want) {
       ctx->save_for_backward({x, c->ids, c->top, c->lse, c->w, kept});

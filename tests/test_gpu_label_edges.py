@@ -376,3 +376,25 @@ def test_captured_steps_with_repeated_labels_equal_eager(dt):
         want = step()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------ what a loss keeps
+@pytest.mark.parametrize('native', [True, False])
+def test_distill_keeps_statistics_only_for_rows_that_need_them(native, monkeypatch):
+    """From forward to backward: float16 logits keep no gradient, and rows that registers hold no statistics either."""
+    L.lib()
+    if not native:
+        monkeypatch.setattr(L, 'host_ext', None)
+    for n, v, stats in ((100000, 21, 0), (1000, 5000, 0), (64, 140001, 64 * 32)):
+        x, ids, top, lse = dev(*C.distill_inputs(n, v, 5, torch.float16, 1, True))
+        x.requires_grad_(True)
+        topk_distill_loss(x, ids, top, lse)
+        gc.collect()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = topk_distill_loss(x, ids, top, lse)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() - before <= 2048 + stats   # (two small blocks of 512 bytes, and rounding)
+        grad, = torch.autograd.grad(loss, x)
+        C.check_distill(loss, grad, x, ids, top, lse, None, 1.0, 'mean') if n < 100 else None
+        del loss, grad
